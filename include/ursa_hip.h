@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define URSA_ABI_VERSION 8
+#define URSA_ABI_VERSION 9
 
 typedef void* ursa_stream_t; /* hipStream_t */
 
@@ -624,6 +624,70 @@ int ursa_fc_ce_f32(const float* pooled, const float* W, const float* b /* or NUL
                    int64_t ignore_index, ursa_stream_t stream);
 int ursa_bn_relu_pool_bwd_f32(const float* z, const float* dpooled, const float* gamma, const float* save /* [4][C] */, float* dz,
                               float* dgamma, float* dbeta, int64_t N, int64_t C, int64_t HW, ursa_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * K15  the linear layer with its epilogue          y = act(x W' + b) + r       (and its gradients)
+ *
+ *   x [M][K], w [N][K], bias [N] or NULL, residual [M][N] or NULL, y [M][N]: contiguous, one element type (`dtype`), pointers
+ *   aligned to an element. z [M][N] or NULL receives x W' + b, rounded to the type, for the backward pass. Sums are fp32; the
+ *   activation sees the sum before it is rounded. fp32 operands are multiplied as three bf16 numbers each (exact split, products
+ *   down to 2^-24 of |x w|): a non-finite one gives NaN in every sum that it enters.
+ *   ursa_linear_act_grad   dz = dy act'(z) (act != URSA_ACT_NONE: z and dz given) and db = its column sums (fp32 before dz is
+ *                          rounded; db NULL: not wanted). act == URSA_ACT_NONE: z, dz NULL, db = column sums of dy.
+ *   ursa_linear_dx         dx [M][K] = dz W
+ *   ursa_linear_dw         dw [N][K] = dz' x, x either as `x` or as its 8-bit form (`q`, `e`; K17), the other NULL. M = 0: zeros.
+ *   ws: ursa_linear_ws_bytes(pass, M, N, K, dtype) bytes of scratch private to the call (0: may be NULL); contents need not be set.
+ * The same call gives the same bits every time (no atomics).
+ */
+#define URSA_F32  0
+#define URSA_BF16 1
+#define URSA_F16  2
+#define URSA_ACT_NONE 0
+#define URSA_ACT_RELU 1
+#define URSA_ACT_GELU 2 /* z Phi(z) */
+#define URSA_ACT_SILU 3 /* z / (1 + exp(-z)) */
+#define URSA_LINEAR_FWD 0
+#define URSA_LINEAR_DX  1
+#define URSA_LINEAR_DW  2
+#define URSA_LINEAR_ACT_GRAD 3
+int64_t ursa_linear_ws_bytes(int32_t pass, int64_t M, int64_t N, int64_t K, int32_t dtype);
+int ursa_linear_act(const void* x, const void* w, const void* bias /* or NULL */, const void* residual /* or NULL */, void* y,
+                    void* z /* or NULL */, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream);
+int ursa_linear_act_grad(const void* dy, const void* z, void* dz, void* db /* or NULL */, void* ws, int64_t M, int64_t N, int32_t dtype,
+                         int32_t act, ursa_stream_t stream);
+int ursa_linear_dx(const void* dz, const void* w, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, ursa_stream_t stream);
+int ursa_linear_dw(const void* dz, const void* x /* or NULL */, const int8_t* q /* or NULL */, const int8_t* e, void* dw, void* ws, int64_t M,
+                   int64_t N, int64_t K, int32_t dtype, ursa_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * K16  layer norm over the last dimension          y = (z - mean) / sqrt(var + eps) * gamma + beta,  z = x or x + addend
+ *
+ *   x, addend, z_out, y [M][D] of `dtype`; gamma, beta [D] or NULL of `pdtype` (the same type or URSA_F32). addend and z_out come
+ *   together: z_out is the sum rounded to the type, and what is normalised. mean, rstd [M] fp32 or both NULL. q, e (K17) or both
+ *   NULL: the 8-bit form of z, written in the same pass, from which ursa_layer_norm_bwd can take xhat instead of x.
+ *   backward: dx (or NULL) = d(loss)/dz + dz (dz: the gradient that reaches z by another way, or NULL); dgamma, dbeta [D] (or NULL).
+ *   x: what was normalised (z_out if there was an addend). ws: ursa_layer_norm_ws_floats(M, D) floats when dgamma or dbeta is given.
+ *   Statistics and sums are fp32, summed in a fixed order.
+ */
+int64_t ursa_layer_norm_ws_floats(int64_t M, int64_t D);
+int ursa_layer_norm_fwd(const void* x, const void* addend /* or NULL */, void* z_out /* iff addend */, void* y, const void* gamma,
+                        const void* beta, float* mean, float* rstd, int8_t* q, int8_t* e, int64_t M, int64_t D, float eps, int32_t dtype,
+                        int32_t pdtype, ursa_stream_t stream);
+int ursa_layer_norm_bwd(const void* x /* or NULL */, const int8_t* q /* or NULL */, const int8_t* e, const void* dy, const void* dz /* or NULL */,
+                        const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma, void* dbeta, float* ws, int64_t M,
+                        int64_t D, int32_t dtype, int32_t pdtype, ursa_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * K17  an activation in 8 bits
+ *
+ *   x [M][D] of `dtype` <-> q [M][P] int8 with P = D rounded up to a multiple of 32 (the rest 0; 16-byte aligned), e [M][P / 32]:
+ *   x ~ q 2^e. Each block of 32 features of a row shares e = k - 7, its largest magnitude being m 2^k with 1/2 <= m < 1 (at least
+ *   -126; fp16: -24); q = x / 2^e to the nearest (ties to even), at most 127 in magnitude: |x - q 2^e| <= 2^e, and <= 2^(e - 1) but
+ *   for magnitudes above 127.5 2^e. q 2^e is a number of the type, exactly. A block with an infinity or a NaN in it has e = 127 and
+ *   reads as NaN.
+ */
+int ursa_act8_pack(const void* x, int8_t* q, int8_t* e, int64_t M, int64_t D, int32_t dtype, ursa_stream_t stream);
+int ursa_act8_unpack(const int8_t* q, const int8_t* e, void* x, int64_t M, int64_t D, int32_t dtype, ursa_stream_t stream);
 
 /* ------------------------------------------------------------------------------------ */
 int ursa_abi_version(void);

@@ -1,0 +1,391 @@
+"""K15: act(x W' + b) + r and its gradients against the definition in fp64, at the sizes, types and forms where a launch can go wrong.
+Every tolerance is a bound on the launch's roundings (dense_bounds)."""
+import pytest
+import torch
+import torch.nn as nn
+
+import dense_bounds as B
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+def _case(M, K, N, dtype, seed=0, bias=True, residual=False, away=None):
+    """Operands; `away`: scale of a bias that keeps |z| off relu's gate (alternating in sign over the features)."""
+    g = torch.Generator().manual_seed(seed + 1000 * M + 10 * K + N)
+    t = B.TYPES[dtype]
+    x, w = torch.randn(M, K, generator=g).to(t), (torch.randn(N, K, generator=g) / max(K, 1) ** 0.5).to(t)
+    b = torch.randn(N, generator=g)
+    if away:
+        b = away * (1 - 2 * (torch.arange(N) % 2)).float()
+    r = torch.randn(M, N, generator=g).to(t) if residual else None
+    dy = (torch.randn(M, N, generator=g) / max(M, 1) ** 0.5).to(t)
+    return x, w, b.to(t) if bias else None, r, dy
+
+
+def _run(x, w, b, r, act, dy=None, save8=False):
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(w.shape[1], w.shape[0], bias=b is not None, device=DEV, dtype=w.dtype)
+    with torch.no_grad():
+        fc.weight.copy_(w)
+        if b is not None:
+            fc.bias.copy_(b)
+    fc.requires_grad_(dy is not None)
+    X = x.to(DEV).requires_grad_(dy is not None)
+    R = None if r is None else r.to(DEV).requires_grad_(dy is not None)
+    y = linear_act(fc, X, act, R, save8=save8)
+    if dy is None:
+        return dict(y=y)
+    leaves = dict(dx=X, dw=fc.weight)
+    if b is not None:
+        leaves['db'] = fc.bias
+    if R is not None:
+        leaves['dr'] = R
+    got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy.to(DEV))))
+    if R is not None:
+        assert torch.equal(got.pop('dr').cpu(), dy)
+    return dict(y=y, **got)
+
+
+SIZES = [(1, 1, 1), (1, 8, 16), (2, 31, 3), (3, 5, 7), (16, 64, 64), (17, 33, 65), (64, 128, 128), (65, 130, 131), (100, 784, 200),
+         (128, 200, 10), (130, 64, 129), (257, 96, 300), (5, 4100, 40), (33, 2048, 72), (400, 24, 16), (1000, 32, 8)]
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('M,K,N', SIZES)
+def test_forward_and_gradients_at_odd_and_even_sizes(M, K, N, dtype):
+    x, w, b, r, dy = _case(M, K, N, dtype, residual=True)
+    B.check(_run(x, w, b, r, 'gelu', dy), *B.linear(x, w, b, r, 'gelu', dy), where=(M, K, N, dtype))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('M,K,N', [(600, 520, 1100), (520, 1048, 520), (1100, 264, 1032), (300, 4096, 300), (2100, 130, 150), (777, 555, 333)])
+def test_larger_tiles_and_cut_contractions(M, K, N, dtype):
+    x, w, b, r, dy = _case(M, K, N, dtype, residual=True)
+    B.check(_run(x, w, b, r, 'silu', dy), *B.linear(x, w, b, r, 'silu', dy), where=(M, K, N, dtype))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('residual', [False, True])
+@pytest.mark.parametrize('bias', [False, True])
+@pytest.mark.parametrize('act', [None, 'gelu', 'silu'])
+def test_every_epilogue(act, bias, residual, dtype):
+    x, w, b, r, dy = _case(70, 72, 90, dtype, bias=bias, residual=residual)
+    B.check(_run(x, w, b, r, act, dy), *B.linear(x, w, b, r, act, dy), where=(act, bias, residual, dtype))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+def test_relu_with_its_gate_away_from_zero(dtype):
+    x, w, b, r, dy = _case(70, 72, 90, dtype, residual=True, away=8.0)
+    assert float((x.double() @ w.double().t() + b.double()).abs().min()) > 1
+    B.check(_run(x, w, b, r, 'relu', dy), *B.linear(x, w, b, r, 'relu', dy))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('M', [1, 2, 5, 8, 16, 17, 31, 48, 64])
+@pytest.mark.parametrize('K,N', [(256, 512), (1000, 333), (4096, 96), (72, 1030)])
+def test_few_rows(M, K, N, dtype):
+    x, w, b, r, _ = _case(M, K, N, dtype, residual=True)
+    B.check(_run(x, w, b, r, 'gelu'), *B.linear(x, w, b, r, 'gelu'), where=(M, K, N, dtype))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('M,K,N', [(1, 32, 16), (40, 64, 48), (130, 100, 72), (300, 1111, 200), (1000, 256, 136), (600, 1056, 1100)])
+def test_input_kept_in_8_bits(M, K, N, dtype):
+    x, w, b, r, dy = _case(M, K, N, dtype)
+    x[:, 3] *= 40                                                    # a feature that sets its blocks' scale
+    got = _run(x, w, b, r, 'gelu', dy, save8=True)
+    B.check(got, *B.linear(x, w, b, r, 'gelu', dy, kept=B.unpacked(x)), where=(M, K, N, dtype))
+
+
+def test_gradients_against_differences():
+    """Central differences of sum(c y) along a random direction, fp32: the launches' forward error over the step, and the third
+    derivative's h^2 term (gelu''' <= 2; every |dz| of the step <= h |direction z|)."""
+    M, K, N, h = 20, 48, 40, 2.0 ** -5
+    x, w, b, r, c = _case(M, K, N, 'float32', residual=True)
+    g = torch.Generator().manual_seed(5)
+    vx, vw, vb, vr = (torch.randn(t.shape, generator=g) * s for t, s in ((x, 0.1), (w, 0.02), (b, 0.1), (r, 0.1)))
+    got = _run(x, w, b, r, 'gelu', c)
+    slope = sum(float((got[k].double().cpu() * v.double()).sum()) for k, v in (('dx', vx), ('dw', vw), ('db', vb))) + float((c.double() * vr.double()).sum())
+    side, err = [], 0.0
+    for s in (h, -h):
+        args = (x + s * vx, w + s * vw, b + s * vb, r + s * vr)
+        side.append(float((_run(*args, 'gelu')['y'].double().cpu() * c.double()).sum()))
+        moved = B.linear(*args, 'gelu')[1]['y']
+        err += float((moved * c.double().abs()).sum())
+        # the moved operands are rounded to fp32 themselves: 2^-24 of each, through the sums
+        err += B.F * float(((args[0].abs().double() @ args[1].abs().double().t() * 2 + args[2].abs() + args[3].abs()) * 1.13 * c.abs()).sum())
+    dz1 = vx.double() @ w.double().t() + x.double() @ vw.double().t() + vb.double()
+    dz2 = 2 * (vx.double() @ vw.double().t())
+    third = (2 * dz1.abs() ** 3 + 3 * 0.8 * (dz1 * dz2).abs() + 4 * h * dz2.abs() ** 2) * c.abs().double()
+    values, bounds = B.linear(x, w, b, r, 'gelu', c)
+    own = sum(float((bounds[k] * v.double().abs()).sum()) for k, v in (('dx', vx), ('dw', vw), ('db', vb)))
+    assert abs((side[0] - side[1]) / (2 * h) - slope) <= err / (2 * h) + h * h / 6 * 1.5 * float(third.sum()) + own
+
+
+def test_leading_dimensions_strides_and_offsets():
+    from ursabench_amd.fused_linear import linear_act
+    torch.manual_seed(0)
+    for t in B.TYPES.values():
+        fc = nn.Linear(40, 24, device=DEV, dtype=t)
+        base = torch.randn(3, 7, 81, device=DEV).to(t)
+        x = base[:, :, 1:41]                                         # rows 81 apart, one element off alignment
+        r = torch.randn(24, device=DEV).to(t).expand(3, 7, 24)       # one vector for every row
+        want = linear_act(fc, x.contiguous().view(21, 40), 'silu', r.contiguous().view(21, 24)).view(3, 7, 24)
+        assert torch.equal(linear_act(fc, x, 'silu', r), want)
+        assert torch.equal(linear_act(fc, base.transpose(0, 1)[:, :, 1:41], 'silu', r.transpose(0, 1)), want.transpose(0, 1))
+        one = torch.randn(41, device=DEV).to(t)[1:]
+        assert torch.equal(linear_act(fc, one), linear_act(fc, one.clone()[None])[0])
+        # a contiguous view whose storage starts at an odd element, as weights in a flat arena do
+        flat = torch.zeros(1 + fc.weight.numel(), device=DEV, dtype=t)
+        flat[1:].copy_(fc.weight.detach().view(-1))
+        other = nn.Linear(40, 24, device=DEV, dtype=t)
+        other.weight.data, other.bias.data = flat[1:].view(24, 40), fc.bias.data
+        assert torch.equal(linear_act(other, x, 'silu', r), want)
+        xb = x.detach().requires_grad_()
+        rb = r.detach().requires_grad_()
+        gx, gr, gw = torch.autograd.grad(linear_act(fc, xb, 'silu', rb), (xb, rb, fc.weight), torch.ones(1, device=DEV, dtype=t).expand(3, 7, 24))
+        assert gx.shape == xb.shape and gr.shape == rb.shape and torch.equal(gr, torch.ones_like(gr))
+        other.weight.requires_grad_()
+        assert torch.equal(torch.autograd.grad(linear_act(other, x, 'silu', r).sum(), other.weight)[0], gw)
+
+
+def test_broadcast_residual_gets_the_summed_gradient():
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(16, 24, device=DEV)
+    v = torch.randn(24, device=DEV, requires_grad=True)
+    y = linear_act(fc, torch.randn(9, 16, device=DEV), None, v.expand(9, 24))
+    assert torch.equal(torch.autograd.grad(y.sum(), v)[0], torch.full((24,), 9.0, device=DEV))
+
+
+@pytest.mark.parametrize('frozen', ['x', 'w', 'b', 'xw', 'wb', 'xb', 'xwb'])
+def test_only_the_gradients_that_are_wanted(frozen):
+    from ursabench_amd.fused_linear import linear_act
+    x, w, b, r, dy = _case(33, 40, 50, 'float32', residual=True)
+    full = _run(x, w, b, r, 'gelu', dy)
+    fc = nn.Linear(40, 50, device=DEV)
+    with torch.no_grad():
+        fc.weight.copy_(w), fc.bias.copy_(b)
+    fc.weight.requires_grad_('w' not in frozen), fc.bias.requires_grad_('b' not in frozen)
+    X, R = x.to(DEV).requires_grad_('x' not in frozen), r.to(DEV).requires_grad_()
+    leaves = {k: t for k, t in (('dx', X), ('dw', fc.weight), ('db', fc.bias)) if t.requires_grad}
+    got = torch.autograd.grad(linear_act(fc, X, 'gelu', R), [*leaves.values(), R], dy.to(DEV))
+    assert torch.equal(got[-1].cpu(), dy)
+    for k, t in zip(leaves, got):
+        assert torch.equal(t, full[k]), k
+
+
+def test_empty_batches():
+    from ursabench_amd.fused_linear import linear_act
+    for t in B.TYPES.values():
+        for save8 in (False, True):
+            fc = nn.Linear(40, 24, device=DEV, dtype=t)
+            x = torch.empty(0, 40, device=DEV, dtype=t, requires_grad=True)
+            y = linear_act(fc, x, 'gelu', save8=save8)
+            assert y.shape == (0, 24)
+            dx, dw, db = torch.autograd.grad(y, (x, fc.weight, fc.bias), torch.empty(0, 24, device=DEV, dtype=t))
+            assert dx.shape == (0, 40) and not dw.any() and not db.any() and dw.shape == (24, 40)
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+def test_infinities_and_nans_stay_in_their_rows(dtype):
+    """Other rows keep their bits; the row itself is not finite."""
+    from ursabench_amd.fused_linear import linear_act
+    x, w, b, r, dy = _case(70, 72, 90, dtype)
+    t = B.TYPES[dtype]
+    fc = nn.Linear(72, 90, device=DEV, dtype=t)
+    clean = linear_act(fc, x.to(DEV), 'gelu')
+    for bad in (float('inf'), float('-inf'), float('nan')):
+        z = x.clone()
+        z[5, 7] = bad
+        y = linear_act(fc, z.to(DEV))
+        assert not torch.isfinite(y[5]).any()
+        y = linear_act(fc, z.to(DEV), 'gelu')
+        keep = [i for i in range(70) if i != 5]
+        assert torch.equal(y[keep], clean[keep])
+        X = z.to(DEV).requires_grad_()
+        dw = torch.autograd.grad(linear_act(fc, X, save8=True), fc.weight, dy.to(DEV))[0]
+        assert torch.isnan(dw[:, :32]).all() and torch.isfinite(dw[:, 32:]).all()     # the block of 32 features, no other
+
+
+def test_large_and_small_magnitudes_fp32():
+    """The three-way split holds over fp32's exponents: products of 2^100 and 2^-100, of the largest numbers, and of numbers
+    whose low parts are subnormal."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    g = torch.Generator().manual_seed(3)
+    x, w = torch.randn(40, 64, generator=g), torch.randn(48, 64, generator=g)
+    for sx, sw in ((2.0 ** 100, 2.0 ** -100), (2.0 ** -100, 2.0 ** 100), (2.0 ** 120, 2.0 ** -60), (2.0 ** -60, 2.0 ** -40)):
+        a, c = x * sx, w * sw
+        got = k.linear_act(a.to(DEV), c.to(DEV)).double().cpu()
+        want, bound = B.linear(a, c, None, None, None)
+        # below 2^-117 the low parts of an operand are subnormal bf16 numbers, kept to 2^-133: 2^-134 of each times the other
+        low = 2.0 ** -134 * (a.abs().double().sum(1)[:, None] + c.abs().double().sum(1)[None, :])
+        assert ((got - want['y']).abs() <= bound['y'] + low).all(), (sx, sw)
+    top = torch.full((16, 32), torch.finfo(torch.float32).max)
+    got = k.linear_act(top.to(DEV), torch.full((16, 32), 2.0 ** -10, device=DEV)).double().cpu()
+    want = float(top[0, 0]) * 2.0 ** -10 * 32
+    assert ((got - want).abs() <= 1e-6 * want).all()
+
+
+def test_the_same_call_gives_the_same_bits():
+    for M, K, N, dtype in ((300, 4096, 300, 'bfloat16'), (300, 1000, 200, 'float32')):
+        x, w, b, r, dy = _case(M, K, N, dtype, residual=True)
+        one = _run(x, w, b, r, 'gelu', dy)
+        for _ in range(3):
+            for key, t in _run(x, w, b, r, 'gelu', dy).items():
+                assert torch.equal(t, one[key]), key
+
+
+def test_side_streams_at_once():
+    """Two streams run the same layer on their own inputs; each waits for what it uses."""
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(512, 700, device=DEV).requires_grad_(False)
+    xs = [torch.randn(300, 512, device=DEV) for _ in range(4)]
+    want = [linear_act(fc, x, 'gelu') for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None] * 4
+    for i, x in enumerate(xs):
+        s = streams[i % 2]
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got[i] = linear_act(fc, x, 'gelu')
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+def test_captured_step_replays_like_the_eager_one(dtype):
+    """Forward and backward of a layer (cut contractions among them) in a graph: several replays on new inputs with eager work and
+    synchronisations between, every one equal to the eager call."""
+    from ursabench_amd import _capture
+    from ursabench_amd.fused_linear import linear_act
+    t = B.TYPES[dtype]
+    torch.manual_seed(1)
+    fc = nn.Linear(1000, 200, device=DEV, dtype=t)
+    x = torch.zeros(96, 1000, device=DEV, dtype=t, requires_grad=True)
+    dy = torch.zeros(96, 200, device=DEV, dtype=t)
+
+    def step(a, c, save8):
+        return torch.autograd.grad(linear_act(fc, a, 'gelu', save8=save8), (a, fc.weight, fc.bias), c)
+
+    for save8 in (False, True):
+        side = _capture.side_streams(torch.device(DEV, 0), 1)[0]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(x, dy, save8)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with _capture.capture(graph):
+            out = step(x, dy, save8)
+        for k in range(4):
+            a, c = torch.randn(96, 1000, device=DEV).to(t), torch.randn(96, 200, device=DEV).to(t)
+            with torch.no_grad():
+                x.copy_(a), dy.copy_(c)
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [o.clone() for o in out]
+            want = step(a.requires_grad_(), c, save8)
+            torch.cuda.synchronize()
+            for p, q in zip(got, want):
+                assert torch.equal(p, q), (save8, k)
+
+
+def test_what_takes_the_stock_path():
+    """Autocast, mixed types, fp64, hooks, subclasses and the switch: fc(x) and the stock activation, same bits."""
+    import torch.nn.functional as F
+    from ursabench_amd import fused_linear
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(40, 24, device=DEV)
+    x = torch.randn(9, 40, device=DEV)
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        y = linear_act(fc, x, 'relu')
+        assert y.dtype == torch.bfloat16 and torch.equal(y, F.relu(fc(x)))
+    d = nn.Linear(40, 24, device=DEV, dtype=torch.float64)
+    assert torch.equal(linear_act(d, x.double(), 'silu'), F.silu(d(x.double())))
+    with pytest.raises(RuntimeError):
+        linear_act(fc, x.to(torch.bfloat16))
+    seen = []
+    hook = fc.register_forward_hook(lambda *a: seen.append(1))
+    linear_act(fc, x)
+    hook.remove()
+    assert seen
+
+    class Doubled(nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    two = Doubled(40, 24, device=DEV)
+    assert torch.equal(linear_act(two, x, 'relu'), F.relu(two(x)))
+    old = fused_linear.enabled(False)
+    try:
+        assert torch.equal(linear_act(fc, x, 'gelu'), F.gelu(fc(x)))
+    finally:
+        fused_linear.enabled(old)
+
+
+def test_saved_memory():
+    """What a layer keeps for its backward pass: x in 8 bits is 33 / 128 of its fp32 size."""
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(4096, 16, device=DEV)
+    held = []
+    for save8 in (False, True):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = linear_act(fc, torch.randn(2048, 4096, device=DEV, requires_grad=True).mul(2), save8=save8)
+        held.append(torch.cuda.memory_allocated() - before)
+        del y
+    full = 2048 * 4096 * 4
+    assert held[0] - held[1] == full - full // 4 - full // 128
+
+
+def test_models_take_it_when_asked():
+    """models.MLP / LeNet5 with in_models(True): logits and gradients of the stock networks to fp32 rounding (the gates' inputs of
+    this seed are not within it of zero: the same units are open)."""
+    from ursabench_amd import fused_linear, models
+    assert fused_linear.in_models() is False
+    for make, shape in ((lambda: models.MLP(200, 784, 10), (64, 1, 28, 28)), (lambda: models.LeNet5(10), (32, 1, 28, 28))):
+        torch.manual_seed(0)
+        net = make().to(DEV)
+        x, y = torch.randn(shape, device=DEV), torch.randint(0, 10, shape[:1], device=DEV)
+
+        def step():
+            logits = net(x)
+            return logits.detach(), torch.autograd.grad(torch.nn.functional.cross_entropy(logits, y), list(net.parameters()))
+
+        want, gw = step()
+        calls = []
+        real, fused_linear.linear_act = fused_linear.linear_act, lambda *a, **k: calls.append(1) or real(*a, **k)
+        old = fused_linear.in_models(True)
+        try:
+            got, gg = step()
+        finally:
+            fused_linear.in_models(old)
+            fused_linear.linear_act = real
+        assert len(calls) == 3
+        # fp32 sums of at most 800 terms through three layers, two orders of summation: 800 x 2^-24 x 3 of the scale
+        assert float((got - want).abs().max()) <= 1.5e-4 * float(want.abs().max())
+        for a, b in zip(gg, gw):
+            assert float((a - b).abs().max()) <= 3e-4 * float(b.abs().max())
+
+
+def test_sampler_runs_on_it():
+    """An SGHMC chain (captured steps) on the MLP with the launches in: the graph path runs and its members are finite and differ."""
+    from ursabench_amd import fused_linear, inference, models
+    from ursabench_amd.data import synthetic
+    torch.manual_seed(0)
+    train = synthetic(512, (1, 28, 28), 10, seed=0, device=torch.device(DEV, 0), batch_size=128)
+    old = fused_linear.in_models(True)
+    try:
+        s = inference.SGHMC({'lr': 0.01, 'prior_std': 0.5, 'num_samples': 2, 'alpha': 0.5, 'burn_in_epochs': 0},
+                            models.MLP(200, 784, 10).to(DEV), train, device=torch.device(DEV, 0))
+        members = s.sample()
+        assert s.engine.stats['graph_replays'] > 0
+    finally:
+        fused_linear.in_models(old)
+    a, b = (torch.cat([p.detach().view(-1) for p in m.parameters()]) for m in members)
+    assert torch.isfinite(a).all() and torch.isfinite(b).all() and not torch.equal(a, b)

@@ -1,0 +1,356 @@
+"""K16 (layer norm, the residual sum in front of it) and K17 (8-bit activations) against the definitions in fp64; tolerances are
+bounds on the launches' roundings (dense_bounds)."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+import dense_bounds as B
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+WIDTHS = [1, 2, 7, 24, 31, 32, 33, 127, 128, 129, 500, 513, 784, 1024, 1111, 2048, 2049, 4096, 5000, 8192, 9999, 16384]
+
+
+def _case(M, D, dtype, seed=0, ptype=None, offset=0.3):
+    g = torch.Generator().manual_seed(seed + 17 * M + D)
+    t = B.TYPES[dtype]
+    x = (torch.randn(M, D, generator=g) * 1.5 + offset).to(t)
+    r = torch.randn(M, D, generator=g).to(t)
+    w, b = (1 + 0.3 * torch.randn(D, generator=g)).to(ptype or t), (0.3 * torch.randn(D, generator=g)).to(ptype or t)
+    dy, dz = torch.randn(M, D, generator=g).to(t), torch.randn(M, D, generator=g).to(t)
+    return x, r, w, b, dy, dz
+
+
+def _module(D, w, b, eps=1e-5, grad=True):
+    ln = nn.LayerNorm(D, eps=eps, elementwise_affine=w is not None, bias=b is not None, device=DEV, dtype=None if w is None else w.dtype)
+    with torch.no_grad():
+        if w is not None:
+            ln.weight.copy_(w)
+        if b is not None:
+            ln.bias.copy_(b)
+    return ln.requires_grad_(grad)
+
+
+def _run(x, w, b, dy, r=None, dz=None, eps=1e-5, save8=False):
+    """Outputs and gradients; z (the stored sum) apart."""
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    ln = _module(x.shape[-1], w, b, eps)
+    X = x.to(DEV).requires_grad_()
+    leaves = dict(dx=X)
+    if w is not None:
+        leaves['dg'] = ln.weight
+    if b is not None:
+        leaves['db'] = ln.bias
+    if r is None:
+        y = layer_norm(ln, X, save8=save8)
+        return None, dict(y=y, **dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy.to(DEV)))))
+    R = r.to(DEV).requires_grad_()
+    z, y = add_layer_norm(ln, (X, R), save8=save8)
+    got = dict(zip([*leaves, 'dr'], torch.autograd.grad((z, y), [*leaves.values(), R], (dz.to(DEV), dy.to(DEV)))))
+    assert torch.equal(got.pop('dr'), got['dx'])
+    return z, dict(y=y, **got)
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('D', WIDTHS + [16385, 20000])
+def test_widths(D, dtype):
+    for M in (1, 5, 37) if D < 5000 else (1, 5):
+        x, r, w, b, dy, dz = _case(M, D, dtype)
+        B.check(_run(x, w, b, dy)[1], *B.norm(x, w, b, 1e-5, dy), where=('norm', M, D, dtype))
+        z, got = _run(x, w, b, dy, r, dz)
+        stored = (x.float() + r.float()).to(x.dtype)
+        assert torch.equal(z.cpu(), stored)
+        B.check(got, *B.norm(stored, w, b, 1e-5, dy, dz), where=('add', M, D, dtype))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('D', [1, 24, 33, 128, 513, 1111, 2048, 4100, 9000, 16384, 17000])
+def test_input_kept_in_8_bits(D, dtype):
+    for M in (1, 6, 70) if D < 5000 else (3,):
+        x, r, w, b, dy, dz = _case(M, D, dtype)
+        x[:, 0] *= 30
+        B.check(_run(x, w, b, dy, save8=True)[1], *B.norm(x, w, b, 1e-5, dy, kept=B.unpacked(x)), where=('norm', M, D, dtype))
+        z, got = _run(x, w, b, dy, r, dz, save8=True)
+        stored = z.detach().cpu()
+        B.check(got, *B.norm(stored, w, b, 1e-5, dy, dz, kept=B.unpacked(stored)), where=('add', M, D, dtype))
+
+
+@pytest.mark.parametrize('dtype', ['bfloat16', 'float16'])
+@pytest.mark.parametrize('M,D', [(40, 100), (700, 96), (3000, 520), (2100, 2304), (600, 5120)])
+def test_fp32_parameters_and_many_rows(M, D, dtype):
+    x, r, w, b, dy, dz = _case(M, D, dtype, ptype=torch.float32)
+    z, got = _run(x, w, b, dy, r, dz)
+    assert got['dg'].dtype == got['db'].dtype == torch.float32
+    B.check(got, *B.norm(z.detach().cpu(), w, b, 1e-5, dy, dz), where=(M, D, dtype))
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('affine', ['none', 'weight'])
+def test_without_weight_or_bias(affine, dtype):
+    x, r, w, b, dy, dz = _case(50, 200, dtype)
+    w = None if affine == 'none' else w
+    B.check(_run(x, w, None, dy)[1], *B.norm(x, w, None, 1e-5, dy), where=(affine, dtype))
+
+
+def test_rows_far_from_zero_keep_their_variance():
+    """Mean 1,000 times the deviation: the squares are summed around the mean, not as a difference of large numbers."""
+    x, r, w, b, dy, dz = _case(20, 700, 'float32', offset=1500.0)
+    B.check(_run(x, w, b, dy)[1], *B.norm(x, w, b, 1e-5, dy))
+
+
+def test_constant_rows_and_eps():
+    from ursabench_amd.fused_norm import layer_norm
+    ln = _module(64, torch.ones(64), torch.zeros(64), eps=1e-3)
+    x = torch.full((3, 64), 2.5, device=DEV)
+    assert torch.equal(layer_norm(ln, x), torch.zeros(3, 64, device=DEV))
+    x, r, w, b, dy, dz = _case(9, 64, 'float32')
+    B.check(_run(x * 1e-3, w, b, dy, eps=1e-3)[1], *B.norm(x * 1e-3, w, b, 1e-3, dy))
+
+
+def test_gradients_against_differences():
+    M, D, h = 6, 50, 2.0 ** -5
+    x, r, w, b, c, _ = _case(M, D, 'float32')
+    g = torch.Generator().manual_seed(2)
+    v = 0.2 * torch.randn(M, D, generator=g)
+    _, got = _run(x, w, b, c)
+    slope = float((got['dx'].double().cpu() * v.double()).sum())
+    side, err = [], 0.0
+    for s in (h, -h):
+        moved = x + s * v
+        side.append(float((_run(moved, w, b, c)[1]['y'].double().cpu() * c.double()).sum()))
+        values, bounds = B.norm(moved, w, b, 1e-5)
+        err += float((bounds['y'] * c.double().abs()).sum())
+        # the rounding of the moved input: 2^-24 |x| an element, through a map whose slope is at most 2 rstd |g| in the largest norm
+        rstd = 1 / (moved.double().var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+        err += float(B.F * (moved.double().abs().amax(1, keepdim=True) * 2 * D ** 0.5 * rstd * w.double().abs() * c.double().abs()).sum())
+    # |third derivative| of a row's y along v: at most 15 (|v| rstd)^3 with |v| the row's norm over sqrt(D) (the norm's own terms)
+    rstd = 1 / (x.double().var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    third = 15 * (v.double().norm(dim=1, keepdim=True) * rstd) ** 3 * (w.double().abs() * c.double().abs())
+    assert abs((side[0] - side[1]) / (2 * h) - slope) <= err / (2 * h) + h * h / 6 * float(third.sum()) + float((B.norm(x, w, b, 1e-5, c)[1]['dx'] * v.double().abs()).sum())
+
+
+def test_shapes_strides_and_several_normalised_dimensions():
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    torch.manual_seed(0)
+    for t in B.TYPES.values():
+        ln = nn.LayerNorm((6, 8), device=DEV, dtype=t)
+        with torch.no_grad():
+            ln.weight.normal_(), ln.bias.normal_()
+        x = torch.randn(3, 4, 6, 8, device=DEV).to(t)
+        flat = nn.LayerNorm(48, device=DEV, dtype=t)
+        with torch.no_grad():
+            flat.weight.copy_(ln.weight.view(-1)), flat.bias.copy_(ln.bias.view(-1))
+        want = layer_norm(flat, x.view(12, 48)).view_as(x)
+        assert torch.equal(layer_norm(ln, x), want)
+        wide = torch.randn(3, 4, 6, 9, device=DEV).to(t)
+        wide[..., 1:] = x
+        assert torch.equal(layer_norm(ln, wide[..., 1:]), want)
+        z, y = add_layer_norm(ln, (wide[..., 1:], torch.zeros(1, device=DEV, dtype=t).expand_as(x)))
+        assert torch.equal(z, x) and torch.equal(y, want)
+        gw = torch.autograd.grad(layer_norm(ln, x).sum(), ln.weight)[0]
+        assert gw.shape == (6, 8)
+        pair = add_layer_norm(ln, x)
+        assert pair[0] is x and torch.equal(pair[1], want)
+
+
+def test_only_the_gradients_that_are_wanted():
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    x, r, w, b, dy, dz = _case(30, 96, 'float32')
+    _, full = _run(x, w, b, dy)
+    for frozen in ('x', 'w', 'b', 'xw', 'wb', 'xb'):
+        ln = _module(96, w, b)
+        ln.weight.requires_grad_('w' not in frozen), ln.bias.requires_grad_('b' not in frozen)
+        X = x.to(DEV).requires_grad_('x' not in frozen)
+        leaves = {k: t for k, t in (('dx', X), ('dg', ln.weight), ('db', ln.bias)) if t.requires_grad}
+        for k, t in zip(leaves, torch.autograd.grad(layer_norm(ln, X), list(leaves.values()), dy.to(DEV))):
+            assert torch.equal(t, full[k]), (frozen, k)
+    # of the pair: one output unused, one summand without a gradient
+    ln = _module(96, w, b)
+    X, R = x.to(DEV).requires_grad_(), r.to(DEV)
+    z, y = add_layer_norm(ln, (X, R))
+    assert torch.equal(torch.autograd.grad(z, X, dz.to(DEV), retain_graph=True)[0].cpu(), dz)
+    only_y = torch.autograd.grad(y, X, dy.to(DEV), retain_graph=True)[0]
+    both = torch.autograd.grad((z, y), X, (torch.zeros_like(z), dy.to(DEV)))[0]
+    assert torch.equal(only_y, both)
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+def test_infinities_and_nans_stay_in_their_rows(dtype):
+    from ursabench_amd.fused_norm import layer_norm
+    x, r, w, b, dy, dz = _case(40, 300, dtype)
+    ln = _module(300, w, b)
+    clean = layer_norm(ln, x.to(DEV))
+    for bad in (float('inf'), float('nan')):
+        x2 = x.clone()
+        x2[7, 5] = bad
+        y = layer_norm(ln, x2.to(DEV))
+        keep = [i for i in range(40) if i != 7]
+        assert torch.equal(y[keep], clean[keep]) and not torch.isfinite(y[7]).any()
+
+
+def test_the_same_call_gives_the_same_bits():
+    for M, D, dtype in ((5000, 300, 'float32'), (3000, 4096, 'bfloat16')):
+        x, r, w, b, dy, dz = _case(M, D, dtype)
+        one = _run(x, w, b, dy, r, dz)[1]
+        for _ in range(3):
+            for k, t in _run(x, w, b, dy, r, dz)[1].items():
+                assert torch.equal(t, one[k]), k
+
+
+@pytest.mark.parametrize('save8', [False, True])
+def test_captured_step_replays_like_the_eager_one(save8):
+    from ursabench_amd import _capture
+    from ursabench_amd.fused_norm import add_layer_norm
+    t, M, D = torch.bfloat16, 200, 1000
+    ln = nn.LayerNorm(D, device=DEV, dtype=t)
+    a = torch.zeros(M, D, device=DEV, dtype=t, requires_grad=True)
+    r, dy, dz = (torch.zeros(M, D, device=DEV, dtype=t) for _ in range(3))
+
+    def step(a, r, dy, dz):
+        z, y = add_layer_norm(ln, (a, r), save8=save8)
+        return (z.detach(), y.detach()) + torch.autograd.grad((z, y), (a, ln.weight, ln.bias), (dz, dy))
+
+    side = _capture.side_streams(torch.device(DEV, 0), 1)[0]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(a, r, dy, dz)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with _capture.capture(graph):
+        out = step(a, r, dy, dz)
+    for k in range(4):
+        new = [torch.randn(M, D, device=DEV).to(t) for _ in range(4)]
+        with torch.no_grad():
+            for dst, src in zip((a, r, dy, dz), new):
+                dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in out]
+        want = step(new[0].requires_grad_(), *new[1:])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), k
+
+
+def test_what_takes_the_stock_path():
+    from ursabench_amd import fused_norm
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    ln = nn.LayerNorm(40, device=DEV)
+    x = torch.randn(9, 40, device=DEV)
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        assert torch.equal(layer_norm(ln, x), ln(x))
+    d = nn.LayerNorm(40, device=DEV, dtype=torch.float64)
+    assert torch.equal(layer_norm(d, x.double()), d(x.double()))
+    assert layer_norm(ln, x[:0]).shape == (0, 40)
+    with pytest.raises(RuntimeError):
+        layer_norm(ln, x[:, :39])
+    z, y = add_layer_norm(ln, (x, x[:1]))                            # a broadcast sum: two stock steps, the norm ours
+    assert torch.equal(z, x + x[:1]) and torch.equal(y, layer_norm(ln, z))
+    old = fused_norm.enabled(False)
+    try:
+        assert torch.equal(layer_norm(ln, x), ln(x))
+    finally:
+        fused_norm.enabled(old)
+
+
+# ---- K17 --------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('M,D', [(1, 1), (3, 31), (2, 32), (5, 33), (7, 100), (64, 1024), (9, 4097), (1000, 8)])
+def test_pack_is_the_definition(M, D, dtype):
+    from ursabench_amd import act8
+    t = B.TYPES[dtype]
+    g = torch.Generator().manual_seed(M + D)
+    x = (torch.randn(M, D, generator=g) * torch.exp(2 * torch.randn(M, 1, generator=g))).to(t)
+    p = act8.pack(x.to(DEV))
+    assert p.q.shape == (M, -(-D // 32) * 32) and not p.q[:, D:].any() and p.nbytes == p.q.numel() * 33 // 32
+    assert int(p.q.min()) >= -127
+    back = act8.unpack(p)
+    assert back.dtype == t and torch.equal(back.double().cpu(), B.unpacked(x))
+    step = torch.pow(2.0, p.e.double().cpu()).repeat_interleave(32, 1)[:, :D]
+    off = (back.double().cpu() - x.double()).abs()
+    assert (off <= step).all() and (off[x.double().abs() <= 127.5 * step] <= (step / 2)[x.double().abs() <= 127.5 * step]).all()
+    again = act8.pack(back)                                          # what is packed once stays what it is
+    assert torch.equal(act8.unpack(again), back)
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+def test_pack_at_the_ends_of_the_type(dtype):
+    from ursabench_amd import act8
+    t = B.TYPES[dtype]
+    info = torch.finfo(t)
+    tiny = info.smallest_normal * info.eps                            # the smallest subnormal number
+    rows = [[0.0] * 32, [info.max] * 32, [-info.max] + [1.0] * 31, [info.smallest_normal] * 32, [tiny] * 32, [tiny] * 16 + [info.smallest_normal * 64] * 16,
+            [127.5] * 16 + [63.5] * 16, [1.0, 0.5] * 16, [-0.0] * 32]
+    x = torch.tensor(rows, dtype=torch.float64).to(t)
+    back = act8.unpack(act8.pack(x.to(DEV)))
+    assert torch.isfinite(back).all() and torch.equal(back.double().cpu(), B.unpacked(x))
+    y = torch.randn(4, 96).to(t)
+    y[0, 3], y[1, 40], y[2, 95] = math.inf, -math.inf, math.nan
+    back = act8.unpack(act8.pack(y.to(DEV))).cpu()
+    gone = torch.zeros(4, 96, dtype=torch.bool)
+    gone[0, :32], gone[1, 32:64], gone[2, 64:] = True, True, True
+    assert torch.equal(torch.isnan(back), gone) and torch.isfinite(back[~gone]).all()
+
+
+def test_pack_shapes_and_refusals():
+    from ursabench_amd import act8
+    x = torch.randn(2, 3, 5, 70, device=DEV)
+    assert torch.equal(act8.unpack(act8.pack(x)), act8.unpack(act8.pack(x.view(30, 70))).view_as(x))
+    assert torch.equal(act8.unpack(act8.pack(x.transpose(0, 2))), act8.unpack(act8.pack(x)).transpose(0, 2))
+    assert act8.unpack(act8.pack(x[:0])).shape == (0, 3, 5, 70)
+    with pytest.raises(TypeError, match='float32, bfloat16 or float16'):
+        act8.pack(x.double())
+    with pytest.raises(ValueError):
+        act8.pack(x.new_tensor(1.0))
+    p = act8.pack(x)
+    with pytest.raises(ValueError, match='elements'):
+        act8.unpack(p._replace(shape=torch.Size((2, 3, 5, 100))))
+    with pytest.raises(TypeError):
+        act8.unpack(p._replace(dtype=torch.float64))
+
+
+# ---- a run of them together -------------------------------------------------------------------
+def _block(ln, up, down, x, save8):
+    """x + down(gelu(up(ln(x)))), handed on as a pending sum like the residual blocks of models.py: (z, branch) -> next norm."""
+    from ursabench_amd.fused_linear import linear_act
+    from ursabench_amd.fused_norm import add_layer_norm
+    z, h = add_layer_norm(ln, x, save8=save8)
+    return z, linear_act(down, linear_act(up, h, 'gelu', save8=save8), save8=save8)
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('save8', [False, True])
+def test_residual_blocks_train_as_the_stock_modules_do(save8, dtype):
+    """Two pre-norm blocks and a head, forward and backward, against the same network in fp64 stock ops: every gradient within the
+    roundings of the chain. One rounding to the type relative to each tensor's scale at each of the 14 tensors a gradient passes
+    through on its way (7 forward, 7 back), doubled for the layers' gain; 8-bit inputs add half a step of 2^-7 of a block's
+    largest value (4 deviations) to each of the three layers of a block."""
+    t = B.TYPES[dtype]
+    torch.manual_seed(4)
+    D, H, M = 96, 200, 50
+    mods = nn.ModuleList([nn.ModuleList([nn.LayerNorm(D), nn.Linear(D, H), nn.Linear(H, D)]) for _ in range(2)] + [nn.LayerNorm(D)])
+    mods = mods.to(t)
+    ref = nn.ModuleList([nn.ModuleList([nn.LayerNorm(D), nn.Linear(D, H), nn.Linear(H, D)]) for _ in range(2)] + [nn.LayerNorm(D)]).double()
+    ref.load_state_dict({k: v.double() for k, v in mods.state_dict().items()})
+    x = torch.randn(M, D).to(t)
+    c = (torch.randn(M, D) / M).to(t)
+    h = x.double()
+    for ln, up, down in ref[:2]:
+        h = h + down(torch.nn.functional.gelu(up(ln(h))))
+    want = ref[2](h)
+    gw = torch.autograd.grad((want * c.double()).sum(), list(ref.parameters()))
+    mods.to(DEV)
+    from ursabench_amd.fused_norm import add_layer_norm
+    s = x.to(DEV)
+    for ln, up, down in mods[:2]:
+        s = _block(ln, up, down, s, save8)
+    y = add_layer_norm(mods[2], s, save8=save8)[1]
+    got = torch.autograd.grad(y, list(mods.parameters()), c.to(DEV))
+    u = max(B.half_step(t), 2.0 ** -20)                               # fp32: sums of up to 200 terms rather than one rounding
+    rms = lambda v: float(v.double().pow(2).mean().sqrt())            # noqa: E731
+    assert rms(y.cpu().double() - want) <= 2 * 7 * u * rms(want)
+    lim = 2 * 14 * u + (6 * 2.0 ** -8 * 4 if save8 else 0)
+    for (k, _), a, b in zip(mods.named_parameters(), got, gw):
+        assert rms(a.cpu().double() - b) <= lim * rms(b), (k, rms(a.cpu().double() - b) / rms(b))

@@ -18,7 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libursa_hip.so')
 KNOBS_LIB_PATH = os.path.join(_HERE, 'csrc', 'libursa_hip_knobs.so')   # -DURSA_DEBUG_KNOBS build: tests / tools only
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 # flags (mirror include/ursa_hip.h)
 STEP_NOISE, STEP_FIRST, STEP_ZERO_GRAD, STEP_WD, STEP_SGD, STEP_ADVANCE = 0x1, 0x2, 0x4, 0x8, 0x10, 0x20
@@ -27,6 +27,10 @@ LEAP_KICK, LEAP_DRIFT = 0x1, 0x2
 REDUCE_WS_FLOATS = 2048
 BN_RELU, BN_TWO_LAUNCH, BN_HELD = 0x1, 0x2, 0x4
 CONV_FLIP, CONV_STRIDE2 = 0x1, 0x2
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # element types of K15 - K17
+ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
+LINEAR_FWD, LINEAR_DX, LINEAR_DW, LINEAR_ACT_GRAD = 0, 1, 2, 3
+ACT8_BLOCK = 32                                                           # features of a row that share a power of two (K17)
 PREACT_BN, PREACT_STATS, PREACT_ADD, PREACT_BNBWD, PREACT_EVAL = 0x10, 0x20, 0x40, 0x80, 0x100
 
 
@@ -94,6 +98,16 @@ SIGNATURES = {
     'ursa_bn_relu_pool_bwd_f32': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     'ursa_bn_apply_f32': (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f, _f, _u32, _vp]),
     'ursa_bn_bwd_dx_f32': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _vp]),
+    'ursa_linear_ws_bytes': (_i64, [_i32, _i64, _i64, _i64, _i32]),
+    'ursa_linear_act': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    'ursa_linear_act_grad': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
+    'ursa_linear_dx': (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    'ursa_linear_dw': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    'ursa_layer_norm_ws_floats': (_i64, [_i64, _i64]),
+    'ursa_layer_norm_fwd': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _i32, _i32, _vp]),
+    'ursa_layer_norm_bwd': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
+    'ursa_act8_pack': (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    'ursa_act8_unpack': (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
 }
 
 
@@ -197,6 +211,36 @@ def _ptr(t, name, n=None, device=None, optional=False):
     if device is not None and t.device != device:
         raise ValueError(f'{name} is on {t.device}, expected {device}')
     return t.data_ptr()
+
+
+def _tptr(t, name, dtype, n=None, device=None, optional=False):
+    """_ptr for the launches that take several element types."""
+    if t is None:
+        if optional:
+            return None
+        raise ValueError(f'{name} is required')
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f'{name} must be a torch.Tensor, got {type(t).__name__}')
+    if not t.is_cuda:
+        raise RuntimeError(f'{name} must live on a HIP device (got {t.device}); ursabench_amd has no CPU path')
+    if t.dtype != dtype:
+        raise TypeError(f'{name} must be {str(dtype)[6:]}, got {t.dtype}')
+    if not t.is_contiguous():
+        raise ValueError(f'{name} must be contiguous')
+    if n is not None and t.numel() != n:
+        raise ValueError(f'{name} has {t.numel()} elements, expected {n}')
+    if device is not None and t.device != device:
+        raise ValueError(f'{name} is on {t.device}, expected {device}')
+    return t.data_ptr()
+
+
+def _element_type(x, name):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f'{name} must be a torch.Tensor, got {type(x).__name__}')
+    dt = DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f'{name} must be float32, bfloat16 or float16, got {x.dtype}')
+    return dt
 
 
 def nhwc_twin_supported(x):
@@ -904,6 +948,172 @@ class HipKernels:
                                                     _ptr(save, 'save', 4 * C, dev), _ptr(dz, 'dz', z.numel(), dev), _ptr(dgamma, 'dgamma', C, dev),
                                                     _ptr(dbeta, 'dbeta', C, dev), N, C, HW, _stream(dev))
         _check(self.lib, rc, 'ursa_bn_relu_pool_bwd_f32')
+
+    # K15 -----------------------------------------------------------------------------
+    def _launch(self, name, dev, *args):
+        fn = getattr(self.lib, name)
+        if torch.cuda.current_device() == dev.index:
+            rc = fn(*args, _stream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, _stream(dev))
+        if rc:
+            _check(self.lib, rc, name)
+
+    def _linear_ws(self, which, M, N, K, dt, x):
+        n = self.lib.ursa_linear_ws_bytes(which, M, N, K, dt)
+        return x.new_empty(n, dtype=torch.uint8) if n else None
+
+    @staticmethod
+    def _act(activation):
+        try:
+            return ACTIVATIONS[activation]
+        except (KeyError, TypeError):
+            raise ValueError(f'activation must be one of {list(ACTIVATIONS)}, got {activation!r}') from None
+
+    def linear_act(self, x, w, bias=None, residual=None, *, activation=None, save_z=False):
+        """act(x W' + bias) + residual for x [M, K], w [N, K] -> y [M, N] (and z = x W' + bias with `save_z`: (y, z))."""
+        dt, act = _element_type(x, 'x'), self._act(activation)
+        if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+            raise ValueError(f'x {tuple(x.shape)} and w {tuple(w.shape)} should be [M, K] and [N, K]')
+        (M, K), N, t, dev = x.shape, w.shape[0], x.dtype, x.device
+        px, pw = _tptr(x, 'x', t), _tptr(w, 'w', t, None, dev)
+        pb, pr = _tptr(bias, 'bias', t, N, dev, True), _tptr(residual, 'residual', t, M * N, dev, True)
+        y = x.new_empty((M, N))
+        z = torch.empty_like(y) if save_z else None
+        ws = self._linear_ws(LINEAR_FWD, M, N, K, dt, x)
+        self._launch('ursa_linear_act', dev, px, pw, pb, pr, y.data_ptr(), None if z is None else z.data_ptr(),
+                     None if ws is None else ws.data_ptr(), M, N, K, dt, act)
+        return (y, z) if save_z else y
+
+    def linear_act_grad(self, dy, z=None, *, activation=None, bias_grad=True):
+        """(dz, db): dz = dy act'(z) (dy itself without an activation), db [N] its column sums or None."""
+        dt, act = _element_type(dy, 'dy'), self._act(activation)
+        (M, N), t, dev = dy.shape, dy.dtype, dy.device
+        pd = _tptr(dy, 'dy', t)
+        pz = _tptr(z, 'z', t, M * N, dev, optional=not act)
+        if not act and z is not None:
+            raise ValueError('z without an activation')
+        if M == 0:
+            return dy, dy.new_zeros(N) if bias_grad else None
+        dz = torch.empty_like(dy) if act else None
+        db = dy.new_empty(N) if bias_grad else None
+        if act or bias_grad:
+            ws = self._linear_ws(LINEAR_ACT_GRAD, M, N, 0, dt, dy) if bias_grad else None
+            self._launch('ursa_linear_act_grad', dev, pd, pz, None if dz is None else dz.data_ptr(), None if db is None else db.data_ptr(),
+                         None if ws is None else ws.data_ptr(), M, N, dt, act)
+        return (dz if act else dy), db
+
+    def linear_dx(self, dz, w):
+        dt = _element_type(dz, 'dz')
+        if dz.dim() != 2 or w.dim() != 2 or dz.shape[1] != w.shape[0]:
+            raise ValueError(f'dz {tuple(dz.shape)} and w {tuple(w.shape)} should be [M, N] and [N, K]')
+        (M, N), K, dev = dz.shape, w.shape[1], dz.device
+        pz, pw = _tptr(dz, 'dz', dz.dtype), _tptr(w, 'w', dz.dtype, None, dev)
+        dx = dz.new_empty((M, K))
+        ws = self._linear_ws(LINEAR_DX, M, N, K, dt, dz)
+        self._launch('ursa_linear_dx', dev, pz, pw, dx.data_ptr(), None if ws is None else ws.data_ptr(), M, N, K, dt)
+        return dx
+
+    def linear_dw(self, dz, x=None, *, q=None, e=None, in_features=None):
+        """dz' x [N, K], x given as itself or as its 8-bit form (q, e) of `in_features` columns."""
+        dt = _element_type(dz, 'dz')
+        if (x is None) == (q is None):
+            raise ValueError('linear_dw wants x or its 8-bit form')
+        (M, N), t, dev = dz.shape, dz.dtype, dz.device
+        pz = _tptr(dz, 'dz', t)
+        if x is not None:
+            if x.dim() != 2 or x.shape[0] != M:
+                raise ValueError(f'dz {tuple(dz.shape)} and x {tuple(x.shape)} should be [M, N] and [M, K]')
+            K, px, pq, pe = x.shape[1], _tptr(x, 'x', t, None, dev), None, None
+        else:
+            K, px = int(in_features), None
+            pq, pe = self._act8_ptrs(q, e, M, K, dev)
+        dw = dz.new_empty((N, K))
+        ws = self._linear_ws(LINEAR_DW, M, N, K, dt, dz)
+        self._launch('ursa_linear_dw', dev, pz, px, pq, pe, dw.data_ptr(), None if ws is None else ws.data_ptr(), M, N, K, dt)
+        return dw
+
+    # K16 -----------------------------------------------------------------------------
+    @staticmethod
+    def _norm_param_type(x, gamma, beta):
+        dt = _element_type(x, 'x')
+        p = gamma if gamma is not None else beta
+        pt = x.dtype if p is None else p.dtype
+        if pt not in (x.dtype, torch.float32):
+            raise TypeError(f'gamma / beta must be {str(x.dtype)[6:]} or float32, got {pt}')
+        return dt, pt
+
+    def layer_norm(self, x, gamma=None, beta=None, *, eps, addend=None, stats=False, save8=False):
+        """x [M, D] -> (z, y, mean, rstd, q, e): z the sum with `addend` (x without one); mean / rstd with `stats`, q / e (the
+        8-bit form of z) with `save8`, None otherwise."""
+        dt, pt = self._norm_param_type(x, gamma, beta)
+        if x.dim() != 2 or x.shape[1] < 1:
+            raise ValueError(f'x {tuple(x.shape)} should be [M, D]')
+        (M, D), t, dev = x.shape, x.dtype, x.device
+        px, pa = _tptr(x, 'x', t), _tptr(addend, 'addend', t, M * D, dev, True)
+        pg, pb = _tptr(gamma, 'gamma', pt, D, dev, True), _tptr(beta, 'beta', pt, D, dev, True)
+        z = x if addend is None else torch.empty_like(x)
+        y = torch.empty_like(x)
+        ms = x.new_empty((2, M), dtype=torch.float32) if stats else None
+        q, e = self._act8_empty(x, M, D) if save8 else (None, None)
+        pm = None if ms is None else ms.data_ptr()
+        self._launch('ursa_layer_norm_fwd', dev, px, pa, None if addend is None else z.data_ptr(), y.data_ptr(), pg, pb, pm,
+                     None if ms is None else pm + 4 * M, None if q is None else q.data_ptr(), None if q is None else e.data_ptr(),
+                     M, D, float(eps), dt, DTYPES[pt])
+        return z, y, (None if ms is None else ms[0]), (None if ms is None else ms[1]), q, e
+
+    def layer_norm_backward(self, dy, mean, rstd, gamma=None, *, x=None, q=None, e=None, dz=None, need_dx=True, param_type=None,
+                            need_dgamma=False, need_dbeta=False):
+        """(dx, dgamma, dbeta), None for what is not wanted; dgamma / dbeta of `param_type` (gamma's)."""
+        dt, t, dev = _element_type(dy, 'dy'), dy.dtype, dy.device
+        pt = gamma.dtype if gamma is not None else (param_type or t)
+        if pt not in (t, torch.float32):
+            raise TypeError(f'gamma / beta must be {str(t)[6:]} or float32, got {pt}')
+        if (x is None) == (q is None):
+            raise ValueError('layer_norm_backward wants x or its 8-bit form')
+        M, D = dy.shape
+        pq = pe = None
+        if q is not None:
+            pq, pe = self._act8_ptrs(q, e, M, D, dev)
+        args = (None if x is None else _tptr(x, 'x', t, M * D, dev), pq, pe, _tptr(dy, 'dy', t), _tptr(dz, 'dz', t, M * D, dev, True),
+                _tptr(gamma, 'gamma', pt, D, dev, True), _ptr(mean, 'mean', M, dev), _ptr(rstd, 'rstd', M, dev))
+        dx = torch.empty_like(dy) if need_dx else None
+        dg = dy.new_empty(D, dtype=pt) if need_dgamma else None
+        db = dy.new_empty(D, dtype=pt) if need_dbeta else None
+        ws = dy.new_empty(self.lib.ursa_layer_norm_ws_floats(M, D), dtype=torch.float32) if need_dgamma or need_dbeta else None
+        self._launch('ursa_layer_norm_bwd', dev, *args, *(None if o is None else o.data_ptr() for o in (dx, dg, db, ws)), M, D, dt, DTYPES[pt])
+        return dx, dg, db
+
+    # K17 -----------------------------------------------------------------------------
+    @staticmethod
+    def _act8_empty(x, M, D):
+        blocks = -(-D // ACT8_BLOCK)
+        return x.new_empty((M, blocks * ACT8_BLOCK), dtype=torch.int8), x.new_empty((M, blocks), dtype=torch.int8)
+
+    @staticmethod
+    def _act8_ptrs(q, e, M, D, dev):
+        blocks = -(-D // ACT8_BLOCK)
+        return (_tptr(q, 'q', torch.int8, M * blocks * ACT8_BLOCK, dev), _tptr(e, 'e', torch.int8, M * blocks, dev))
+
+    def act8_pack(self, x):
+        """x [M, D] -> (q [M, P], e [M, P / 32]), P = D rounded up to a multiple of 32."""
+        dt, px = _element_type(x, 'x'), _tptr(x, 'x', x.dtype)
+        if x.dim() != 2:
+            raise ValueError(f'x {tuple(x.shape)} should be [M, D]')
+        M, D = x.shape
+        q, e = self._act8_empty(x, M, D)
+        self._launch('ursa_act8_pack', x.device, px, q.data_ptr(), e.data_ptr(), M, D, dt)
+        return q, e
+
+    def act8_unpack(self, q, e, D, dtype):
+        if dtype not in DTYPES:
+            raise TypeError(f'an activation must be float32, bfloat16 or float16, got {dtype}')
+        M = q.shape[0]
+        pq, pe = self._act8_ptrs(q, e, M, D, q.device)
+        x = q.new_empty((M, D), dtype=dtype)
+        self._launch('ursa_act8_unpack', q.device, pq, pe, x.data_ptr(), M, D, DTYPES[dtype])
+        return x
 
 
 def knobs_kernels():

@@ -1,0 +1,44 @@
+"""Activations kept in 8 bits for the backward pass (K17, include/ursa_hip.h).
+
+`pack(x)` -> `Packed8`, `unpack(p)` -> the tensor it stands for. Each block of 32 consecutive features (last dimension) of a row shares
+one power of two 2^e; a value is a whole number in [-127, 127] times it: x to within 2^e, where the block's largest magnitude is at
+least 63.5 2^e. A value is a number of x's type exactly, so the gradients computed from it have no further rounding. A block with an
+infinity or a NaN in it comes back as NaN. 1.03 bytes a value instead of 4 (fp32) or 2.
+
+`fused_linear.linear_act(..., save8=True)` and `fused_norm.layer_norm(..., save8=True)` keep their inputs so and read them in this form
+in their backward launches; `pack` / `unpack` are for what else a program wants to keep. HIP tensors of float32, bfloat16 or float16
+(no CPU path: a host tensor raises); not differentiable.
+"""
+from typing import NamedTuple
+
+import torch
+
+from . import _native
+
+
+class Packed8(NamedTuple):
+    q: torch.Tensor          # int8 [rows, features rounded up to a multiple of 32]
+    e: torch.Tensor          # int8 [rows, that / 32]
+    shape: torch.Size
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self):
+        return self.q.numel() + self.e.numel()
+
+
+def pack(x):
+    """The 8-bit form of x (at least one dimension; a copy is made first if x is not contiguous)."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError('pack wants a tensor with at least one dimension')
+    with torch.no_grad():
+        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        q, e = _native.default_kernels().act8_pack(x.detach().reshape(rows, x.shape[-1]).contiguous())
+    return Packed8(q, e, x.shape, x.dtype)
+
+
+def unpack(packed):
+    """The tensor that `packed` stands for."""
+    features = packed.shape[-1]
+    with torch.no_grad():
+        return _native.default_kernels().act8_unpack(packed.q, packed.e, features, packed.dtype).view(packed.shape)

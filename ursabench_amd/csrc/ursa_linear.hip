@@ -1,0 +1,494 @@
+// ursa_linear.hip — K15: the linear layer with its epilogue, y = act(x W' + b) + r, and its gradients.
+//
+//   z = x W' + b ; y = act(z) + r            act: none, relu, gelu (z Phi(z)), silu (z sigmoid(z))
+//   dz = dy act'(z) ; dr = dy ; dx = dz W ; dW = dz' x ; db = sum_rows dz
+//
+// All three products are one kernel, C[m][n] = sum_k X(m, k) Y(n, k), whose operands are stored either along the contraction (k
+// contiguous: x and W forward) or across it (W in dx; dz and x in dW). Both go to LDS as rows of 16-bit numbers; the first kind is
+// read as eight consecutive k of a row (ds_read_b128), the second by the transposing LDS read (ds_read_b64_tr_b16), which hands
+// each lane four k of its column. fp32 operands are split while they are staged, v = hi + mid + lo with three bf16 numbers
+// (8 + 8 + 8 bits: exact), and six of the nine partial products are summed in fp32: what is left out is below 2^-24 of |x w|, less
+// than one fp32 rounding, and the bf16 matrix instruction does 16 times the work of the fp32 one. A non-finite fp32 operand
+// makes the sums it enters NaN (its remainder is inf - inf).
+//
+// Sums are fp32; a contraction is cut over workgroups where there are few tiles, and a second launch adds the pieces in order.
+#include "ursa_ops.h"
+
+namespace {
+
+using namespace ursa;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kFlat = 0, kAcross = 1, kAcross8 = 2;      // how an operand is stored: k contiguous; across k; across k in 8 bits
+
+template <int K> struct Kind { static constexpr int value = K; };
+
+template <typename T> struct Arith { typedef T type; };  // what the matrix instruction multiplies
+template <> struct Arith<float> { typedef bf16 type; };
+
+template <typename A>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    if constexpr (__is_same(A, bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float act_value(float z, int act) {
+    switch (act) {
+        case URSA_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+        case URSA_ACT_GELU: return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        case URSA_ACT_SILU: return z / (1.f + expf(-z));
+        default: return z;
+    }
+}
+
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case URSA_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case URSA_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+        case URSA_ACT_SILU: { const float s = 1.f / (1.f + expf(-z)); return s * (1.f + z * (1.f - s)); }
+        default: return 1.f;
+    }
+}
+
+struct Operand {
+    const void* p;               // [rows][k] (kFlat) or [k][rows] (kAcross); kAcross8: int8 [k][pitch]
+    const int8_t* e;             // kAcross8: [k][pitch / 32]
+    int64_t pitch;               // elements from one stored row to the next
+    int rows;
+};
+
+struct Epilogue {
+    void *out, *z;               // [M][N]; z (or NULL): x W' + b before the activation
+    const void *bias, *residual; // [N], [M][N], or NULL
+    float* partial;              // [slices][M][N] when the contraction is cut
+    int act;
+};
+
+struct Shape {
+    int M, N, K;
+    int tiles_m, tiles_n, slices, k_slice;   // k_slice: a multiple of the k step
+};
+
+// one 8-element chunk on its way from memory to LDS
+template <typename T, int KIND> struct Chunk { T v[8]; };
+template <typename T> struct Chunk<T, kAcross8> { int8_t v[8]; int8_t e; };
+
+template <typename T, int KIND>
+__device__ __forceinline__ void load_chunk(Chunk<T, KIND>& c, const Operand& o, int64_t outer, int inner, bool in, int inner_end) {
+    // stored row `outer`, elements inner .. inner + 7, those below inner_end
+    if constexpr (KIND == kAcross8) {
+        const bool ok = in && inner < inner_end;              // rows are padded to whole blocks of 32 with zeros
+        if (ok) {
+            __builtin_memcpy(c.v, (const int8_t*)o.p + outer * o.pitch + inner, 8);
+            c.e = o.e[outer * (o.pitch / kBlock8) + inner / kBlock8];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c.v[i] = 0;
+            c.e = 0;
+        }
+    } else {
+        const T* p = (const T*)o.p + outer * o.pitch + inner;
+        if (in && inner + 8 <= inner_end) {
+            __builtin_memcpy(c.v, p, sizeof c.v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c.v[i] = in && inner + i < inner_end ? p[i] : (T)0.f;
+        }
+    }
+}
+
+template <typename T, int KIND> constexpr int planes() { return __is_same(T, float) && KIND != kAcross8 ? 3 : 1; }
+
+// the chunk as `planes` vectors of eight 16-bit numbers
+template <typename T, int KIND>
+__device__ __forceinline__ void split_chunk(const Chunk<T, KIND>& c, s16x8 (&out)[3]) {
+    typedef typename Arith<T>::type A;
+    if constexpr (KIND == kAcross8) {
+        const float s = c.e == kNonFinite8 ? __builtin_nanf("") : pow2_bits(c.e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[0][i] = __builtin_bit_cast(short, (A)((float)c.v[i] * s));     // exact
+    } else if constexpr (__is_same(T, float)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, (float)c.v[i]);
+            const float r = c.v[i] - __builtin_bit_cast(float, b & 0xffff0000u);    // exact: the low 16 bits
+            const bf16 mid = (bf16)r;
+            const bf16 lo = (bf16)(r - (float)mid);
+            out[0][i] = (short)(b >> 16);
+            out[1][i] = __builtin_bit_cast(short, mid);
+            out[2][i] = __builtin_bit_cast(short, lo);
+        }
+    } else {
+        __builtin_memcpy(&out[0], c.v, 16);
+    }
+}
+
+// LDS places of a 16-byte piece. kFlat: [rows][BK], the pieces of a row permuted so that eight rows' reads of one k fall into
+// different banks; kAcross: [BK][R], 32-byte slots permuted by k so that the four rows of a transposing read do.
+template <int BK> __device__ __forceinline__ int flat_at(int row, int piece) {
+    return BK == 64 ? row * 64 + ((piece ^ (row & 7)) << 3) : row * 32 + ((piece ^ ((row >> 1) & 3)) << 3);
+}
+template <int R> __device__ __forceinline__ int across_at(int k, int slot) { return k * R + ((slot ^ (k & (R >= 128 ? 7 : 3))) << 4); }
+
+// the fragment of 16 rows from row0, k .. k + 31: lane l holds row l % 16, k + 8 (l / 16) .. + 7
+template <int KIND, int BK, int R>
+__device__ __forceinline__ s16x8 fragment(const short* plane, int row0, int k, int lane) {
+    if constexpr (KIND == kFlat) {
+        return *(const s16x8*)(plane + flat_at<BK>(row0 + (lane & 15), (k >> 3) + (lane >> 4)));
+    } else {
+        const int kr = k + 8 * (lane >> 4) + ((lane & 15) >> 2), in = (lane & 3) << 2;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(plane + across_at<R>(kr, row0 >> 4) + in));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(plane + across_at<R>(kr + 4, row0 >> 4) + in));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int valid, const float (&v)[4]) { store_piece<T, 4>(p, valid, v); }
+
+// four consecutive n of one m through the epilogue
+template <typename T>
+__device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, int N, const float (&acc)[4]) {
+    const int valid = N - n;
+    const int64_t at = m * N + n;
+    float v[4], t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = acc[i];
+    if (ep.bias) {
+        load_piece<T, 4>((const T*)ep.bias + n, valid, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += t[i];
+    }
+    if (ep.z) store4<T>((T*)ep.z + at, valid, v);
+    if (ep.act) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], ep.act);
+    }
+    if (ep.residual) {
+        load_piece<T, 4>((const T*)ep.residual + at, valid, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += t[i];
+    }
+    store4<T>((T*)ep.out + at, valid, v);
+}
+
+// tile of this workgroup: workgroups go round the 8 XCDs, so every eighth is a neighbour in one L2; those take consecutive tiles, and
+// consecutive tiles run down 8 rows of tiles before they step right, so that both operands of a group of tiles stay in that L2
+__device__ __forceinline__ void tile_of(int id, const Shape& s, int& tm, int& tn) {
+    const int n = s.tiles_m * s.tiles_n, per = n >> 3, rem = n & 7, x = id & 7, i = id >> 3;
+    const int t = x < rem ? x * (per + 1) + i : rem * (per + 1) + (x - rem) * per + i;
+    const int band = 8 * s.tiles_n, b = t / band, rows = s.tiles_m - 8 * b < 8 ? s.tiles_m - 8 * b : 8, j = t - b * band;
+    tm = 8 * b + j % rows;
+    tn = j / rows;
+}
+
+// TILE x TILE outputs by four waves (2 x 2), operands through registers (types that are converted, rows at any alignment)
+template <typename T, int XK, int YK, int TILE>
+__global__ __launch_bounds__(256) void k_product(Operand X, Operand Y, Shape s, Epilogue ep) {
+    typedef typename Arith<T>::type A;
+    constexpr int BK = __is_same(T, float) ? 32 : 64, PX = planes<T, XK>(), PY = planes<T, YK>();
+    constexpr int CH = TILE * BK / 8 / 256, F = TILE / 32;          // chunks a thread stages per operand; 16-row fragments a wave has
+    __shared__ __attribute__((aligned(16))) short xs[PX][TILE * BK], ys[PY][TILE * BK];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int tm, tn;
+    tile_of(blockIdx.x, s, tm, tn);
+    const int m0 = tm * TILE, n0 = tn * TILE;
+    const int k_begin = blockIdx.y * s.k_slice, k_end = s.K - k_begin < s.k_slice ? s.K : k_begin + s.k_slice;
+    const int wm = (wave & 1) * (TILE / 2), wn = (wave >> 1) * (TILE / 2);
+    Chunk<T, XK> cx[CH];
+    Chunk<T, YK> cy[CH];
+    auto fetch = [&](auto& c, const Operand& o, auto kind, int r0, int k0) {
+        constexpr int KIND = decltype(kind)::value;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int id = i * 256 + tid;
+            if constexpr (KIND == kFlat) {
+                const int row = r0 + id / (BK / 8), k = k0 + id % (BK / 8) * 8;
+                load_chunk<T, KIND>(c[i], o, row, k, row < o.rows, k_end);
+            } else {
+                const int k = k0 + id / (TILE / 8), row = r0 + id % (TILE / 8) * 8;
+                load_chunk<T, KIND>(c[i], o, k, row, k < k_end, o.rows);
+            }
+        }
+    };
+    auto stage = [&](auto& c, auto& lds, auto kind) {
+        constexpr int KIND = decltype(kind)::value, P = planes<T, KIND>();
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int id = i * 256 + tid;
+            s16x8 out[3];
+            split_chunk<T, KIND>(c[i], out);
+            int at;
+            if constexpr (KIND == kFlat) at = flat_at<BK>(id / (BK / 8), id % (BK / 8));
+            else at = across_at<TILE>(id / (TILE / 8), id % (TILE / 8) >> 1) + (id % (TILE / 8) & 1) * 8;
+#pragma unroll
+            for (int p = 0; p < P; ++p) *(s16x8*)(&lds[p][at]) = out[p];
+        }
+    };
+    f32x4 acc[F][F] = {};
+    if (k_begin < k_end) {
+        fetch(cx, X, Kind<XK>{}, m0, k_begin);
+        fetch(cy, Y, Kind<YK>{}, n0, k_begin);
+    }
+    for (int k = k_begin; k < k_end; k += BK) {
+        __syncthreads();
+        stage(cx, xs, Kind<XK>{});
+        stage(cy, ys, Kind<YK>{});
+        __syncthreads();
+        if (k + BK < k_end) {
+            fetch(cx, X, Kind<XK>{}, m0, k + BK);
+            fetch(cy, Y, Kind<YK>{}, n0, k + BK);
+        }
+#pragma unroll
+        for (int kk = 0; kk < BK; kk += 32) {
+            s16x8 fx[PX][F];
+#pragma unroll
+            for (int p = 0; p < PX; ++p)
+#pragma unroll
+                for (int i = 0; i < F; ++i) fx[p][i] = fragment<XK, BK, TILE>(xs[p], wm + 16 * i, kk, lane);
+#pragma unroll
+            for (int j = 0; j < F; ++j) {
+                s16x8 fy[PY];
+#pragma unroll
+                for (int p = 0; p < PY; ++p) fy[p] = fragment<YK, BK, TILE>(ys[p], wn + 16 * j, kk, lane);
+#pragma unroll
+                for (int px = PX - 1; px >= 0; --px)                 // small products first
+#pragma unroll
+                    for (int py = PY - 1; py >= 0; --py)
+                        if (px + py <= 2)
+#pragma unroll
+                            for (int i = 0; i < F; ++i) acc[j][i] = mfma<A>(fy[py], fx[px][i], acc[j][i]);
+            }
+        }
+    }
+    // accumulator of (fy, fx): lane l holds m = l % 16 and n = 4 (l / 16) .. + 3
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+        const int m = m0 + wm + 16 * i + (lane & 15);
+        if (m >= s.M) continue;
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+            const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
+            if (n >= s.N) continue;
+            const float v[4] = {acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]};
+            if (ep.partial) store_piece<float, 4>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
+            else finish4<T>(ep, m, n, s.N, v);
+        }
+    }
+}
+
+// the slices of a cut contraction, added in ascending order, and the epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
+    const int quads = (s.N + 3) / 4;
+    const int64_t n_q = (int64_t)s.M * quads;
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < n_q; id += (int64_t)gridDim.x * 256) {
+        const int64_t m = id / quads;
+        const int n = (int)(id - m * quads) * 4;
+        float v[4] = {}, t[4];
+        for (int z = 0; z < s.slices; ++z) {
+            load_piece<float, 4>(ep.partial + (z * (int64_t)s.M + m) * s.N + n, s.N - n, t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += t[i];
+        }
+        finish4<T>(ep, m, n, s.N, v);
+    }
+}
+
+// dz = dy act'(z) and the slices' sums of its columns. A workgroup: 32 column pieces x 8 rows at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, float* __restrict__ partial,
+                                                  int64_t M, int N, int act, int rows) {
+    constexpr int V = Piece<T>::kN;
+    __shared__ float red[8][32 * V];
+    const int piece = threadIdx.x & 31, strand = threadIdx.x >> 5;
+    const int64_t n = ((int64_t)blockIdx.x * 32 + piece) * V, left = N - n;
+    const int64_t begin = (int64_t)blockIdx.y * rows, end = begin + rows < M ? begin + rows : M;
+    float s[V] = {};
+    if (left > 0)
+        for (int64_t m = begin + strand; m < end; m += 8) {
+            float g[V];
+            load_piece<T, V>(dy + m * N + n, left, g);
+            if (z) {
+                float a[V];
+                load_piece<T, V>(z + m * N + n, left, a);
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] *= act_slope(a[i], act);
+                store_piece<T, V>(dz + m * N + n, left, g);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] += g[i];               // before dz is rounded to its type
+        }
+    if (!partial) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[strand][piece * V + i] = s[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += 256) {
+        float t = red[0][c];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) t += red[w][c];
+        const int64_t col = (int64_t)blockIdx.x * 32 * V + c;
+        if (col < N) partial[(int64_t)blockIdx.y * N + col] = t;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_columns_join(const float* __restrict__ partial, int slices, int N, T* __restrict__ out) {
+    __shared__ float s[8][32];
+    const int col = threadIdx.x & 31, strand = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
+    float acc = 0.f;
+    if (n < N)
+        for (int g = strand; g < slices; g += 8) acc += partial[(int64_t)g * N + n];
+    s[strand][col] = acc;
+    __syncthreads();
+    if (strand || n >= N) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) acc += s[k][col];
+    out[n] = (T)acc;
+}
+
+// ---- plans ----------------------------------------------------------------------------------
+struct Plan {
+    int tile;
+    Shape s;
+    int64_t ws() const { return s.slices > 1 ? (int64_t)s.slices * s.M * s.N * 4 : 0; }
+};
+
+// 128 x 128 tiles where they give every CU one, 64 x 64 otherwise; a contraction is cut while there are fewer than 512 workgroups
+// (two for each CU) and each keeps eight k steps
+Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+    Plan p;
+    const int bk = dtype == URSA_F32 ? 32 : 64;
+    const int64_t big = ((M + 127) / 128) * ((N + 127) / 128);
+    p.tile = big >= 256 ? 128 : 64;
+    p.s.M = (int)M, p.s.N = (int)N, p.s.K = (int)K;
+    p.s.tiles_m = (int)((M + p.tile - 1) / p.tile), p.s.tiles_n = (int)((N + p.tile - 1) / p.tile);
+    const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, steps = (K + bk - 1) / bk;
+    int64_t cut = tiles < 512 && tiles ? 512 / tiles : 1;
+    if (cut > steps / 8) cut = steps / 8;
+    if (cut > 16) cut = 16;
+    if (cut < 1) cut = 1;
+    const int64_t per = (steps + cut - 1) / cut;
+    p.s.k_slice = (int)((per > 0 ? per : 1) * bk);
+    p.s.slices = per > 0 ? (int)((steps + per - 1) / per) : 1;
+    return p;
+}
+
+template <typename T, int XK, int YK>
+int product(const Operand& x, const Operand& y, const Plan& p, Epilogue ep, hipStream_t st) {
+    if (p.s.slices == 1) ep.partial = nullptr;
+    const dim3 grid((unsigned)(p.s.tiles_m * p.s.tiles_n), (unsigned)p.s.slices);
+    if (p.tile == 128) hipLaunchKernelGGL((k_product<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
+    else hipLaunchKernelGGL((k_product<T, XK, YK, 64>), grid, dim3(256), 0, st, x, y, p.s, ep);
+    int rc = launch_status();
+    if (rc || p.s.slices == 1) return rc;
+    const int64_t quads = (int64_t)p.s.M * ((p.s.N + 3) / 4), blocks = (quads + 255) / 256;
+    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, p.s, ep);
+    return launch_status();
+}
+
+#define URSA_LINEAR_TYPES(dtype, call) (dtype == URSA_F32 ? call(float) : dtype == URSA_BF16 ? call(bf16) : call(f16))
+
+// 0: go on; 1: nothing to write; < 0: an error
+int check(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+    if (dtype < URSA_F32 || dtype > URSA_F16) return URSA_EFLAGS;
+    const int64_t most = INT32_MAX - 256;
+    if (M < 0 || N < 0 || K < 0 || M > most || N > most || K > most) return URSA_ESIZE;
+    if (((M + 63) / 64) * ((N + 63) / 64) > INT32_MAX) return URSA_ESIZE;
+    return M == 0 || N == 0 ? 1 : 0;
+}
+
+bool misaligned(int32_t dtype, uintptr_t pointers) { return pointers & (uintptr_t)(element_size(dtype) - 1); }
+
+int act_rows(int64_t M, int64_t N, int32_t dtype) {       // rows of a slice of k_act_grad: about 2,048 workgroups, 8 rows at least
+    const int64_t cols = (N + 32 * 16 / element_size(dtype) - 1) / (32 * 16 / element_size(dtype));
+    int64_t slices = 2048 / (cols ? cols : 1);
+    if (slices < 1) slices = 1;
+    if (slices > 256) slices = 256;
+    int64_t rows = (M + slices - 1) / slices;
+    rows = (rows + 7) / 8 * 8;
+    return (int)(rows < 8 ? 8 : rows);
+}
+
+template <typename T>
+int act_grad(dim3 grid, const T* dy, const T* z, T* dz, T* db, float* partial, int64_t M, int N, int act, int rows, int slices, hipStream_t st) {
+    hipLaunchKernelGGL(k_act_grad<T>, grid, dim3(256), 0, st, dy, z, dz, partial, M, N, act, rows);
+    const int rc = launch_status();
+    if (rc || !db) return rc;
+    hipLaunchKernelGGL(k_columns_join<T>, dim3((unsigned)((N + 31) / 32)), dim3(256), 0, st, (const float*)partial, slices, N, db);
+    return launch_status();
+}
+
+}  // namespace
+
+extern "C" int64_t ursa_linear_ws_bytes(int32_t pass, int64_t M, int64_t N, int64_t K, int32_t dtype) {
+    if (check(M, N, K, dtype)) return 0;
+    switch (pass) {
+        case URSA_LINEAR_FWD: return plan_of(M, N, K, dtype).ws();
+        case URSA_LINEAR_DX: return K ? plan_of(M, K, N, dtype).ws() : 0;
+        case URSA_LINEAR_DW: return K ? plan_of(N, K, M, dtype).ws() : 0;
+        case URSA_LINEAR_ACT_GRAD: { const int r = act_rows(M, N, dtype); return (M + r - 1) / r * N * 4; }
+    }
+    return 0;
+}
+
+extern "C" int ursa_linear_act(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, void* ws, int64_t M,
+                               int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream) {
+    if (act < URSA_ACT_NONE || act > URSA_ACT_SILU) return URSA_EFLAGS;
+    if (int rc = check(M, N, K, dtype)) return rc > 0 ? URSA_OK : rc;
+    const Plan p = plan_of(M, N, K, dtype);
+    if ((K && (!x || !w)) || !y || (p.ws() && !ws)) return URSA_ENULL;
+    if (misaligned(dtype, (uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)z) || (uintptr_t)ws & 3) return URSA_EALIGN;
+    const Operand X{x, nullptr, K, (int)M}, Y{w, nullptr, K, (int)N};
+    const Epilogue ep{y, z, bias, residual, (float*)ws, act};
+#define URSA_CALL(T) product<T, kFlat, kFlat>(X, Y, p, ep, (hipStream_t)stream)
+    return URSA_LINEAR_TYPES(dtype, URSA_CALL);
+#undef URSA_CALL
+}
+
+extern "C" int ursa_linear_dx(const void* dz, const void* w, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, ursa_stream_t stream) {
+    if (int rc = check(M, K, N, dtype)) return rc > 0 ? URSA_OK : rc;
+    const Plan p = plan_of(M, K, N, dtype);
+    if ((N && (!dz || !w)) || !dx || (p.ws() && !ws)) return URSA_ENULL;
+    if (misaligned(dtype, (uintptr_t)dz | (uintptr_t)w | (uintptr_t)dx) || (uintptr_t)ws & 3) return URSA_EALIGN;
+    const Operand X{dz, nullptr, N, (int)M}, Y{w, nullptr, K, (int)K};
+    const Epilogue ep{dx, nullptr, nullptr, nullptr, (float*)ws, URSA_ACT_NONE};
+#define URSA_CALL(T) product<T, kFlat, kAcross>(X, Y, p, ep, (hipStream_t)stream)
+    return URSA_LINEAR_TYPES(dtype, URSA_CALL);
+#undef URSA_CALL
+}
+
+extern "C" int ursa_linear_dw(const void* dz, const void* x, const int8_t* q, const int8_t* e, void* dw, void* ws, int64_t M, int64_t N, int64_t K,
+                              int32_t dtype, ursa_stream_t stream) {
+    if (int rc = check(N, K, M, dtype)) return rc > 0 ? URSA_OK : rc;
+    const Plan p = plan_of(N, K, M, dtype);
+    if ((M && (!dz || (x != nullptr) == (q != nullptr) || (q != nullptr) != (e != nullptr))) || !dw || (p.ws() && !ws)) return URSA_ENULL;
+    if (misaligned(dtype, (uintptr_t)dz | (uintptr_t)x | (uintptr_t)dw) || (uintptr_t)q & 15 || (uintptr_t)ws & 3) return URSA_EALIGN;
+    const int64_t qpitch = (K + kBlock8 - 1) / kBlock8 * kBlock8;
+    const Operand X{dz, nullptr, N, (int)N}, Y{q ? (const void*)q : x, e, q ? qpitch : K, (int)K};
+    const Epilogue ep{dw, nullptr, nullptr, nullptr, (float*)ws, URSA_ACT_NONE};
+#define URSA_CALL(T) (q ? product<T, kAcross, kAcross8>(X, Y, p, ep, (hipStream_t)stream) : product<T, kAcross, kAcross>(X, Y, p, ep, (hipStream_t)stream))
+    return URSA_LINEAR_TYPES(dtype, URSA_CALL);
+#undef URSA_CALL
+}
+
+extern "C" int ursa_linear_act_grad(const void* dy, const void* z, void* dz, void* db, void* ws, int64_t M, int64_t N, int32_t dtype, int32_t act,
+                                    ursa_stream_t stream) {
+    if (act < URSA_ACT_NONE || act > URSA_ACT_SILU) return URSA_EFLAGS;
+    if (int rc = check(M, N, 0, dtype)) return rc > 0 ? URSA_OK : rc;
+    if (!dy || (z != nullptr) != (dz != nullptr) || (act != URSA_ACT_NONE) != (z != nullptr) || (db && !ws)) return URSA_ENULL;
+    if (misaligned(dtype, (uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz | (uintptr_t)db) || (uintptr_t)ws & 3) return URSA_EALIGN;
+    const int rows = act_rows(M, N, dtype), slices = (int)((M + rows - 1) / rows);
+    float* part = db ? (float*)ws : nullptr;
+    const int per = 32 * 16 / (int)element_size(dtype);
+    const dim3 grid((unsigned)((N + per - 1) / per), (unsigned)slices);
+#define URSA_CALL(T) act_grad<T>(grid, (const T*)dy, (const T*)z, (T*)dz, (T*)db, part, M, (int)N, act, rows, slices, (hipStream_t)stream)
+    return URSA_LINEAR_TYPES(dtype, URSA_CALL);
+#undef URSA_CALL
+}

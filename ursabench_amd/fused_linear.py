@@ -1,0 +1,122 @@
+"""The linear layer with its epilogue, act(x W' + b) + residual, as gfx950 launches (K15, include/ursa_hip.h).
+
+`linear_act(fc, x, activation, residual)` stands for `F.relu(self.fc1(x))` and the like (URSABench/models/mlp.py:20-23) and for the
+`out += residual` behind it. `fc` stays a plain `nn.Linear` (same state_dict keys, initialisation and optimizer view); only the
+launches differ:
+
+  forward           one launch: product, bias, activation and residual (two where the contraction is cut over workgroups)
+  backward          the activation's gradient and the bias gradient in one pass over dy, then one launch for dx and one for dW
+
+float32, bfloat16 and float16, any sizes and leading dimensions, on a HIP device. Operands that are not contiguous are copied first.
+Anything else - host tensors, other or mixed types, autocast, a subclass with a forward of its own, hooks on `fc` - takes
+`fc(x)`, the activation and the sum as stock ops, where `save8` keeps x itself. Double backward is not offered. On a HIP tensor the
+fused path needs csrc/libursa_hip.so (no silent fallback: a missing library raises).
+
+`save8=True` keeps the x that the weight gradient needs in 8 bits (K17, `act8`) instead of the tensor: a quarter / half of its
+memory, dW as if x had been rounded to 8 bits per block of 32 features; y, dx and db do not change.
+
+`URSA_FUSED_LINEAR=0` / `enabled(False)` selects the stock ops in `linear_act` everywhere (A/B runs). `URSA_LINEAR_IN_MODELS=1` /
+`in_models(True)` makes `models.MLP` and `models.LeNet5` call it (off by default: their products stay the library's, bit for bit).
+"""
+import os
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_on = os.environ.get('URSA_FUSED_LINEAR', '1') != '0'
+_models = os.environ.get('URSA_LINEAR_IN_MODELS', '0') == '1'
+_STOCK = {None: lambda z: z, 'relu': F.relu, 'gelu': F.gelu, 'silu': F.silu}
+
+
+def enabled(flag=None):
+    """Query / set whether `linear_act` takes this module's launches at all (process-wide); returns the previous value."""
+    global _on
+    old = _on
+    if flag is not None:
+        _on = bool(flag)
+    return old
+
+
+def in_models(flag=None):
+    """Query / set whether models.MLP / models.LeNet5 run their linear layers through `linear_act` (process-wide)."""
+    global _models
+    old = _models
+    if flag is not None:
+        _models = bool(flag)
+    return old
+
+
+class _LinearAct(torch.autograd.Function):
+    """y = act(x w' + b) + r for 2-d contiguous x."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, r, activation, save8):
+        K = _native.default_kernels()
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        z = None
+        if activation is not None and (need_x or need_w or need_b):
+            y, z = K.linear_act(x, w, b, r, activation=activation, save_z=True)
+        else:
+            y = K.linear_act(x, w, b, r, activation=activation)
+        q = e = None
+        if need_w and save8:
+            q, e = K.act8_pack(x)
+        ctx.save_for_backward(x if need_w and not save8 else None, w if need_x else None, z, q, e)
+        ctx.activation, ctx.in_features = activation, x.shape[1]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, z, q, e = ctx.saved_tensors
+        K = _native.default_kernels()
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dy = dy.contiguous()
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            dz, db = K.linear_act_grad(dy, z, activation=ctx.activation, bias_grad=need_b)
+            if need_x:
+                dx = K.linear_dx(dz, w)
+            if need_w:
+                dw = K.linear_dw(dz, x) if q is None else K.linear_dw(dz, q=q, e=e, in_features=ctx.in_features)
+        return dx, dw, db, (dy if need_r else None), None, None
+
+
+def _fusable(fc, x, residual):
+    w, b = fc.weight, fc.bias
+    return (_on and x.is_cuda and x.dtype in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
+            and type(fc).forward is nn.Linear.forward and not fc._forward_hooks and not fc._forward_pre_hooks
+            and not fc._backward_hooks and not fc._backward_pre_hooks
+            and w.dtype == x.dtype and w.device == x.device and x.shape[-1] == w.shape[1] and w.numel() > 0
+            and (b is None or (b.dtype == x.dtype and b.device == x.device))
+            and (residual is None or (residual.dtype == x.dtype and residual.device == x.device)))
+
+
+def linear_act(fc, x, activation=None, residual=None, *, save8=False):
+    """act(fc(x)) + residual. activation: None, 'relu', 'gelu' (the exact one, z Phi(z)) or 'silu'; residual: None or a tensor of
+    the result's shape. save8: keep x in 8 bits for the weight gradient (module docstring)."""
+    if activation not in _STOCK:
+        raise ValueError(f'activation must be one of {list(_STOCK)}, got {activation!r}')
+    if not isinstance(fc, nn.Linear):
+        raise TypeError(f'linear_act wants an nn.Linear, got {type(fc).__name__}')
+    shape = x.shape[:-1] + (fc.weight.shape[0],)
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f'residual {tuple(residual.shape)} should have the result\'s shape {tuple(shape)}')
+    if not _fusable(fc, x, residual):
+        y = _STOCK[activation](fc(x))
+        return y if residual is None else y + residual
+    w, b = fc.weight, fc.bias
+    flat = x.dim() == 2
+    x2 = (x if flat else x.reshape(-1, x.shape[-1])).contiguous()
+    r2 = None if residual is None else (residual if flat else residual.reshape(-1, shape[-1])).contiguous()
+    w, b = w.contiguous(), None if b is None else b.contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
+                                    or (r2 is not None and r2.requires_grad)):
+        y = _LinearAct.apply(x2, w, b, r2, activation, save8)
+    else:
+        y = _native.default_kernels().linear_act(x2, w, b, r2, activation=activation)
+    return y if flat else y.view(shape)

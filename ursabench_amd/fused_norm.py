@@ -1,0 +1,139 @@
+"""Layer norm and the residual sum in front of it as gfx950 launches (K16, include/ursa_hip.h): what `fused_bn` is to the
+convolutional blocks, for networks that normalise each row by itself.
+
+`layer_norm(ln, x)` stands for `ln(x)`; `add_layer_norm(ln, (a, b))` for `z = a + b; return z, ln(z)`. `ln` stays a plain
+`nn.LayerNorm` (state_dict keys, eps, no weight or no bias included); only the launches differ:
+
+  forward           one launch: sum, statistics, scale and shift (and the 8-bit copy of z with `save8`)
+  backward          one launch for dx (the gradient that reaches z past the norm added in it) and the columns' partial sums, and a
+                    small one that adds those in a fixed order
+
+float32, bfloat16 and float16 on a HIP device, parameters of the same type or float32, any width. Inputs that are not contiguous are
+copied first. Anything else - host tensors, other types, autocast, empty tensors, a subclass with a forward of its own, hooks on
+`ln` - takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward is not offered. On a HIP tensor the
+fused path needs csrc/libursa_hip.so (no silent fallback: a missing library raises).
+
+`save8=True` keeps the normalised input in 8 bits for the backward pass (K17, `act8`): gradients are the formula's with xhat
+taken from those values; mean and 1 / std are the exact input's. `URSA_FUSED_NORM=0` / `enabled(False)` selects the stock path
+everywhere (A/B runs).
+"""
+import os
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_on = os.environ.get('URSA_FUSED_NORM', '1') != '0'
+
+
+def enabled(flag=None):
+    """Query / set the process-wide switch; returns the previous value."""
+    global _on
+    old = _on
+    if flag is not None:
+        _on = bool(flag)
+    return old
+
+
+def _gradients(ctx, dy, dz, need_x, need_w, need_b):
+    z, q, e, mean, rstd, w = ctx.saved_tensors
+    return _native.default_kernels().layer_norm_backward(
+        dy.contiguous(), mean, rstd, w, x=z, q=q, e=e, dz=None if dz is None else dz.contiguous(), need_dx=need_x,
+        param_type=ctx.param_type, need_dgamma=need_w, need_dbeta=need_b)
+
+
+class _Norm(torch.autograd.Function):
+    """y = layer_norm(x) for 2-d contiguous x."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps, save8):
+        z, y, mean, rstd, q, e = _native.default_kernels().layer_norm(x, w, b, eps=eps, stats=True, save8=save8)
+        ctx.save_for_backward(None if save8 else z, q, e, mean, rstd, w)
+        ctx.param_type = None if b is None else b.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return (*_gradients(ctx, dy, None, *ctx.needs_input_grad[:3]), None, None)
+
+
+class _AddNorm(torch.autograd.Function):
+    """(z, y) = (a + b, layer_norm(a + b)); d(a) = d(b) = dz + the norm's gradient, in the same launch."""
+
+    @staticmethod
+    def forward(ctx, a, b, w, bias, eps, save8):
+        ctx.set_materialize_grads(False)                 # an unused output's gradient arrives as None, not as zeros
+        z, y, mean, rstd, q, e = _native.default_kernels().layer_norm(a, w, bias, eps=eps, addend=b, stats=True, save8=save8)
+        ctx.save_for_backward(None if save8 else z, q, e, mean, rstd, w)
+        ctx.param_type = None if bias is None else bias.dtype
+        return z, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dz, dy):
+        need_a, need_b, need_w, need_bias = ctx.needs_input_grad[:4]
+        if dy is None:                                   # y unused: only the sum's own gradient flows
+            return dz if need_a else None, dz if need_b else None, None, None, None, None
+        dx, dw, db = _gradients(ctx, dy, dz, need_a or need_b, need_w, need_bias)
+        return dx if need_a else None, dx if need_b else None, dw, db, None, None
+
+
+def _fusable(ln, x):
+    n = len(ln.normalized_shape)
+    params = [p for p in (ln.weight, ln.bias) if p is not None]
+    return (_on and x.is_cuda and x.dtype in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
+            and type(ln).forward is nn.LayerNorm.forward and not ln._forward_hooks and not ln._forward_pre_hooks
+            and not ln._backward_hooks and not ln._backward_pre_hooks
+            and x.dim() >= n and tuple(x.shape[x.dim() - n:]) == tuple(ln.normalized_shape) and ln.eps >= 0
+            and all(p.device == x.device and p.dtype in (x.dtype, torch.float32) and p.dtype == params[0].dtype for p in params))
+
+
+def _rows(ln, x):
+    width = 1
+    for d in ln.normalized_shape:
+        width *= d
+    return x.reshape(-1, width).contiguous()
+
+
+def _params(ln):
+    return tuple(None if p is None else p.reshape(-1).contiguous() for p in (ln.weight, ln.bias))
+
+
+def _recorded(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def layer_norm(ln, x, *, save8=False):
+    """ln(x). save8: keep x in 8 bits for the backward pass (module docstring)."""
+    if not isinstance(ln, nn.LayerNorm):
+        raise TypeError(f'layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
+    if not _fusable(ln, x):
+        return ln(x)
+    x2, (w, b) = _rows(ln, x), _params(ln)
+    if _recorded(x2, w, b):
+        y = _Norm.apply(x2, w, b, ln.eps, save8)
+    else:
+        y = _native.default_kernels().layer_norm(x2, w, b, eps=ln.eps)[1]
+    return y.view(x.shape)
+
+
+def add_layer_norm(ln, x, *, save8=False):
+    """(z, ln(z)) for z = a + b of the pair x = (a, b); of a tensor x: (x, ln(x)). z is rounded to the tensors' type before it is
+    normalised, as the two stock ops would do."""
+    if not isinstance(x, tuple):
+        return x, layer_norm(ln, x, save8=save8)
+    if not isinstance(ln, nn.LayerNorm):
+        raise TypeError(f'add_layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
+    a, b = x
+    if not (_fusable(ln, a) and b.shape == a.shape and b.dtype == a.dtype and b.device == a.device):
+        z = a + b
+        return z, layer_norm(ln, z, save8=save8)
+    a2, b2, (w, bias) = _rows(ln, a), _rows(ln, b), _params(ln)
+    if _recorded(a2, b2, w, bias):
+        z, y = _AddNorm.apply(a2, b2, w, bias, ln.eps, save8)
+    else:
+        z, y = _native.default_kernels().layer_norm(a2, w, bias, eps=ln.eps, addend=b2)[:2]
+    return z.view(a.shape), y.view(a.shape)

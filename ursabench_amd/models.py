@@ -1,6 +1,6 @@
 """The networks the benchmark configurations name (BASELINE.json `configs`), as plain nn.Modules.
 
-Linear layers stay stock PyTorch-ROCm (rocBLAS), and so do convolutions outside a gradient-recording step. Two things these
+Linear layers stay stock PyTorch-ROCm (rocBLAS; MLP and LeNet5 take K15's launches with `fused_linear.in_models(True)`), and so do convolutions outside a gradient-recording step. Two things these
 modules do differently from the reference's on a HIP device: the convolutions of a training step (`fused_conv.Conv2d`: K8 / K9
 forward and input gradient, K7 weight gradient - every convolution of the BasicBlock ResNets, instead of MIOpen's launches) and
 `relu(bn(x))`: every BatchNorm of the
@@ -22,12 +22,20 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import fused_block, fused_bottleneck
+from . import fused_block, fused_bottleneck, fused_linear
 from .fused_bn import add_bn_relu, bn_relu
 from .fused_conv import Conv2d
 
 __all__ = ['LeNet5', 'MLP', 'MLP_dropout', 'PreResNet', 'PreResNet_dropout', 'WideResNet', 'MLP200MNIST',
            'MLP200MNIST_dropout', 'LeNet5MNIST', 'PreResNet8', 'PreResNet20', 'PreResNet164', 'WideResNet28x10']
+
+
+def _dense3(net, x):
+    """fc3(relu(fc2(relu(fc1(x))))): stock ops, or K15's launches when fused_linear.in_models() says so."""
+    if fused_linear.in_models():
+        h = fused_linear.linear_act(net.fc2, fused_linear.linear_act(net.fc1, x, 'relu'), 'relu')
+        return fused_linear.linear_act(net.fc3, h)
+    return net.fc3(F.relu(net.fc2(F.relu(net.fc1(x)))))
 
 
 class LeNet5(nn.Module):
@@ -43,7 +51,7 @@ class LeNet5(nn.Module):
         x = F.max_pool2d(F.relu(self.conv1(x)), 2)
         x = F.max_pool2d(F.relu(self.conv2(x)), 2)
         x = x.flatten(1)
-        return self.fc3(F.relu(self.fc2(F.relu(self.fc1(x)))))
+        return _dense3(self, x)
 
 
 class MLP(nn.Module):
@@ -55,8 +63,7 @@ class MLP(nn.Module):
         self.fc3 = nn.Linear(hidden_size, num_classes)
 
     def forward(self, x):
-        h = F.relu(self.fc1(x.view(-1, self.input_dim)))
-        return self.fc3(F.relu(self.fc2(h)))
+        return _dense3(self, x.view(-1, self.input_dim))
 
 
 class MLP_dropout(nn.Module):
