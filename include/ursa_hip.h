@@ -632,11 +632,11 @@ int ursa_bn_relu_pool_bwd_f32(const float* z, const float* dpooled, const float*
  *   aligned to an element. z [M][N] or NULL receives x W' + b, rounded to the type, for the backward pass. Sums are fp32; the
  *   activation sees the sum before it is rounded. fp32 operands are multiplied as three bf16 numbers each (exact split, products
  *   down to 2^-24 of |x w|): a non-finite one gives NaN in every sum that it enters.
- *   ursa_linear_act_grad   dz = dy act'(z) (act != URSA_ACT_NONE: z and dz given) and db = its column sums (fp32 before dz is
- *                          rounded; db NULL: not wanted). act == URSA_ACT_NONE: z, dz NULL, db = column sums of dy.
- *   ursa_linear_dx         dx [M][K] = dz W
- *   ursa_linear_dw         dw [N][K] = dz' x, x either as `x` or as its 8-bit form (`q`, `e`; K17), the other NULL. M = 0: zeros.
- *   ws: ursa_linear_ws_bytes(pass, M, N, K, dtype) bytes of scratch private to the call (0: may be NULL); contents need not be set.
+ *   backward: dz = dy act'(z) (z as the forward call gave it; rounded to the type for the products, not for db), dx [M][K] = dz W,
+ *   dw [N][K] = dz' x, db [N] = column sums of dz; each of dx, dw, db may be NULL: not wanted. x: as `x`, or as its 8-bit form (`q`,
+ *   `e`; K17), the other NULL. w is read for dx, x for dw, z with an activation. M = 0: dw and db are zeros.
+ *   ws: ursa_linear_ws_bytes / ursa_linear_bwd_ws_bytes bytes of scratch, 16-byte aligned, private to the call (0: may be NULL); its
+ *   contents need not be set.
  * The same call gives the same bits every time (no atomics).
  */
 #define URSA_F32  0
@@ -646,18 +646,12 @@ int ursa_bn_relu_pool_bwd_f32(const float* z, const float* dpooled, const float*
 #define URSA_ACT_RELU 1
 #define URSA_ACT_GELU 2 /* z Phi(z) */
 #define URSA_ACT_SILU 3 /* z / (1 + exp(-z)) */
-#define URSA_LINEAR_FWD 0
-#define URSA_LINEAR_DX  1
-#define URSA_LINEAR_DW  2
-#define URSA_LINEAR_ACT_GRAD 3
-int64_t ursa_linear_ws_bytes(int32_t pass, int64_t M, int64_t N, int64_t K, int32_t dtype);
+int64_t ursa_linear_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype);
+int64_t ursa_linear_bwd_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, int32_t dx, int32_t dw, int32_t db);
 int ursa_linear_act(const void* x, const void* w, const void* bias /* or NULL */, const void* residual /* or NULL */, void* y,
                     void* z /* or NULL */, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream);
-int ursa_linear_act_grad(const void* dy, const void* z, void* dz, void* db /* or NULL */, void* ws, int64_t M, int64_t N, int32_t dtype,
-                         int32_t act, ursa_stream_t stream);
-int ursa_linear_dx(const void* dz, const void* w, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, ursa_stream_t stream);
-int ursa_linear_dw(const void* dz, const void* x /* or NULL */, const int8_t* q /* or NULL */, const int8_t* e, void* dw, void* ws, int64_t M,
-                   int64_t N, int64_t K, int32_t dtype, ursa_stream_t stream);
+int ursa_linear_bwd(const void* dy, const void* x /* or NULL */, const int8_t* q /* or NULL */, const int8_t* e, const void* w, const void* z,
+                    void* dx, void* dw, void* db, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
  * K16  layer norm over the last dimension          y = (z - mean) / sqrt(var + eps) * gamma + beta,  z = x or x + addend

@@ -51,7 +51,7 @@ def linear(x, w, b, r, name, dy=None, kept=None):
     ez = product_error(zs, X.shape[1] + 1, t)
     a, da, l1, l2 = act(z, name)
     y = a if r is None else a + r.double()
-    # the activation: a few roundings of its factors (the library's erf / exp are within 4 steps), the residual's sum: one
+    # the activation: its distribution function to 2^-22 of the smaller tail, a few roundings of its factors; the residual's sum: one
     ey = l1 * ez + (0 if name is None else 12 * F * (z.abs() + 1)) + F * (a.abs() + y.abs())
     values, bounds = dict(y=y), dict(y=ey + last_rounding(y, t))
     if dy is None:

@@ -24,7 +24,7 @@ def p():
 
 
 def test_linear_entries_refuse_bad_arguments(lib, p):
-    fwd, dx, dw, ag, ws = lib.ursa_linear_act, lib.ursa_linear_dx, lib.ursa_linear_dw, lib.ursa_linear_act_grad, lib.ursa_linear_ws_bytes
+    fwd, bwd, ws, bws = lib.ursa_linear_act, lib.ursa_linear_bwd, lib.ursa_linear_ws_bytes, lib.ursa_linear_bwd_ws_bytes
     assert fwd(p, p, None, None, p, None, None, 4, 4, 4, 3, 0, None) == -4            # no such type
     assert fwd(p, p, None, None, p, None, None, 4, 4, 4, F32, 4, None) == -4          # no such activation
     assert fwd(p, p, None, None, p, None, None, -1, 4, 4, F32, 0, None) == -2
@@ -35,21 +35,18 @@ def test_linear_entries_refuse_bad_arguments(lib, p):
     assert fwd(p + 2, p, None, None, p, None, None, 4, 4, 4, F32, 0, None) == -3
     assert fwd(p, p, p + 1, None, p, None, None, 4, 4, 4, BF16, 0, None) == -3
     assert fwd(None, None, None, None, None, None, None, 0, 4, 4, F32, 0, None) == 0  # no rows: nothing to do
-    assert ws(0, 64, 64, 1 << 16, F32) > 0
+    assert ws(64, 64, 1 << 16, F32) > 0
     assert fwd(p, p, None, None, p, None, None, 64, 64, 1 << 16, F32, 0, None) == -1  # a cut contraction without its scratch
-    assert dx(None, p, p, None, 4, 4, 4, F16, None) == -1
-    assert dx(p, p, p, None, 4, -4, 4, F16, None) == -2
-    assert dx(p, p, p + 1, None, 4, 4, 4, F16, None) == -3
-    assert dw(p, None, None, None, p, None, 4, 4, 4, F16, None) == -1                 # neither x nor its 8-bit form
-    assert dw(p, p, p, p, p, None, 4, 4, 4, F16, None) == -1                          # both
-    assert dw(p, None, p, None, p, None, 4, 4, 4, F16, None) == -1                    # q without e
-    assert dw(p, None, p + 4, p, p, None, 4, 4, 4, F16, None) == -3
-    assert ag(p, None, p, p, p, 4, 4, F32, 1, None) == -1                             # an activation without z
-    assert ag(p, p, p, p, p, 4, 4, F32, 0, None) == -1                                # z without one
-    assert ag(p, None, None, p, None, 4, 4, F32, 0, None) == -1                       # db without scratch
-    assert ag(p, p, p, None, None, 4, 4, F32, 9, None) == -4
-    assert [ws(k, 0, 4, 4, F32) for k in range(4)] == [0, 0, 0, 0] or ws(0, 0, 4, 4, F32) == 0
-    assert ws(9, 4, 4, 4, F32) == 0
+    ok = dict(dy=p, x=p, q=None, e=None, w=p, z=p, dx=p, dw=p, db=p, ws=p, M=4, N=4, K=4, t=F16, act=2)
+    back = lambda **k: bwd(*{**ok, **k}.values(), None)                               # noqa: E731
+    assert back(t=3) == -4 and back(act=4) == -4 and back(M=-1) == -2 and back(N=1 << 31) == -2 and back(K=1 << 31) == -2
+    assert back(dy=None) == -1 and back(w=None) == -1 and back(ws=None) == -1
+    assert back(z=None) == -1                                                         # an activation without z
+    assert back(x=None) == -1 and back(q=p, e=p) == -1 and back(x=None, q=p) == -1    # neither x nor its 8-bit form; both; q without e
+    assert back(dx=p + 1) == -3 and back(x=None, q=p + 4, e=p) == -3 and back(ws=p + 4) == -3
+    assert back(dx=None, dw=None, db=None) == 0 and back(N=0) == 0                    # nothing to do
+    assert bws(4, 4, 4, F16, 0, 1, 1, 0) == 0 and bws(4, 4, 4, F16, 2, 1, 1, 0) == 256 and bws(4, 4, 4, F16, 2, 0, 0, 1) == 16
+    assert ws(0, 4, 4, F32) == 0 and ws(4, 4, 4, 9) == 0 and bws(-1, 4, 4, F32, 0, 1, 1, 1) == 0
 
 
 def test_norm_and_pack_entries_refuse_bad_arguments(lib, p):
@@ -90,7 +87,7 @@ def test_wrappers_refuse_before_they_launch():
     with pytest.raises(TypeError, match='float32, bfloat16 or float16'):
         k.linear_act(x.double(), w.double())
     with pytest.raises(ValueError, match='8-bit form'):
-        k.linear_dw(x, x, q=x, e=x)
+        k.linear_backward(x, x, w, q=x, e=x)
 
 
 def test_calls_that_are_refused():

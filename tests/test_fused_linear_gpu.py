@@ -217,13 +217,13 @@ def test_large_and_small_magnitudes_fp32():
     x, w = torch.randn(40, 64, generator=g), torch.randn(48, 64, generator=g)
     for sx, sw in ((2.0 ** 100, 2.0 ** -100), (2.0 ** -100, 2.0 ** 100), (2.0 ** 120, 2.0 ** -60), (2.0 ** -60, 2.0 ** -40)):
         a, c = x * sx, w * sw
-        got = k.linear_act(a.to(DEV), c.to(DEV)).double().cpu()
+        got = k.linear_act(a.to(DEV), c.to(DEV))[0].double().cpu()
         want, bound = B.linear(a, c, None, None, None)
         # below 2^-117 the low parts of an operand are subnormal bf16 numbers, kept to 2^-133: 2^-134 of each times the other
         low = 2.0 ** -134 * (a.abs().double().sum(1)[:, None] + c.abs().double().sum(1)[None, :])
         assert ((got - want['y']).abs() <= bound['y'] + low).all(), (sx, sw)
     top = torch.full((16, 32), torch.finfo(torch.float32).max)
-    got = k.linear_act(top.to(DEV), torch.full((16, 32), 2.0 ** -10, device=DEV)).double().cpu()
+    got = k.linear_act(top.to(DEV), torch.full((16, 32), 2.0 ** -10, device=DEV))[0].double().cpu()
     want = float(top[0, 0]) * 2.0 ** -10 * 32
     assert ((got - want).abs() <= 1e-6 * want).all()
 

@@ -29,7 +29,6 @@ BN_RELU, BN_TWO_LAUNCH, BN_HELD = 0x1, 0x2, 0x4
 CONV_FLIP, CONV_STRIDE2 = 0x1, 0x2
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # element types of K15 - K17
 ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
-LINEAR_FWD, LINEAR_DX, LINEAR_DW, LINEAR_ACT_GRAD = 0, 1, 2, 3
 ACT8_BLOCK = 32                                                           # features of a row that share a power of two (K17)
 PREACT_BN, PREACT_STATS, PREACT_ADD, PREACT_BNBWD, PREACT_EVAL = 0x10, 0x20, 0x40, 0x80, 0x100
 
@@ -98,11 +97,10 @@ SIGNATURES = {
     'ursa_bn_relu_pool_bwd_f32': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     'ursa_bn_apply_f32': (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f, _f, _u32, _vp]),
     'ursa_bn_bwd_dx_f32': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _vp]),
-    'ursa_linear_ws_bytes': (_i64, [_i32, _i64, _i64, _i64, _i32]),
+    'ursa_linear_ws_bytes': (_i64, [_i64, _i64, _i64, _i32]),
+    'ursa_linear_bwd_ws_bytes': (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32]),
     'ursa_linear_act': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
-    'ursa_linear_act_grad': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
-    'ursa_linear_dx': (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
-    'ursa_linear_dw': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    'ursa_linear_bwd': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
     'ursa_layer_norm_ws_floats': (_i64, [_i64, _i64]),
     'ursa_layer_norm_fwd': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _i32, _i32, _vp]),
     'ursa_layer_norm_bwd': (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
@@ -232,6 +230,11 @@ def _tptr(t, name, dtype, n=None, device=None, optional=False):
     if device is not None and t.device != device:
         raise ValueError(f'{name} is on {t.device}, expected {device}')
     return t.data_ptr()
+
+
+def _raw_stream(index):
+    """torch's current stream on device `index`, as the address the C ABI takes (0.1 us; current_stream().cuda_stream: 1.9)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _element_type(x, name):
@@ -950,19 +953,14 @@ class HipKernels:
         _check(self.lib, rc, 'ursa_bn_relu_pool_bwd_f32')
 
     # K15 -----------------------------------------------------------------------------
-    def _launch(self, name, dev, *args):
-        fn = getattr(self.lib, name)
+    def _launch(self, fn, dev, *args):
         if torch.cuda.current_device() == dev.index:
-            rc = fn(*args, _stream(dev))
+            rc = fn(*args, _raw_stream(dev.index))
         else:
             with torch.cuda.device(dev):
-                rc = fn(*args, _stream(dev))
+                rc = fn(*args, _raw_stream(dev.index))
         if rc:
-            _check(self.lib, rc, name)
-
-    def _linear_ws(self, which, M, N, K, dt, x):
-        n = self.lib.ursa_linear_ws_bytes(which, M, N, K, dt)
-        return x.new_empty(n, dtype=torch.uint8) if n else None
+            _check(self.lib, rc, fn.__name__)
 
     @staticmethod
     def _act(activation):
@@ -972,67 +970,49 @@ class HipKernels:
             raise ValueError(f'activation must be one of {list(ACTIVATIONS)}, got {activation!r}') from None
 
     def linear_act(self, x, w, bias=None, residual=None, *, activation=None, save_z=False):
-        """act(x W' + bias) + residual for x [M, K], w [N, K] -> y [M, N] (and z = x W' + bias with `save_z`: (y, z))."""
+        """act(x W' + bias) + residual for x [M, K], w [N, K] -> (y [M, N], z = x W' + bias with `save_z`, else None)."""
         dt, act = _element_type(x, 'x'), self._act(activation)
         if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
             raise ValueError(f'x {tuple(x.shape)} and w {tuple(w.shape)} should be [M, K] and [N, K]')
         (M, K), N, t, dev = x.shape, w.shape[0], x.dtype, x.device
         px, pw = _tptr(x, 'x', t), _tptr(w, 'w', t, None, dev)
-        pb, pr = _tptr(bias, 'bias', t, N, dev, True), _tptr(residual, 'residual', t, M * N, dev, True)
+        pb = None if bias is None else _tptr(bias, 'bias', t, N, dev)
+        pr = None if residual is None else _tptr(residual, 'residual', t, M * N, dev)
         y = x.new_empty((M, N))
-        z = torch.empty_like(y) if save_z else None
-        ws = self._linear_ws(LINEAR_FWD, M, N, K, dt, x)
-        self._launch('ursa_linear_act', dev, px, pw, pb, pr, y.data_ptr(), None if z is None else z.data_ptr(),
+        z = x.new_empty((M, N)) if save_z else None
+        n = self.lib.ursa_linear_ws_bytes(M, N, K, dt)
+        ws = x.new_empty(n, dtype=torch.uint8) if n else None
+        self._launch(self.lib.ursa_linear_act, dev, px, pw, pb, pr, y.data_ptr(), None if z is None else z.data_ptr(),
                      None if ws is None else ws.data_ptr(), M, N, K, dt, act)
-        return (y, z) if save_z else y
+        return y, z
 
-    def linear_act_grad(self, dy, z=None, *, activation=None, bias_grad=True):
-        """(dz, db): dz = dy act'(z) (dy itself without an activation), db [N] its column sums or None."""
+    def linear_backward(self, dy, x=None, w=None, z=None, *, q=None, e=None, in_features=None, activation=None, need_dx=True, need_dw=True,
+                        need_db=True):
+        """(dx, dw, db) of linear_act from dy [M, N], None for what is not wanted. w is read for dx; x - or its 8-bit form (q, e) of
+        `in_features` columns - for dw; z with an activation."""
         dt, act = _element_type(dy, 'dy'), self._act(activation)
         (M, N), t, dev = dy.shape, dy.dtype, dy.device
+        K = int(in_features) if in_features is not None else (x if x is not None else w).shape[1]
+        if need_dw and (x is None) == (q is None):
+            raise ValueError('linear_backward wants x or its 8-bit form')
         pd = _tptr(dy, 'dy', t)
-        pz = _tptr(z, 'z', t, M * N, dev, optional=not act)
-        if not act and z is not None:
-            raise ValueError('z without an activation')
-        if M == 0:
-            return dy, dy.new_zeros(N) if bias_grad else None
-        dz = torch.empty_like(dy) if act else None
-        db = dy.new_empty(N) if bias_grad else None
-        if act or bias_grad:
-            ws = self._linear_ws(LINEAR_ACT_GRAD, M, N, 0, dt, dy) if bias_grad else None
-            self._launch('ursa_linear_act_grad', dev, pd, pz, None if dz is None else dz.data_ptr(), None if db is None else db.data_ptr(),
-                         None if ws is None else ws.data_ptr(), M, N, dt, act)
-        return (dz if act else dy), db
-
-    def linear_dx(self, dz, w):
-        dt = _element_type(dz, 'dz')
-        if dz.dim() != 2 or w.dim() != 2 or dz.shape[1] != w.shape[0]:
-            raise ValueError(f'dz {tuple(dz.shape)} and w {tuple(w.shape)} should be [M, N] and [N, K]')
-        (M, N), K, dev = dz.shape, w.shape[1], dz.device
-        pz, pw = _tptr(dz, 'dz', dz.dtype), _tptr(w, 'w', dz.dtype, None, dev)
-        dx = dz.new_empty((M, K))
-        ws = self._linear_ws(LINEAR_DX, M, N, K, dt, dz)
-        self._launch('ursa_linear_dx', dev, pz, pw, dx.data_ptr(), None if ws is None else ws.data_ptr(), M, N, K, dt)
-        return dx
-
-    def linear_dw(self, dz, x=None, *, q=None, e=None, in_features=None):
-        """dz' x [N, K], x given as itself or as its 8-bit form (q, e) of `in_features` columns."""
-        dt = _element_type(dz, 'dz')
-        if (x is None) == (q is None):
-            raise ValueError('linear_dw wants x or its 8-bit form')
-        (M, N), t, dev = dz.shape, dz.dtype, dz.device
-        pz = _tptr(dz, 'dz', t)
-        if x is not None:
-            if x.dim() != 2 or x.shape[0] != M:
-                raise ValueError(f'dz {tuple(dz.shape)} and x {tuple(x.shape)} should be [M, N] and [M, K]')
-            K, px, pq, pe = x.shape[1], _tptr(x, 'x', t, None, dev), None, None
-        else:
-            K, px = int(in_features), None
-            pq, pe = self._act8_ptrs(q, e, M, K, dev)
-        dw = dz.new_empty((N, K))
-        ws = self._linear_ws(LINEAR_DW, M, N, K, dt, dz)
-        self._launch('ursa_linear_dw', dev, pz, px, pq, pe, dw.data_ptr(), None if ws is None else ws.data_ptr(), M, N, K, dt)
-        return dw
+        px = pq = pe = None
+        if need_dw:
+            if q is None:
+                px = _tptr(x, 'x', t, M * K, dev)
+            else:
+                pq, pe = self._act8_ptrs(q, e, M, K, dev)
+        pw = _tptr(w, 'w', t, N * K, dev) if need_dx else None
+        pz = _tptr(z, 'z', t, M * N, dev) if act else None
+        dx = dy.new_empty((M, K)) if need_dx else None
+        dw = dy.new_empty((N, K)) if need_dw else None
+        db = dy.new_empty(N) if need_db else None
+        n = self.lib.ursa_linear_bwd_ws_bytes(M, N, K, dt, act, need_dx, need_dw, need_db)
+        ws = dy.new_empty(n, dtype=torch.uint8) if n else None
+        self._launch(self.lib.ursa_linear_bwd, dev, pd, px, pq, pe, pw, pz, None if dx is None else dx.data_ptr(),
+                     None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
+                     M, N, K, dt, act)
+        return dx, dw, db
 
     # K16 -----------------------------------------------------------------------------
     @staticmethod
@@ -1058,7 +1038,7 @@ class HipKernels:
         ms = x.new_empty((2, M), dtype=torch.float32) if stats else None
         q, e = self._act8_empty(x, M, D) if save8 else (None, None)
         pm = None if ms is None else ms.data_ptr()
-        self._launch('ursa_layer_norm_fwd', dev, px, pa, None if addend is None else z.data_ptr(), y.data_ptr(), pg, pb, pm,
+        self._launch(self.lib.ursa_layer_norm_fwd, dev, px, pa, None if addend is None else z.data_ptr(), y.data_ptr(), pg, pb, pm,
                      None if ms is None else pm + 4 * M, None if q is None else q.data_ptr(), None if q is None else e.data_ptr(),
                      M, D, float(eps), dt, DTYPES[pt])
         return z, y, (None if ms is None else ms[0]), (None if ms is None else ms[1]), q, e
@@ -1082,7 +1062,7 @@ class HipKernels:
         dg = dy.new_empty(D, dtype=pt) if need_dgamma else None
         db = dy.new_empty(D, dtype=pt) if need_dbeta else None
         ws = dy.new_empty(self.lib.ursa_layer_norm_ws_floats(M, D), dtype=torch.float32) if need_dgamma or need_dbeta else None
-        self._launch('ursa_layer_norm_bwd', dev, *args, *(None if o is None else o.data_ptr() for o in (dx, dg, db, ws)), M, D, dt, DTYPES[pt])
+        self._launch(self.lib.ursa_layer_norm_bwd, dev, *args, *(None if o is None else o.data_ptr() for o in (dx, dg, db, ws)), M, D, dt, DTYPES[pt])
         return dx, dg, db
 
     # K17 -----------------------------------------------------------------------------
@@ -1103,7 +1083,7 @@ class HipKernels:
             raise ValueError(f'x {tuple(x.shape)} should be [M, D]')
         M, D = x.shape
         q, e = self._act8_empty(x, M, D)
-        self._launch('ursa_act8_pack', x.device, px, q.data_ptr(), e.data_ptr(), M, D, dt)
+        self._launch(self.lib.ursa_act8_pack, x.device, px, q.data_ptr(), e.data_ptr(), M, D, dt)
         return q, e
 
     def act8_unpack(self, q, e, D, dtype):
@@ -1112,7 +1092,7 @@ class HipKernels:
         M = q.shape[0]
         pq, pe = self._act8_ptrs(q, e, M, D, q.device)
         x = q.new_empty((M, D), dtype=dtype)
-        self._launch('ursa_act8_unpack', q.device, pq, pe, x.data_ptr(), M, D, DTYPES[dtype])
+        self._launch(self.lib.ursa_act8_unpack, q.device, pq, pe, x.data_ptr(), M, D, DTYPES[dtype])
         return x
 
 

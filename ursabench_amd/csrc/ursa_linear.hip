@@ -38,21 +38,62 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float act_value(float z, int act) {
-    switch (act) {
-        case URSA_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-        case URSA_ACT_GELU: return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
-        case URSA_ACT_SILU: return z / (1.f + expf(-z));
-        default: return z;
+// Phi(z), the standard normal distribution, and e = exp(-z^2 / 2): Phi(-u) = e g(u) for u >= 0 with g(u) = erfcx(u / sqrt 2) / 2, and
+// g as a polynomial in t = 1 / (1 + 0.3 u) without a constant term (g falls like 1 / u), fitted to the least largest relative error:
+// 1.5e-7 in exact arithmetic, so the tails keep their relative accuracy. About 22 vector operations where erff takes three times that:
+// an epilogue's activations would cost as much as its matrix instructions.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float u = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(0.3f, u, 1.f));
+    e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);          // log2(e) / 2
+    float g = 0.03567589074373245f;
+    g = fmaf(g, t, -0.15720807015895844f);
+    g = fmaf(g, t, 0.20636247098445892f);
+    g = fmaf(g, t, -0.05369199067354202f);
+    g = fmaf(g, t, 0.1285659670829773f);
+    g = fmaf(g, t, 0.09991223365068436f);
+    g = fmaf(g, t, 0.12075414508581161f);
+    g = fmaf(g, t, 0.11962928622961044f);
+    const float tail = g * t * e;
+    return z > 0.f ? 1.f - tail : tail;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
+
+// act over N values at once: one uniform branch for all of them
+template <int N>
+__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+    float e;
+    if (act == URSA_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= normal_cdf(v[i], e);
+    } else if (act == URSA_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+    } else if (act == URSA_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];      // a NaN stays one
     }
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case URSA_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case URSA_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
-        case URSA_ACT_SILU: { const float s = 1.f / (1.f + expf(-z)); return s * (1.f + z * (1.f - s)); }
-        default: return 1.f;
+// g *= act'(z)
+template <int N>
+__device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], int act) {
+    if (act == URSA_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float e;
+            const float phi = normal_cdf(z[i], e);
+            g[i] *= fmaf(z[i] * 0.39894228040143268f, e, phi);
+        }
+    } else if (act == URSA_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float s = sigmoid(z[i]);
+            g[i] *= s * fmaf(z[i], 1.f - s, 1.f);
+        }
+    } else if (act == URSA_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : 0.f;
     }
 }
 
@@ -149,33 +190,32 @@ __device__ __forceinline__ s16x8 fragment(const short* plane, int row0, int k, i
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* p, int valid, const float (&v)[4]) { store_piece<T, 4>(p, valid, v); }
-
-// four consecutive n of one m through the epilogue
-template <typename T>
-__device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, int N, const float (&acc)[4]) {
+// C consecutive n of one m through the epilogue; `bias`: those of the bias, or zeros
+template <typename T, int C>
+__device__ __forceinline__ void finish(const Epilogue& ep, int64_t m, int n, int N, float (&v)[C], const float (&bias)[C]) {
     const int valid = N - n;
     const int64_t at = m * N + n;
-    float v[4], t[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = acc[i];
-    if (ep.bias) {
-        load_piece<T, 4>((const T*)ep.bias + n, valid, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
-    }
-    if (ep.z) store4<T>((T*)ep.z + at, valid, v);
-    if (ep.act) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], ep.act);
-    }
+    for (int i = 0; i < C; ++i) v[i] += bias[i];
+    if (ep.z) store_piece<T, C>((T*)ep.z + at, valid, v);
+    act_values(v, ep.act);
     if (ep.residual) {
-        load_piece<T, 4>((const T*)ep.residual + at, valid, t);
+        float t[C];
+        load_piece<T, C>((const T*)ep.residual + at, valid, t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
+        for (int i = 0; i < C; ++i) v[i] += t[i];
     }
-    store4<T>((T*)ep.out + at, valid, v);
+    store_piece<T, C>((T*)ep.out + at, valid, v);
+}
+
+template <typename T, int C>
+__device__ __forceinline__ void load_bias(const Epilogue& ep, int n, int N, float (&b)[C]) {
+    if (ep.bias) {
+        load_piece<T, C>((const T*)ep.bias + n, N - n, b);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) b[i] = 0.f;
+    }
 }
 
 // tile of this workgroup: workgroups go round the 8 XCDs, so every eighth is a neighbour in one L2; those take consecutive tiles, and
@@ -276,9 +316,162 @@ __global__ __launch_bounds__(256) void k_product(Operand X, Operand Y, Shape s, 
         for (int j = 0; j < F; ++j) {
             const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
             if (n >= s.N) continue;
-            const float v[4] = {acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]};
-            if (ep.partial) store_piece<float, 4>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
-            else finish4<T>(ep, m, n, s.N, v);
+            float v[4] = {acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]}, b[4];
+            if (ep.partial) {
+                store_piece<float, 4>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
+            } else {
+                load_bias<T, 4>(ep, n, s.N, b);
+                finish<T, 4>(ep, m, n, s.N, v, b);
+            }
+        }
+    }
+}
+
+// ---- 256 x 256 outputs by eight waves, 16-bit operands straight from memory to LDS ------------------------------------------
+// A wave owns 128 x 64 outputs (32 accumulators of 16 x 16, two waves on each SIMD): 12 fragment reads feed 32 matrix instructions, so
+// the LDS is busy three quarters of the time that the matrix pipe is. The fragments of the next 32 k are read while the present ones
+// are multiplied. Two stages of 64 k in LDS: as soon as every wave has its last fragments of a stage, the pieces of the stage after
+// the next start from memory to LDS, past the registers, and have a whole stage's time to arrive. A wave's 64 pieces land side by
+// side, so what spreads the banks is a permutation of the addresses that they come from (and 64 bytes between two rows of a
+// kAcross stage). Buffer loads: what lies behind an operand's last element reads as 0. For operands whose rows and start are multiples of
+// 16 bytes and whose rows are at most 2^22 long (32-bit offsets within a tile).
+typedef __attribute__((address_space(3))) const void* lptr;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes from each lane's `offset` in the buffer to LDS at `dst` + 16 lane (dst the same in the whole wave). Not the compiler's
+// builtin: that one makes it wait for every such load before the next LDS read of any address. Whoever reads the LDS waits
+// (vmcnt(0), then a barrier). m0 has no other use here; one wait state between its write and its use.
+__device__ __forceinline__ void memory_to_lds(i32x4 buffer, uint32_t offset, const short* dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 ::"s"((uint32_t)(uintptr_t)(lptr)dst), "v"(offset), "s"(buffer) : "memory");
+}
+
+constexpr int kWide = 256, kWideK = 64, kWideThreads = 512;
+constexpr int kWidePair = 2 * kWide + 32;                 // shorts of two k rows of a kAcross stage and the gap behind them
+constexpr int kWideStage = kWideK / 2 * kWidePair;        // shorts of a stage of either kind (kFlat: 64 x 256)
+constexpr int64_t kWideMaxPitch = 1 << 22;
+
+// an operand's tile on its way: the buffer starts at (r0, k) and ends with the operand, so that rows and k behind it are out of range
+template <typename T, int KIND>
+struct WideTile {
+    uint64_t at, end;            // addresses
+    uint32_t offset, step;       // of this lane's piece 0; from one piece to the next
+    int k0, advance;             // k of piece 0 within the stage (kFlat: of every piece); bytes from stage to stage
+    __device__ __forceinline__ WideTile(const Operand& o, int r0, int k_begin, int K, int wave, int lane) {
+        const uint64_t p = (uint64_t)o.p;
+        if constexpr (KIND == kFlat) {
+            const int row = wave * 8 + (lane >> 3), piece = (lane & 7) ^ (row & 7);        // piece i: 64 rows further
+            k0 = piece * 8;
+            offset = (uint32_t)(row * o.pitch + k0) * 2, step = (uint32_t)(64 * o.pitch * 2), advance = kWideK * 2;
+            at = p + ((uint64_t)r0 * o.pitch + k_begin) * 2, end = p + (uint64_t)o.rows * o.pitch * 2;
+        } else {
+            const int k = wave * 2 + (lane >> 5), slot = ((lane & 31) >> 1) ^ (k & 1);     // piece i: 16 k further
+            k0 = k;
+            offset = (uint32_t)(k * o.pitch + slot * 16 + (lane & 1) * 8) * 2, step = (uint32_t)(16 * o.pitch * 2), advance = (int)(kWideK * o.pitch * 2);
+            at = p + ((uint64_t)k_begin * o.pitch + r0) * 2, end = p + (uint64_t)K * o.pitch * 2;
+        }
+    }
+    // piece i of the stage from k, which is left to the next stage with the last piece
+    __device__ __forceinline__ void fetch(short* stage, int wave, int i, int k, int K) {
+        const int64_t left = (int64_t)(end - at);
+        const uint32_t records = left <= 0 ? 0 : left < 0x7fffffff ? (uint32_t)left : 0x7fffffffu;
+        const i32x4 buffer = {(int)(uint32_t)at, (int)((at >> 32) & 0xffff), (int)records, 0x00027000};
+        uint32_t from = offset + i * step;
+        if constexpr (KIND == kFlat)
+            if (k + kWideK > K) from = k + k0 < K ? from : 0x80000000u;                    // the row goes on with other numbers
+        short* dst = KIND == kFlat ? stage + (i * kWideThreads + wave * 64) * 8 : stage + (i * 8 + wave) * kWidePair;
+        memory_to_lds(buffer, from, dst);
+        if (i == 3) at += advance;
+    }
+};
+
+template <int KIND>
+__device__ __forceinline__ s16x8 wide_fragment(const short* stage, int row0, int k, int lane) {
+    if constexpr (KIND == kFlat) {
+        return *(const s16x8*)(stage + flat_at<kWideK>(row0 + (lane & 15), (k >> 3) + (lane >> 4)));
+    } else {
+        const int kr = 8 * (lane >> 4) + ((lane & 15) >> 2), odd = kr & 1;
+        const short* p = stage + (kr >> 1) * kWidePair + odd * kWide + ((lane & 3) << 2) + (k >> 1) * kWidePair + (((row0 >> 4) ^ odd) << 4);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2 * kWidePair));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+template <typename T, int XK, int YK>
+__global__ __launch_bounds__(kWideThreads, 2) void k_product_wide(Operand X, Operand Y, Shape s, Epilogue ep) {
+    constexpr int BK = kWideK;
+    __shared__ __attribute__((aligned(16))) short lds[2][2][kWideStage];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, s, tm, tn);
+    const int m0 = tm * kWide, n0 = tn * kWide;
+    const int k_begin = blockIdx.y * s.k_slice, k_end = s.K - k_begin < s.k_slice ? s.K : k_begin + s.k_slice;
+    const int steps = (k_end - k_begin + BK - 1) / BK;
+    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 64;
+    WideTile<T, XK> tx(X, m0, k_begin, s.K, wave, lane);
+    WideTile<T, YK> ty(Y, n0, k_begin, s.K, wave, lane);
+    f32x4 acc[4][8] = {};                                 // [n][m]
+    s16x8 fx[2][8], fy[2][4];
+    // fetches and fragment reads run past the last step without a branch: nobody uses what they bring
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tx.fetch(lds[0][0], wave, i, k_begin, s.K), ty.fetch(lds[0][1], wave, i, k_begin, s.K);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tx.fetch(lds[1][0], wave, i, k_begin + BK, s.K), ty.fetch(lds[1][1], wave, i, k_begin + BK, s.K);
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fy[0][j] = wide_fragment<YK>(lds[0][1], wn + 16 * j, 0, lane);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) fx[0][g] = wide_fragment<XK>(lds[0][0], wm + 16 * g, 0, lane);
+    for (int t = 0; t < steps; ++t) {
+        short *xs = lds[t & 1][0], *ys = lds[t & 1][1];
+        const short *xn = lds[(t + 1) & 1][0], *yn = lds[(t + 1) & 1][1];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {                     // first 32 k; the second's fragments on their way
+            if (g < 4) fy[1][g] = wide_fragment<YK>(ys, wn + 16 * g, 32, lane);
+            fx[1][g] = wide_fragment<XK>(xs, wm + 16 * g, 32, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][g] = mfma<T>(fy[0][j], fx[0][g], acc[j][g]);
+        }
+        // every wave has read all of this stage, and this wave's pieces of the next one have arrived
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int k = k_begin + (t + 2) * BK;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            if (g < 4) tx.fetch(xs, wave, g, k, s.K), ty.fetch(ys, wave, g, k, s.K);
+            if (g < 4) fy[0][g] = wide_fragment<YK>(yn, wn + 16 * g, 0, lane);
+            fx[0][g] = wide_fragment<XK>(xn, wm + 16 * g, 0, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][g] = mfma<T>(fy[1][j], fx[1][g], acc[j][g]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // nothing is on its way to LDS any more, and nobody reads it
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // Through LDS, 16 rows of 64 fp32 sums of a wave at a time, so that a lane stores 16 bytes and a row 128: a lane of an accumulator
+    // holds m = l % 16, n = 4 (l / 16) .. + 3. Each wave has its own 16 x 68 (the pitch spreads the banks).
+    constexpr int P = 68;
+    float* tile = (float*)&lds[0][0][0] + wave * (16 * P);
+    const int n = n0 + wn + 8 * (lane & 7);
+    float bias[8];
+    load_bias<T, 8>(ep, n, s.N, bias);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(f32x4*)(tile + (lane & 15) * P + 16 * j + 4 * (lane >> 4)) = acc[j][i];
+#pragma unroll 1
+        for (int r = 0; r < 2; ++r) {
+            const int row = 8 * r + (lane >> 3), m = m0 + wm + 16 * i + row;
+            const float* from = tile + row * P + 8 * (lane & 7);
+            const f32x4 a = *(const f32x4*)from, b = *(const f32x4*)(from + 4);
+            float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            if (m >= s.M || n >= s.N) continue;
+            if (ep.partial) store_piece<float, 8>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
+            else finish<T, 8>(ep, m, n, s.N, v, bias);
         }
     }
 }
@@ -297,7 +490,8 @@ __global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += t[i];
         }
-        finish4<T>(ep, m, n, s.N, v);
+        load_bias<T, 4>(ep, n, s.N, t);
+        finish<T, 4>(ep, m, n, s.N, v, t);
     }
 }
 
@@ -315,12 +509,11 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
         for (int64_t m = begin + strand; m < end; m += 8) {
             float g[V];
             load_piece<T, V>(dy + m * N + n, left, g);
-            if (z) {
+            if (z) {                                               // dz NULL: the column sums alone are wanted
                 float a[V];
                 load_piece<T, V>(z + m * N + n, left, a);
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[i] *= act_slope(a[i], act);
-                store_piece<T, V>(dz + m * N + n, left, g);
+                act_slopes(g, a, act);
+                if (dz) store_piece<T, V>(dz + m * N + n, left, g);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] += g[i];               // before dz is rounded to its type
@@ -361,16 +554,18 @@ struct Plan {
 };
 
 // 128 x 128 tiles where they give every CU one, 64 x 64 otherwise; a contraction is cut while there are fewer than 512 workgroups
-// (two for each CU) and each keeps eight k steps
-Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+// (two for each CU) and each keeps eight k steps. `wide`: the operands suit the 256 x 256 form, taken where it gives 192 CUs a tile.
+Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide = false) {
     Plan p;
     const int bk = dtype == URSA_F32 ? 32 : 64;
-    const int64_t big = ((M + 127) / 128) * ((N + 127) / 128);
+    const int64_t big = ((M + 127) / 128) * ((N + 127) / 128), huge = ((M + 255) / 256) * ((N + 255) / 256);
     p.tile = big >= 256 ? 128 : 64;
+    if (wide && huge >= 192) p.tile = 256;
     p.s.M = (int)M, p.s.N = (int)N, p.s.K = (int)K;
     p.s.tiles_m = (int)((M + p.tile - 1) / p.tile), p.s.tiles_n = (int)((N + p.tile - 1) / p.tile);
     const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, steps = (K + bk - 1) / bk;
-    int64_t cut = tiles < 512 && tiles ? 512 / tiles : 1;
+    const int64_t want = p.tile == 256 ? 256 : 512;
+    int64_t cut = tiles < want && tiles ? want / tiles : 1;
     if (cut > steps / 8) cut = steps / 8;
     if (cut > 16) cut = 16;
     if (cut < 1) cut = 1;
@@ -380,17 +575,31 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype) {
     return p;
 }
 
+template <typename T>
+int join(const Plan& p, const Epilogue& ep, hipStream_t st) {
+    const int64_t quads = (int64_t)p.s.M * ((p.s.N + 3) / 4), blocks = (quads + 255) / 256;
+    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, p.s, ep);
+    return launch_status();
+}
+
+// whether an operand's rows (of `pitch` elements) and start suit 16-byte pieces
+bool whole_pieces(int32_t dtype, const void* p, int64_t pitch) { return dtype != URSA_F32 && pitch % 8 == 0 && pitch <= kWideMaxPitch && ((uintptr_t)p & 15) == 0; }
+
 template <typename T, int XK, int YK>
 int product(const Operand& x, const Operand& y, const Plan& p, Epilogue ep, hipStream_t st) {
     if (p.s.slices == 1) ep.partial = nullptr;
     const dim3 grid((unsigned)(p.s.tiles_m * p.s.tiles_n), (unsigned)p.s.slices);
+    if constexpr (!__is_same(T, float) && YK != kAcross8)
+        if (p.tile == 256) {
+            hipLaunchKernelGGL((k_product_wide<T, XK, YK>), grid, dim3(kWideThreads), 0, st, x, y, p.s, ep);
+            const int rc = launch_status();
+            return rc || p.s.slices == 1 ? rc : join<T>(p, ep, st);
+        }
     if (p.tile == 128) hipLaunchKernelGGL((k_product<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
     else hipLaunchKernelGGL((k_product<T, XK, YK, 64>), grid, dim3(256), 0, st, x, y, p.s, ep);
     int rc = launch_status();
     if (rc || p.s.slices == 1) return rc;
-    const int64_t quads = (int64_t)p.s.M * ((p.s.N + 3) / 4), blocks = (quads + 255) / 256;
-    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, p.s, ep);
-    return launch_status();
+    return join<T>(p, ep, st);
 }
 
 #define URSA_LINEAR_TYPES(dtype, call) (dtype == URSA_F32 ? call(float) : dtype == URSA_BF16 ? call(bf16) : call(f16))
@@ -417,32 +626,70 @@ int act_rows(int64_t M, int64_t N, int32_t dtype) {       // rows of a slice of 
 }
 
 template <typename T>
-int act_grad(dim3 grid, const T* dy, const T* z, T* dz, T* db, float* partial, int64_t M, int N, int act, int rows, int slices, hipStream_t st) {
-    hipLaunchKernelGGL(k_act_grad<T>, grid, dim3(256), 0, st, dy, z, dz, partial, M, N, act, rows);
-    const int rc = launch_status();
-    if (rc || !db) return rc;
-    hipLaunchKernelGGL(k_columns_join<T>, dim3((unsigned)((N + 31) / 32)), dim3(256), 0, st, (const float*)partial, slices, N, db);
-    return launch_status();
+int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T* w, const T* z, T* dx, T* dw, T* db, char* ws, int64_t dz_bytes,
+             int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, hipStream_t st) {
+    int rc = URSA_OK;
+    T* dz = dz_bytes ? (T*)ws : nullptr;
+    float* scratch = (float*)(ws + dz_bytes);
+    if (dz || db) {
+        const int rows = act_rows(M, N, dtype), slices = (int)((M + rows - 1) / rows), per = 32 * Piece<T>::kN;
+        if (M) {
+            hipLaunchKernelGGL(k_act_grad<T>, dim3((unsigned)((N + per - 1) / per), (unsigned)slices), dim3(256), 0, st, dy, act ? z : nullptr, dz,
+                               db ? scratch : nullptr, M, (int)N, act, rows);
+            if ((rc = launch_status())) return rc;
+        }
+        if (db) {
+            hipLaunchKernelGGL(k_columns_join<T>, dim3((unsigned)((N + 31) / 32)), dim3(256), 0, st, (const float*)scratch, slices, (int)N, db);
+            if ((rc = launch_status())) return rc;
+        }
+    }
+    const T* g = dz ? dz : dy;
+    if (dx && M && K) {
+        const Operand X{g, nullptr, N, (int)M}, Y{w, nullptr, K, (int)K};
+        if ((rc = product<T, kFlat, kAcross>(X, Y, plan_of(M, K, N, dtype, whole_pieces(dtype, g, N) && whole_pieces(dtype, w, K)), {dx, nullptr, nullptr, nullptr, scratch, URSA_ACT_NONE}, st))) return rc;
+    }
+    if (dw && K) {
+        const Epilogue ep{dw, nullptr, nullptr, nullptr, scratch, URSA_ACT_NONE};
+        const Operand X{g, nullptr, N, (int)N}, Y{q ? (const void*)q : x, e, q ? (K + kBlock8 - 1) / kBlock8 * kBlock8 : K, (int)K};
+        const Plan p = plan_of(N, K, M, dtype, whole_pieces(dtype, g, N) && !q && whole_pieces(dtype, x, K));
+        rc = q ? product<T, kAcross, kAcross8>(X, Y, p, ep, st) : product<T, kAcross, kAcross>(X, Y, p, ep, st);
+    }
+    return rc;
 }
+
+// scratch: what either form of a plan takes (alignment decides). Of a backward call: dz (with an activation), then what one of its launches needs at a time - they run one after another
+int64_t most_ws(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+    const int64_t a = plan_of(M, N, K, dtype).ws(), b = plan_of(M, N, K, dtype, dtype != URSA_F32).ws();
+    return a > b ? a : b;
+}
+
+struct BwdScratch {
+    int64_t dz, rest;
+    BwdScratch(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, bool dx, bool dw, bool db) : dz(0), rest(0) {
+        if (act && (dx || dw)) dz = (M * N * element_size(dtype) + 255) / 256 * 256;
+        if (dx && M && K) rest = most_ws(M, K, N, dtype);
+        if (dw && N && K) { const int64_t n = most_ws(N, K, M, dtype); rest = n > rest ? n : rest; }
+        if (db) { const int64_t r = act_rows(M, N, dtype), n = (M + r - 1) / r * N * 4; rest = n > rest ? n : rest; }
+    }
+};
 
 }  // namespace
 
-extern "C" int64_t ursa_linear_ws_bytes(int32_t pass, int64_t M, int64_t N, int64_t K, int32_t dtype) {
-    if (check(M, N, K, dtype)) return 0;
-    switch (pass) {
-        case URSA_LINEAR_FWD: return plan_of(M, N, K, dtype).ws();
-        case URSA_LINEAR_DX: return K ? plan_of(M, K, N, dtype).ws() : 0;
-        case URSA_LINEAR_DW: return K ? plan_of(N, K, M, dtype).ws() : 0;
-        case URSA_LINEAR_ACT_GRAD: { const int r = act_rows(M, N, dtype); return (M + r - 1) / r * N * 4; }
-    }
-    return 0;
+extern "C" int64_t ursa_linear_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+    return check(M, N, K, dtype) ? 0 : most_ws(M, N, K, dtype);
+}
+
+extern "C" int64_t ursa_linear_bwd_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, int32_t dx, int32_t dw, int32_t db) {
+    if (check(M, N, K, dtype) < 0) return 0;
+    const BwdScratch s(M, N, K, dtype, act, dx, dw, db);
+    return s.dz + s.rest;
 }
 
 extern "C" int ursa_linear_act(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, void* ws, int64_t M,
                                int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream) {
     if (act < URSA_ACT_NONE || act > URSA_ACT_SILU) return URSA_EFLAGS;
     if (int rc = check(M, N, K, dtype)) return rc > 0 ? URSA_OK : rc;
-    const Plan p = plan_of(M, N, K, dtype);
+    const Plan p = plan_of(M, N, K, dtype, whole_pieces(dtype, x, K) && whole_pieces(dtype, w, K));
     if ((K && (!x || !w)) || !y || (p.ws() && !ws)) return URSA_ENULL;
     if (misaligned(dtype, (uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)z) || (uintptr_t)ws & 3) return URSA_EALIGN;
     const Operand X{x, nullptr, K, (int)M}, Y{w, nullptr, K, (int)N};
@@ -452,43 +699,18 @@ extern "C" int ursa_linear_act(const void* x, const void* w, const void* bias, c
 #undef URSA_CALL
 }
 
-extern "C" int ursa_linear_dx(const void* dz, const void* w, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, ursa_stream_t stream) {
-    if (int rc = check(M, K, N, dtype)) return rc > 0 ? URSA_OK : rc;
-    const Plan p = plan_of(M, K, N, dtype);
-    if ((N && (!dz || !w)) || !dx || (p.ws() && !ws)) return URSA_ENULL;
-    if (misaligned(dtype, (uintptr_t)dz | (uintptr_t)w | (uintptr_t)dx) || (uintptr_t)ws & 3) return URSA_EALIGN;
-    const Operand X{dz, nullptr, N, (int)M}, Y{w, nullptr, K, (int)K};
-    const Epilogue ep{dx, nullptr, nullptr, nullptr, (float*)ws, URSA_ACT_NONE};
-#define URSA_CALL(T) product<T, kFlat, kAcross>(X, Y, p, ep, (hipStream_t)stream)
-    return URSA_LINEAR_TYPES(dtype, URSA_CALL);
-#undef URSA_CALL
-}
-
-extern "C" int ursa_linear_dw(const void* dz, const void* x, const int8_t* q, const int8_t* e, void* dw, void* ws, int64_t M, int64_t N, int64_t K,
-                              int32_t dtype, ursa_stream_t stream) {
-    if (int rc = check(N, K, M, dtype)) return rc > 0 ? URSA_OK : rc;
-    const Plan p = plan_of(N, K, M, dtype);
-    if ((M && (!dz || (x != nullptr) == (q != nullptr) || (q != nullptr) != (e != nullptr))) || !dw || (p.ws() && !ws)) return URSA_ENULL;
-    if (misaligned(dtype, (uintptr_t)dz | (uintptr_t)x | (uintptr_t)dw) || (uintptr_t)q & 15 || (uintptr_t)ws & 3) return URSA_EALIGN;
-    const int64_t qpitch = (K + kBlock8 - 1) / kBlock8 * kBlock8;
-    const Operand X{dz, nullptr, N, (int)N}, Y{q ? (const void*)q : x, e, q ? qpitch : K, (int)K};
-    const Epilogue ep{dw, nullptr, nullptr, nullptr, (float*)ws, URSA_ACT_NONE};
-#define URSA_CALL(T) (q ? product<T, kAcross, kAcross8>(X, Y, p, ep, (hipStream_t)stream) : product<T, kAcross, kAcross>(X, Y, p, ep, (hipStream_t)stream))
-    return URSA_LINEAR_TYPES(dtype, URSA_CALL);
-#undef URSA_CALL
-}
-
-extern "C" int ursa_linear_act_grad(const void* dy, const void* z, void* dz, void* db, void* ws, int64_t M, int64_t N, int32_t dtype, int32_t act,
-                                    ursa_stream_t stream) {
+extern "C" int ursa_linear_bwd(const void* dy, const void* x, const int8_t* q, const int8_t* e, const void* w, const void* z, void* dx, void* dw,
+                               void* db, void* ws, int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream) {
     if (act < URSA_ACT_NONE || act > URSA_ACT_SILU) return URSA_EFLAGS;
-    if (int rc = check(M, N, 0, dtype)) return rc > 0 ? URSA_OK : rc;
-    if (!dy || (z != nullptr) != (dz != nullptr) || (act != URSA_ACT_NONE) != (z != nullptr) || (db && !ws)) return URSA_ENULL;
-    if (misaligned(dtype, (uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz | (uintptr_t)db) || (uintptr_t)ws & 3) return URSA_EALIGN;
-    const int rows = act_rows(M, N, dtype), slices = (int)((M + rows - 1) / rows);
-    float* part = db ? (float*)ws : nullptr;
-    const int per = 32 * 16 / (int)element_size(dtype);
-    const dim3 grid((unsigned)((N + per - 1) / per), (unsigned)slices);
-#define URSA_CALL(T) act_grad<T>(grid, (const T*)dy, (const T*)z, (T*)dz, (T*)db, part, M, (int)N, act, rows, slices, (hipStream_t)stream)
+    if (int rc = check(M, N, K, dtype); rc < 0) return rc;
+    if (int rc = check(N, K, M, dtype); rc < 0) return rc;
+    if (N == 0 || !(dx || dw || db)) return URSA_OK;
+    const BwdScratch size(M, N, K, dtype, act, dx, dw, db);
+    if (M && (!dy || (act && !z) || (dx && K && !w) || (dw && K && ((x != nullptr) == (q != nullptr) || (q != nullptr) != (e != nullptr))) ||
+              (size.dz + size.rest && !ws))) return URSA_ENULL;
+    if (misaligned(dtype, (uintptr_t)dy | (uintptr_t)x | (uintptr_t)w | (uintptr_t)z | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db) ||
+        (uintptr_t)q & 15 || (uintptr_t)ws & 15) return URSA_EALIGN;
+#define URSA_CALL(T) backward<T>((const T*)dy, (const T*)x, q, e, (const T*)w, (const T*)z, (T*)dx, (T*)dw, (T*)db, (char*)ws, size.dz, M, N, K, dtype, act, (hipStream_t)stream)
     return URSA_LINEAR_TYPES(dtype, URSA_CALL);
 #undef URSA_CALL
 }

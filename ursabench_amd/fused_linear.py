@@ -5,7 +5,7 @@
 launches differ:
 
   forward           one launch: product, bias, activation and residual (two where the contraction is cut over workgroups)
-  backward          the activation's gradient and the bias gradient in one pass over dy, then one launch for dx and one for dW
+  backward          the activation's gradient and the bias gradient in one pass over dy, then dx and dW by the same product kernel
 
 float32, bfloat16 and float16, any sizes and leading dimensions, on a HIP device. Operands that are not contiguous are copied first.
 Anything else - host tensors, other or mixed types, autocast, a subclass with a forward of its own, hooks on `fc` - takes
@@ -57,11 +57,7 @@ class _LinearAct(torch.autograd.Function):
     def forward(ctx, x, w, b, r, activation, save8):
         K = _native.default_kernels()
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        z = None
-        if activation is not None and (need_x or need_w or need_b):
-            y, z = K.linear_act(x, w, b, r, activation=activation, save_z=True)
-        else:
-            y = K.linear_act(x, w, b, r, activation=activation)
+        y, z = K.linear_act(x, w, b, r, activation=activation, save_z=activation is not None and (need_x or need_w or need_b))
         q = e = None
         if need_w and save8:
             q, e = K.act8_pack(x)
@@ -73,27 +69,23 @@ class _LinearAct(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, z, q, e = ctx.saved_tensors
-        K = _native.default_kernels()
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dy = dy.contiguous()
         dx = dw = db = None
         if need_x or need_w or need_b:
-            dz, db = K.linear_act_grad(dy, z, activation=ctx.activation, bias_grad=need_b)
-            if need_x:
-                dx = K.linear_dx(dz, w)
-            if need_w:
-                dw = K.linear_dw(dz, x) if q is None else K.linear_dw(dz, q=q, e=e, in_features=ctx.in_features)
+            dx, dw, db = _native.default_kernels().linear_backward(
+                dy, x, w, z, q=q, e=e, in_features=ctx.in_features, activation=ctx.activation, need_dx=need_x, need_dw=need_w, need_db=need_b)
         return dx, dw, db, (dy if need_r else None), None, None
 
 
-def _fusable(fc, x, residual):
-    w, b = fc.weight, fc.bias
-    return (_on and x.is_cuda and x.dtype in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
-            and type(fc).forward is nn.Linear.forward and not fc._forward_hooks and not fc._forward_pre_hooks
-            and not fc._backward_hooks and not fc._backward_pre_hooks
-            and w.dtype == x.dtype and w.device == x.device and x.shape[-1] == w.shape[1] and w.numel() > 0
-            and (b is None or (b.dtype == x.dtype and b.device == x.device))
-            and (residual is None or (residual.dtype == x.dtype and residual.device == x.device)))
+def _fusable(fc, w, b, x, residual):
+    t, dev = x.dtype, x.device
+    return (_on and dev.type == 'cuda' and t in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
+            and type(fc).forward is nn.Linear.forward
+            and not (fc._forward_hooks or fc._forward_pre_hooks or fc._backward_hooks or fc._backward_pre_hooks)
+            and w.dtype == t and w.device == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
+            and (b is None or (b.dtype == t and b.device == dev))
+            and (residual is None or (residual.dtype == t and residual.device == dev)))
 
 
 def linear_act(fc, x, activation=None, residual=None, *, save8=False):
@@ -103,20 +95,20 @@ def linear_act(fc, x, activation=None, residual=None, *, save8=False):
         raise ValueError(f'activation must be one of {list(_STOCK)}, got {activation!r}')
     if not isinstance(fc, nn.Linear):
         raise TypeError(f'linear_act wants an nn.Linear, got {type(fc).__name__}')
-    shape = x.shape[:-1] + (fc.weight.shape[0],)
+    w, b = fc.weight, fc.bias
+    shape = x.shape[:-1] + (w.shape[0],)
     if residual is not None and residual.shape != shape:
         raise ValueError(f'residual {tuple(residual.shape)} should have the result\'s shape {tuple(shape)}')
-    if not _fusable(fc, x, residual):
+    if not _fusable(fc, w, b, x, residual):
         y = _STOCK[activation](fc(x))
         return y if residual is None else y + residual
-    w, b = fc.weight, fc.bias
     flat = x.dim() == 2
     x2 = (x if flat else x.reshape(-1, x.shape[-1])).contiguous()
     r2 = None if residual is None else (residual if flat else residual.reshape(-1, shape[-1])).contiguous()
     w, b = w.contiguous(), None if b is None else b.contiguous()
-    if torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
-                                    or (r2 is not None and r2.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         y = _LinearAct.apply(x2, w, b, r2, activation, save8)
     else:
-        y = _native.default_kernels().linear_act(x2, w, b, r2, activation=activation)
+        y = _native.default_kernels().linear_act(x2, w, b, r2, activation=activation)[0]
     return y if flat else y.view(shape)

@@ -17,6 +17,7 @@ fused path needs csrc/libursa_hip.so (no silent fallback: a missing library rais
 taken from those values; mean and 1 / std are the exact input's. `URSA_FUSED_NORM=0` / `enabled(False)` selects the stock path
 everywhere (A/B runs).
 """
+import math
 import os
 
 import torch
@@ -81,25 +82,25 @@ class _AddNorm(torch.autograd.Function):
         return dx if need_a else None, dx if need_b else None, dw, db, None, None
 
 
-def _fusable(ln, x):
-    n = len(ln.normalized_shape)
-    params = [p for p in (ln.weight, ln.bias) if p is not None]
-    return (_on and x.is_cuda and x.dtype in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
-            and type(ln).forward is nn.LayerNorm.forward and not ln._forward_hooks and not ln._forward_pre_hooks
-            and not ln._backward_hooks and not ln._backward_pre_hooks
-            and x.dim() >= n and tuple(x.shape[x.dim() - n:]) == tuple(ln.normalized_shape) and ln.eps >= 0
-            and all(p.device == x.device and p.dtype in (x.dtype, torch.float32) and p.dtype == params[0].dtype for p in params))
+def _fusable(ln, w, b, x):
+    t, dev, shape = x.dtype, x.device, ln.normalized_shape
+    return (_on and dev.type == 'cuda' and t in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
+            and type(ln).forward is nn.LayerNorm.forward
+            and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks or ln._backward_pre_hooks)
+            and x.dim() >= len(shape) and tuple(x.shape[x.dim() - len(shape):]) == tuple(shape) and ln.eps >= 0
+            and (w is None or (w.device == dev and (w.dtype == t or w.dtype == torch.float32)))
+            and (b is None or (b.device == dev and (b.dtype == t or b.dtype == torch.float32) and (w is None or w.dtype == b.dtype))))
 
 
-def _rows(ln, x):
-    width = 1
-    for d in ln.normalized_shape:
-        width *= d
-    return x.reshape(-1, width).contiguous()
+def _rows(n, x):
+    """x as rows of its last n dimensions."""
+    if n == 1:
+        return (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
+    return x.flatten(x.dim() - n).reshape(-1, math.prod(x.shape[x.dim() - n:])).contiguous()
 
 
-def _params(ln):
-    return tuple(None if p is None else p.reshape(-1).contiguous() for p in (ln.weight, ln.bias))
+def _flat(p):
+    return p if p is None or (p.dim() == 1 and p.is_contiguous()) else p.reshape(-1).contiguous()
 
 
 def _recorded(*tensors):
@@ -110,14 +111,17 @@ def layer_norm(ln, x, *, save8=False):
     """ln(x). save8: keep x in 8 bits for the backward pass (module docstring)."""
     if not isinstance(ln, nn.LayerNorm):
         raise TypeError(f'layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
-    if not _fusable(ln, x):
+    w, b = ln.weight, ln.bias
+    if not _fusable(ln, w, b, x):
         return ln(x)
-    x2, (w, b) = _rows(ln, x), _params(ln)
-    if _recorded(x2, w, b):
+    n = len(ln.normalized_shape)
+    flat = n == 1 and x.dim() == 2
+    x2, w, b = _rows(n, x), _flat(w), _flat(b)
+    if _recorded(x, w, b):
         y = _Norm.apply(x2, w, b, ln.eps, save8)
     else:
         y = _native.default_kernels().layer_norm(x2, w, b, eps=ln.eps)[1]
-    return y.view(x.shape)
+    return y if flat else y.view(x.shape)
 
 
 def add_layer_norm(ln, x, *, save8=False):
@@ -128,12 +132,15 @@ def add_layer_norm(ln, x, *, save8=False):
     if not isinstance(ln, nn.LayerNorm):
         raise TypeError(f'add_layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
     a, b = x
-    if not (_fusable(ln, a) and b.shape == a.shape and b.dtype == a.dtype and b.device == a.device):
+    w, bias = ln.weight, ln.bias
+    if not (_fusable(ln, w, bias, a) and b.shape == a.shape and b.dtype == a.dtype and b.device == a.device):
         z = a + b
         return z, layer_norm(ln, z, save8=save8)
-    a2, b2, (w, bias) = _rows(ln, a), _rows(ln, b), _params(ln)
-    if _recorded(a2, b2, w, bias):
+    n = len(ln.normalized_shape)
+    flat = n == 1 and a.dim() == 2
+    a2, b2, w, bias = _rows(n, a), _rows(n, b), _flat(w), _flat(bias)
+    if _recorded(a, b, w, bias):
         z, y = _AddNorm.apply(a2, b2, w, bias, ln.eps, save8)
     else:
         z, y = _native.default_kernels().layer_norm(a2, w, bias, eps=ln.eps, addend=b2)[:2]
-    return z.view(a.shape), y.view(a.shape)
+    return (z, y) if flat else (z.view(a.shape), y.view(a.shape))
