@@ -82,7 +82,7 @@ def unpacked(x):
     """The 8-bit form's values in fp64."""
     rows, n = x.shape
     blocks = -(-n // 32)
-    v = torch.zeros(rows, blocks * 32, dtype=torch.float64)
+    v = torch.zeros(rows, blocks * 32, dtype=torch.float64, device=x.device)
     v[:, :n] = x.double()
     v = v.view(rows, blocks, 32)
     top = v.abs().amax(-1, keepdim=True)
@@ -140,7 +140,7 @@ def check(got, values, bounds, where=''):
     fp16) rounds to that infinity: it has to where the whole bound lies there, and may where a part does."""
     for key, t in got.items():
         v, e = values[key], bounds[key]
-        g = t.detach().double().cpu()
+        g = t.detach().double().to(v.device)
         assert g.shape == v.shape, (where, key, g.shape, v.shape)
         top = torch.finfo(t.dtype).max * (1 + half_step(t.dtype) / 2)
         must, may = v.abs() - e > top, (v.abs() + e > top) & (g == v.sign() * math.inf)

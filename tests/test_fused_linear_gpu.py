@@ -43,7 +43,7 @@ def _run(x, w, b, r, act, dy=None, save8=False):
         leaves['dr'] = R
     got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy.to(DEV))))
     if R is not None:
-        assert torch.equal(got.pop('dr').cpu(), dy)
+        assert torch.equal(got.pop('dr').to(dy.device), dy)
     return dict(y=y, **got)
 
 
@@ -63,6 +63,16 @@ def test_forward_and_gradients_at_odd_and_even_sizes(M, K, N, dtype):
 def test_larger_tiles_and_cut_contractions(M, K, N, dtype):
     x, w, b, r, dy = _case(M, K, N, dtype, residual=True)
     B.check(_run(x, w, b, r, 'silu', dy), *B.linear(x, w, b, r, 'silu', dy), where=(M, K, N, dtype))
+
+
+@pytest.mark.parametrize('save8', [False, True])
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('M,K,N', [(3592, 3600, 3608), (2056, 2056, 2056), (4104, 72, 4104), (200, 4104, 4104), (4104, 4104, 72), (3600, 3601, 3600)])
+def test_whole_tiles_and_their_edges(M, K, N, dtype, save8):
+    """Sizes that give every product of the step its largest tiles (and its second largest, and one it cannot use them for), none
+    a multiple of a tile or of a step over the contraction; fp64 on the device."""
+    x, w, b, r, dy = (None if t is None else t.to(DEV) for t in _case(M, K, N, dtype, residual=True))
+    B.check(_run(x, w, b, r, 'silu', dy, save8=save8), *B.linear(x, w, b, r, 'silu', dy, kept=B.unpacked(x) if save8 else None), where=(M, K, N, dtype))
 
 
 @pytest.mark.parametrize('dtype', list(B.TYPES))

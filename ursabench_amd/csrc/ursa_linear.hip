@@ -151,9 +151,13 @@ template <typename T, int KIND>
 __device__ __forceinline__ void split_chunk(const Chunk<T, KIND>& c, s16x8 (&out)[3]) {
     typedef typename Arith<T>::type A;
     if constexpr (KIND == kAcross8) {
+        // bytes + 128 convert in one instruction each; everything behind that is exact, the rounding to A too
         const float s = c.e == kNonFinite8 ? __builtin_nanf("") : pow2_bits(c.e);
+        uint32_t b[2];
+        __builtin_memcpy(b, c.v, 8);
+        b[0] ^= 0x80808080u, b[1] ^= 0x80808080u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[0][i] = __builtin_bit_cast(short, (A)((float)c.v[i] * s));     // exact
+        for (int i = 0; i < 8; ++i) out[0][i] = __builtin_bit_cast(short, (A)(((float)(b[i >> 2] >> (8 * (i & 3)) & 0xff) - 128.f) * s));
     } else if constexpr (__is_same(T, float)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -346,28 +350,36 @@ __device__ __forceinline__ void memory_to_lds(i32x4 buffer, uint32_t offset, con
                  ::"s"((uint32_t)(uintptr_t)(lptr)dst), "v"(offset), "s"(buffer) : "memory");
 }
 
-constexpr int kWide = 256, kWideK = 64, kWideThreads = 512;
-constexpr int kWidePair = 2 * kWide + 32;                 // shorts of two k rows of a kAcross stage and the gap behind them
-constexpr int kWideStage = kWideK / 2 * kWidePair;        // shorts of a stage of either kind (kFlat: 64 x 256)
+constexpr int kWideK = 64;
 constexpr int64_t kWideMaxPitch = 1 << 22;
 
+// A stage of R rows: kFlat [R][64], kAcross [64][R] with 64 bytes after every 1,024 where R = 256 (two k rows)
+template <int R> constexpr int pair_pitch() { return R == 256 ? 2 * R + 32 : 2 * R; }     // shorts from k to k + 2
+template <int R> constexpr int stage_shorts() { return kWideK / 2 * pair_pitch<R>(); }
+
+// where the 32-byte slot of 16 rows lies within a k row: four consecutive k have to fall into different banks
+template <int R> __device__ __forceinline__ int slot_of(int slot, int k) { return R == 256 ? slot ^ (k & 1) : slot ^ (k & 3); }
+
 // an operand's tile on its way: the buffer starts at (r0, k) and ends with the operand, so that rows and k behind it are out of range
-template <typename T, int KIND>
+template <typename T, int KIND, int R, int THREADS>
 struct WideTile {
+    static constexpr int kPieces = R * kWideK / 8 / THREADS;
     uint64_t at, end;            // addresses
     uint32_t offset, step;       // of this lane's piece 0; from one piece to the next
     int k0, advance;             // k of piece 0 within the stage (kFlat: of every piece); bytes from stage to stage
     __device__ __forceinline__ WideTile(const Operand& o, int r0, int k_begin, int K, int wave, int lane) {
         const uint64_t p = (uint64_t)o.p;
         if constexpr (KIND == kFlat) {
-            const int row = wave * 8 + (lane >> 3), piece = (lane & 7) ^ (row & 7);        // piece i: 64 rows further
+            const int row = wave * 8 + (lane >> 3), piece = (lane & 7) ^ (row & 7);        // piece i: THREADS / 8 rows further
             k0 = piece * 8;
-            offset = (uint32_t)(row * o.pitch + k0) * 2, step = (uint32_t)(64 * o.pitch * 2), advance = kWideK * 2;
+            offset = (uint32_t)(row * o.pitch + k0) * 2, step = (uint32_t)(THREADS / 8 * o.pitch * 2), advance = kWideK * 2;
             at = p + ((uint64_t)r0 * o.pitch + k_begin) * 2, end = p + (uint64_t)o.rows * o.pitch * 2;
         } else {
-            const int k = wave * 2 + (lane >> 5), slot = ((lane & 31) >> 1) ^ (k & 1);     // piece i: 16 k further
+            constexpr int PER = R / 8;                                                     // pieces of a k row
+            const int id = wave * 64 + lane, k = id / PER, slot = slot_of<R>((id % PER) >> 1, k);   // piece i: THREADS / PER k further
             k0 = k;
-            offset = (uint32_t)(k * o.pitch + slot * 16 + (lane & 1) * 8) * 2, step = (uint32_t)(16 * o.pitch * 2), advance = (int)(kWideK * o.pitch * 2);
+            offset = (uint32_t)(k * o.pitch + slot * 16 + (lane & 1) * 8) * 2, step = (uint32_t)(THREADS / PER * o.pitch * 2);
+            advance = (int)(kWideK * o.pitch * 2);
             at = p + ((uint64_t)k_begin * o.pitch + r0) * 2, end = p + (uint64_t)K * o.pitch * 2;
         }
     }
@@ -379,61 +391,133 @@ struct WideTile {
         uint32_t from = offset + i * step;
         if constexpr (KIND == kFlat)
             if (k + kWideK > K) from = k + k0 < K ? from : 0x80000000u;                    // the row goes on with other numbers
-        short* dst = KIND == kFlat ? stage + (i * kWideThreads + wave * 64) * 8 : stage + (i * 8 + wave) * kWidePair;
+        constexpr int kGap = pair_pitch<R>() - 2 * R;                                      // a wave's 512 shorts: two k rows of 256
+        short* dst = stage + (i * (THREADS / 64) + wave) * (512 + (KIND == kFlat ? 0 : kGap));
         memory_to_lds(buffer, from, dst);
-        if (i == 3) at += advance;
+        if (i == kPieces - 1) at += advance;
     }
 };
 
-template <int KIND>
+// a kAcross8 operand: 8 bytes and their exponent a piece through registers, one stage ahead of the others; LDS holds what a kAcross
+// stage would
+template <typename T, int R, int THREADS>
+struct WideTile<T, kAcross8, R, THREADS> {
+    static constexpr int kPieces = R * kWideK / 8 / THREADS, kRows = THREADS / (R / 8);      // k from piece to piece
+    Chunk<T, kAcross8> c[kPieces];
+    uint64_t at, end, at_e, end_e;
+    uint32_t offset, offset_e, step, step_e;
+    int to;                       // of piece 0 within a stage
+    __device__ __forceinline__ WideTile(const Operand& o, int r0, int k_begin, int K, int wave, int lane) {
+        const int id = wave * 64 + lane, kr = id / (R / 8), piece = id % (R / 8);
+        const int64_t pe = o.pitch / kBlock8;
+        offset = (uint32_t)(kr * o.pitch + piece * 8), offset_e = (uint32_t)(kr * pe + piece / 4);
+        step = (uint32_t)(kRows * o.pitch), step_e = (uint32_t)(kRows * pe);
+        at = (uint64_t)o.p + (uint64_t)k_begin * o.pitch + r0, end = (uint64_t)o.p + (uint64_t)K * o.pitch;
+        at_e = (uint64_t)o.e + (uint64_t)k_begin * pe + r0 / kBlock8, end_e = (uint64_t)o.e + (uint64_t)K * pe;
+        to = (kr >> 1) * pair_pitch<R>() + (kr & 1) * R + (slot_of<R>(piece >> 1, kr) << 4) + (piece & 1) * 8;
+    }
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(uint64_t at, uint64_t end) {
+        const int64_t left = (int64_t)(end - at);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff, 0x00027000);
+    }
+    // piece i of the next stage; behind the last k: zeros
+    __device__ __forceinline__ void load(int i) {
+        const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(buffer(at, end), offset + i * step, 0, 0));
+        __builtin_memcpy(c[i].v, &b, 8);
+        c[i].e = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buffer(at_e, end_e), offset_e + i * step_e, 0, 0);
+        if (i == kPieces - 1) at += (uint64_t)step * kPieces, at_e += (uint64_t)step_e * kPieces;
+    }
+    __device__ __forceinline__ void put(short* stage, int i) {
+        s16x8 out[3];
+        split_chunk<T, kAcross8>(c[i], out);
+        static_assert(kRows % 4 == 0, "the permutation of the slots repeats every 4 k");
+        *(s16x8*)(stage + to + i * (kRows / 2) * pair_pitch<R>()) = out[0];
+    }
+};
+
+template <int KIND, int R>
 __device__ __forceinline__ s16x8 wide_fragment(const short* stage, int row0, int k, int lane) {
     if constexpr (KIND == kFlat) {
         return *(const s16x8*)(stage + flat_at<kWideK>(row0 + (lane & 15), (k >> 3) + (lane >> 4)));
     } else {
-        const int kr = 8 * (lane >> 4) + ((lane & 15) >> 2), odd = kr & 1;
-        const short* p = stage + (kr >> 1) * kWidePair + odd * kWide + ((lane & 3) << 2) + (k >> 1) * kWidePair + (((row0 >> 4) ^ odd) << 4);
+        const int kr = 8 * (lane >> 4) + ((lane & 15) >> 2);
+        const short* p = stage + ((k + kr) >> 1) * pair_pitch<R>() + (kr & 1) * R + (slot_of<R>(row0 >> 4, kr) << 4) + ((lane & 3) << 2);
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2 * kWidePair));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2 * pair_pitch<R>()));
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 }
 
-template <typename T, int XK, int YK>
-__global__ __launch_bounds__(kWideThreads, 2) void k_product_wide(Operand X, Operand Y, Shape s, Epilogue ep) {
-    constexpr int BK = kWideK;
-    __shared__ __attribute__((aligned(16))) short lds[2][2][kWideStage];
+// R x R outputs by WAVES waves, two across m; a wave: 16 FX x 16 FY of them
+template <typename T, int XK, int YK, int R>
+__global__ __launch_bounds__(R == 256 ? 512 : 256, 2) void k_product_wide(Operand X, Operand Y, Shape s, Epilogue ep) {
+    constexpr int BK = kWideK, THREADS = R == 256 ? 512 : 256, WAVES = THREADS / 64, FX = R / 32, FY = R / (8 * WAVES);
+    typedef WideTile<T, XK, R, THREADS> TileX;
+    typedef WideTile<T, YK, R, THREADS> TileY;
+    constexpr int kPieces = TileX::kPieces;
+    __shared__ __attribute__((aligned(16))) short lds[2][2][stage_shorts<R>()];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tm, tn;
     tile_of(blockIdx.x, s, tm, tn);
-    const int m0 = tm * kWide, n0 = tn * kWide;
+    const int m0 = tm * R, n0 = tn * R;
     const int k_begin = blockIdx.y * s.k_slice, k_end = s.K - k_begin < s.k_slice ? s.K : k_begin + s.k_slice;
     const int steps = (k_end - k_begin + BK - 1) / BK;
-    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 64;
-    WideTile<T, XK> tx(X, m0, k_begin, s.K, wave, lane);
-    WideTile<T, YK> ty(Y, n0, k_begin, s.K, wave, lane);
-    f32x4 acc[4][8] = {};                                 // [n][m]
-    s16x8 fx[2][8], fy[2][4];
+    const int wm = (wave & 1) * (16 * FX), wn = (wave >> 1) * (16 * FY);
+    TileX tx(X, m0, k_begin, s.K, wave, lane);
+    TileY ty(Y, n0, k_begin, s.K, wave, lane);
+    f32x4 acc[FY][FX] = {};                               // [n][m]
+    // two sets of fragments; beside a kAcross8 operand's pieces there are registers for one of X's, refilled behind its last use
+    constexpr int A1 = YK == kAcross8 ? 0 : 1;
+    s16x8 fx[A1 + 1][FX], fy[2][FY];
     // fetches and fragment reads run past the last step without a branch: nobody uses what they bring
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tx.fetch(lds[0][0], wave, i, k_begin, s.K), ty.fetch(lds[0][1], wave, i, k_begin, s.K);
+    for (int st = 0; st < 2; ++st) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tx.fetch(lds[1][0], wave, i, k_begin + BK, s.K), ty.fetch(lds[1][1], wave, i, k_begin + BK, s.K);
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        for (int i = 0; i < kPieces; ++i) {
+            tx.fetch(lds[st][0], wave, i, k_begin + st * BK, s.K);
+            if constexpr (YK != kAcross8) ty.fetch(lds[st][1], wave, i, k_begin + st * BK, s.K);
+            else ty.load(i);
+        }
+        if constexpr (YK == kAcross8)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) ty.put(lds[st][1], i);
+    }
+    if constexpr (YK != kAcross8) {
+        static_assert(2 * kPieces == 8, "the second stage's loads");
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) ty.load(i);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fy[0][j] = wide_fragment<YK>(lds[0][1], wn + 16 * j, 0, lane);
+    for (int j = 0; j < FY; ++j) fy[0][j] = wide_fragment<YK, R>(lds[0][1], wn + 16 * j, 0, lane);
 #pragma unroll
-    for (int g = 0; g < 8; ++g) fx[0][g] = wide_fragment<XK>(lds[0][0], wm + 16 * g, 0, lane);
+    for (int g = 0; g < FX; ++g) fx[0][g] = wide_fragment<XK, R>(lds[0][0], wm + 16 * g, 0, lane);
     for (int t = 0; t < steps; ++t) {
         short *xs = lds[t & 1][0], *ys = lds[t & 1][1];
         const short *xn = lds[(t + 1) & 1][0], *yn = lds[(t + 1) & 1][1];
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {                     // first 32 k; the second's fragments on their way
-            if (g < 4) fy[1][g] = wide_fragment<YK>(ys, wn + 16 * g, 32, lane);
-            fx[1][g] = wide_fragment<XK>(xs, wm + 16 * g, 32, lane);
+        for (int g = 0; g < FX; ++g) {                    // first 32 k; the second's fragments on their way
+            if (g < FY) fy[1][g] = wide_fragment<YK, R>(ys, wn + 16 * g, 32, lane);
+            if (A1) fx[A1][g] = wide_fragment<XK, R>(xs, wm + 16 * g, 32, lane);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j][g] = mfma<T>(fy[0][j], fx[0][g], acc[j][g]);
+            for (int j = 0; j < FY; ++j) acc[j][g] = mfma<T>(fy[0][j], fx[0][g], acc[j][g]);
+            if (!A1) fx[0][g] = wide_fragment<XK, R>(xs, wm + 16 * g, 32, lane);
+        }
+        // the order to issue them in: a group of reads, the instructions that cover it (+2 - 4 % with transposing reads)
+        constexpr int RX = XK == kFlat ? 1 : 2, RB = RX + (YK == kFlat ? 1 : 2);
+#pragma unroll
+        for (int g = 0; A1 && g < FY; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x100, RB, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, FY, 0);
+        }
+#pragma unroll
+        for (int g = FY; A1 && g < FX; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x100, RX, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, FY, 0);
         }
         // every wave has read all of this stage, and this wave's pieces of the next one have arrived
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -441,12 +525,17 @@ __global__ __launch_bounds__(kWideThreads, 2) void k_product_wide(Operand X, Ope
         asm volatile("" ::: "memory");
         const int k = k_begin + (t + 2) * BK;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-            if (g < 4) tx.fetch(xs, wave, g, k, s.K), ty.fetch(ys, wave, g, k, s.K);
-            if (g < 4) fy[0][g] = wide_fragment<YK>(yn, wn + 16 * g, 0, lane);
-            fx[0][g] = wide_fragment<XK>(xn, wm + 16 * g, 0, lane);
+        for (int g = 0; g < FX; ++g) {
+            if (g < kPieces) {
+                tx.fetch(xs, wave, g, k, s.K);
+                if constexpr (YK != kAcross8) ty.fetch(ys, wave, g, k, s.K);
+                else ty.put(ys, g), ty.load(g);
+            }
+            if (g < FY) fy[0][g] = wide_fragment<YK, R>(yn, wn + 16 * g, 0, lane);
+            if (A1) fx[0][g] = wide_fragment<XK, R>(xn, wm + 16 * g, 0, lane);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j][g] = mfma<T>(fy[1][j], fx[1][g], acc[j][g]);
+            for (int j = 0; j < FY; ++j) acc[j][g] = mfma<T>(fy[1][j], fx[A1][g], acc[j][g]);
+            if (!A1) fx[0][g] = wide_fragment<XK, R>(xn, wm + 16 * g, 0, lane);
         }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // nothing is on its way to LDS any more, and nobody reads it
@@ -454,13 +543,14 @@ __global__ __launch_bounds__(kWideThreads, 2) void k_product_wide(Operand X, Ope
     asm volatile("" ::: "memory");
     // Through LDS, 16 rows of 64 fp32 sums of a wave at a time, so that a lane stores 16 bytes and a row 128: a lane of an accumulator
     // holds m = l % 16, n = 4 (l / 16) .. + 3. Each wave has its own 16 x 68 (the pitch spreads the banks).
+    static_assert(FY == 4, "64 columns a wave");
     constexpr int P = 68;
     float* tile = (float*)&lds[0][0][0] + wave * (16 * P);
     const int n = n0 + wn + 8 * (lane & 7);
     float bias[8];
     load_bias<T, 8>(ep, n, s.N, bias);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < FX; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(f32x4*)(tile + (lane & 15) * P + 16 * j + 4 * (lane >> 4)) = acc[j][i];
 #pragma unroll 1
@@ -495,7 +585,9 @@ __global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
     }
 }
 
-// dz = dy act'(z) and the slices' sums of its columns. A workgroup: 32 column pieces x 8 rows at a time.
+// dz = dy act'(z) and the slices' sums of its columns. A workgroup: 32 column pieces x 8 rows at a time, the loads of kRows of those
+// together.
+constexpr int kRows = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, float* __restrict__ partial,
                                                   int64_t M, int N, int act, int rows) {
@@ -506,17 +598,23 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
     const int64_t begin = (int64_t)blockIdx.y * rows, end = begin + rows < M ? begin + rows : M;
     float s[V] = {};
     if (left > 0)
-        for (int64_t m = begin + strand; m < end; m += 8) {
-            float g[V];
-            load_piece<T, V>(dy + m * N + n, left, g);
-            if (z) {                                               // dz NULL: the column sums alone are wanted
-                float a[V];
-                load_piece<T, V>(z + m * N + n, left, a);
-                act_slopes(g, a, act);
-                if (dz) store_piece<T, V>(dz + m * N + n, left, g);
+        for (int64_t m0 = begin + strand; m0 < end; m0 += 8 * kRows) {
+            float g[kRows][V], a[kRows][V];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const int64_t m = m0 + 8 * r, have = m < end ? left : 0;
+                load_piece<T, V>(dy + m * N + n, have, g[r]);
+                if (z) load_piece<T, V>(z + m * N + n, have, a[r]);
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[i] += g[i];               // before dz is rounded to its type
+            for (int r = 0; r < kRows; ++r) {
+                const int64_t m = m0 + 8 * r;
+                if (m >= end) break;
+                if (z) act_slopes(g[r], a[r], act);
+                if (dz) store_piece<T, V>(dz + m * N + n, left, g[r]);      // dz NULL: the column sums alone are wanted
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] += g[r][i];                // before dz is rounded to its type
+            }
         }
     if (!partial) return;
 #pragma unroll
@@ -537,6 +635,7 @@ __global__ __launch_bounds__(256) void k_columns_join(const float* __restrict__ 
     const int col = threadIdx.x & 31, strand = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
     float acc = 0.f;
     if (n < N)
+#pragma unroll 8
         for (int g = strand; g < slices; g += 8) acc += partial[(int64_t)g * N + n];
     s[strand][col] = acc;
     __syncthreads();
@@ -549,18 +648,27 @@ __global__ __launch_bounds__(256) void k_columns_join(const float* __restrict__ 
 // ---- plans ----------------------------------------------------------------------------------
 struct Plan {
     int tile;
+    bool wide;
     Shape s;
     int64_t ws() const { return s.slices > 1 ? (int64_t)s.slices * s.M * s.N * 4 : 0; }
 };
 
 // 128 x 128 tiles where they give every CU one, 64 x 64 otherwise; a contraction is cut while there are fewer than 512 workgroups
 // (two for each CU) and each keeps eight k steps. `wide`: the operands suit the 256 x 256 form, taken where it gives 192 CUs a tile.
-Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide = false) {
+Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide = false, bool packed = false) {
     Plan p;
     const int bk = dtype == URSA_F32 ? 32 : 64;
     const int64_t big = ((M + 127) / 128) * ((N + 127) / 128), huge = ((M + 255) / 256) * ((N + 255) / 256);
     p.tile = big >= 256 ? 128 : 64;
-    if (wide && huge >= 192) p.tile = 256;
+#ifdef NO256
+    wide = wide;
+    const bool no256 = true;
+#else
+    const bool no256 = false;
+#endif
+    const int64_t most = (K + bk - 1) / bk / 8 < 16 ? (K + bk - 1) / bk / 8 : 16;
+    if (!no256 && wide && (huge >= 192 || (packed && huge * most >= 192))) p.tile = 256;
+    p.wide = wide && p.tile >= 128;
     p.s.M = (int)M, p.s.N = (int)N, p.s.K = (int)K;
     p.s.tiles_m = (int)((M + p.tile - 1) / p.tile), p.s.tiles_n = (int)((N + p.tile - 1) / p.tile);
     const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, steps = (K + bk - 1) / bk;
@@ -589,9 +697,10 @@ template <typename T, int XK, int YK>
 int product(const Operand& x, const Operand& y, const Plan& p, Epilogue ep, hipStream_t st) {
     if (p.s.slices == 1) ep.partial = nullptr;
     const dim3 grid((unsigned)(p.s.tiles_m * p.s.tiles_n), (unsigned)p.s.slices);
-    if constexpr (!__is_same(T, float) && YK != kAcross8)
-        if (p.tile == 256) {
-            hipLaunchKernelGGL((k_product_wide<T, XK, YK>), grid, dim3(kWideThreads), 0, st, x, y, p.s, ep);
+    if constexpr (!__is_same(T, float))
+        if (p.wide) {
+            if (p.tile == 256) hipLaunchKernelGGL((k_product_wide<T, XK, YK, 256>), grid, dim3(512), 0, st, x, y, p.s, ep);
+            else hipLaunchKernelGGL((k_product_wide<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
             const int rc = launch_status();
             return rc || p.s.slices == 1 ? rc : join<T>(p, ep, st);
         }
@@ -651,7 +760,7 @@ int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T*
     if (dw && K) {
         const Epilogue ep{dw, nullptr, nullptr, nullptr, scratch, URSA_ACT_NONE};
         const Operand X{g, nullptr, N, (int)N}, Y{q ? (const void*)q : x, e, q ? (K + kBlock8 - 1) / kBlock8 * kBlock8 : K, (int)K};
-        const Plan p = plan_of(N, K, M, dtype, whole_pieces(dtype, g, N) && !q && whole_pieces(dtype, x, K));
+        const Plan p = plan_of(N, K, M, dtype, whole_pieces(dtype, g, N) && (q || whole_pieces(dtype, x, K)), q);
         rc = q ? product<T, kAcross, kAcross8>(X, Y, p, ep, st) : product<T, kAcross, kAcross>(X, Y, p, ep, st);
     }
     return rc;
@@ -659,8 +768,9 @@ int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T*
 
 // scratch: what either form of a plan takes (alignment decides). Of a backward call: dz (with an activation), then what one of its launches needs at a time - they run one after another
 int64_t most_ws(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-    const int64_t a = plan_of(M, N, K, dtype).ws(), b = plan_of(M, N, K, dtype, dtype != URSA_F32).ws();
-    return a > b ? a : b;
+    const bool wide = dtype != URSA_F32;
+    const int64_t a = plan_of(M, N, K, dtype).ws(), b = plan_of(M, N, K, dtype, wide).ws(), c = plan_of(M, N, K, dtype, wide, true).ws();
+    return a > b ? (a > c ? a : c) : (b > c ? b : c);
 }
 
 struct BwdScratch {

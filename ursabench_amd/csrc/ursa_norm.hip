@@ -144,36 +144,86 @@ struct NormBwd {
     float inv_d;
 };
 
-template <typename T, typename P, int TPR, int CV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(NormBwd<T, P> a) {
-    constexpr int V = Piece<T>::kN, C = CV / V, R = TPR < 256 ? 256 / TPR : 1;
+// a row's numbers of this thread as they are in memory
+template <typename T, int C>
+struct Raw {
+    T v[C][Piece<T>::kN];
+    template <int TPR>
+    __device__ __forceinline__ void load(const T* __restrict__ row, int t, int64_t D) {
+        constexpr int V = Piece<T>::kN;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int64_t d = (int64_t)(c * TPR + t) * V;
+            if (d + V <= D) {
+                __builtin_memcpy(v[c], row + d, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[c][i] = d + i < D ? row[d + i] : (T)0.f;
+            }
+        }
+    }
+};
+
+template <int V, int C>
+struct Raw8 {
+    int8_t v[C][V], e[C];
+    template <int TPR>
+    __device__ __forceinline__ void load(const int8_t* __restrict__ q, const int8_t* __restrict__ ex, int t, int64_t pitch) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int64_t d = (int64_t)(c * TPR + t) * V;
+            if (d < pitch) {
+                __builtin_memcpy(v[c], q + d, V);
+                e[c] = ex[d / kBlock8];
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[c][i] = 0;
+                e[c] = 0;
+            }
+        }
+    }
+};
+
+constexpr int bwd_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }      // rows of a wave or less: several in a workgroup
+
+// PACKED: x comes in its 8-bit form; DZ: a gradient reaches z by another way
+template <typename T, typename P, int TPR, int CV, bool PACKED, bool DZ>
+__global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) {
+    constexpr int V = Piece<T>::kN, C = CV / V, R = bwd_threads(TPR) / TPR;
     constexpr int kJoin = R > 1 ? R * TPR * CV : 32;
     __shared__ float red[kJoin];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-    const int64_t qpitch = (a.D + kBlock8 - 1) / kBlock8 * kBlock8;
+    const int64_t qpitch = (a.D + kBlock8 - 1) / kBlock8 * kBlock8, stride = (int64_t)gridDim.x * R;
     float dg[C][V] = {}, db[C][V] = {};
-    for (int64_t row = (int64_t)blockIdx.x * R + sub; row < a.M; row += (int64_t)gridDim.x * R) {
+    Raw<T, C> rx, rd, rz;
+    Raw8<V, C> rq;
+    float mean = 0.f, rstd = 0.f;
+    auto fetch = [&](int64_t row) {
+        if constexpr (PACKED) rq.template load<TPR>(a.q + row * qpitch, a.e + row * (qpitch / kBlock8), t, qpitch);
+        else rx.template load<TPR>(a.x + row * a.D, t, a.D);
+        rd.template load<TPR>(a.dy + row * a.D, t, a.D);
+        if constexpr (DZ) rz.template load<TPR>(a.dz + row * a.D, t, a.D);
+        mean = a.mean[row], rstd = a.rstd[row];
+    };
+    for (int64_t row = (int64_t)blockIdx.x * R + sub; row < a.M; row += stride) {
         const int64_t base = row * a.D;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float xh[C][V], tt[C][V];
+        fetch(row);                                              // all of it before the first sum waits for any
+        const float rs = rstd;
+        float xh[C][V], tt[C][V], z[C][V];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int64_t d = (int64_t)(c * TPR + t) * V, left = a.D - d;
-            if (a.q) {
-                if (d < qpitch) load_q<V>(a.q + row * qpitch + d, a.e[row * (qpitch / kBlock8) + d / kBlock8], xh[c]);
-                else
-#pragma unroll
-                    for (int i = 0; i < V; ++i) xh[c][i] = 0.f;
-            } else {
-                load_piece<T, V>(a.x + base + d, left, xh[c]);
-            }
-            load_piece<T, V>(a.dy + base + d, left, tt[c]);
             float g[V];
             if (a.gamma) load_piece<P, V>(a.gamma + d, left, g);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                xh[c][i] = (xh[c][i] - mean) * rstd;             // behind the row's end dy is 0, so these never count
+                float x;
+                if constexpr (PACKED) x = value8(rq.v[c][i], rq.e[c]);
+                else x = (float)rx.v[c][i];
+                if constexpr (DZ) z[c][i] = (float)rz.v[c][i];
+                tt[c][i] = (float)rd.v[c][i];
+                xh[c][i] = (x - mean) * rs;                      // behind the row's end dy is 0, so these never count
                 dg[c][i] += i < left ? tt[c][i] * xh[c][i] : 0.f;
                 db[c][i] += tt[c][i];
                 if (a.gamma) tt[c][i] *= g[i];
@@ -186,12 +236,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(NormBwd<T, P
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int64_t d = (int64_t)(c * TPR + t) * V, left = a.D - d;
-            float z[V];
-            if (a.dz) load_piece<T, V>(a.dz + base + d, left, z);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                tt[c][i] = rstd * (tt[c][i] - m1 - xh[c][i] * m2);
-                if (a.dz) tt[c][i] += z[i];
+                tt[c][i] = rs * (tt[c][i] - m1 - xh[c][i] * m2);
+                if constexpr (DZ) tt[c][i] += z[c][i];
             }
             if (a.dx) store_piece<T, V>(a.dx + base + d, left, tt[c]);
         }
@@ -336,6 +384,7 @@ __global__ __launch_bounds__(256) void k_norm_join(const float* __restrict__ par
     const int64_t j = (int64_t)blockIdx.x * 32 + col;          // 0 .. 2 D: dgamma, then dbeta
     float acc = 0.f;
     if (j < 2 * D)
+#pragma unroll 8
         for (int g = strand; g < groups; g += 8) acc += partial[(int64_t)g * 2 * D + j];
     s[strand][col] = acc;
     __syncthreads();
@@ -374,14 +423,18 @@ __global__ __launch_bounds__(256) void k_unpack8(const int8_t* __restrict__ q, c
 
 constexpr int64_t kLong = 16384;         // features that the register forms hold
 
-// rows side by side in one workgroup, by width (the dispatch below)
+// rows side by side in one workgroup of the forward, by width (the dispatch below)
 int rows_per_group(int64_t D) { return D <= 128 ? 16 : D <= 2048 ? 4 : 1; }
 
-// Workgroups of the backward's walk: enough to fill 256 CUs four times over (two for rows of a whole workgroup), and no more than
-// leave each four rows, so that the partial sums (2 D floats each) stay small beside the rows
+// Threads of a row in the backward's walk: 8 columns each, so that their sums leave registers for many waves (with 16 or 32 a CU holds
+// few, and 16,384 x 4,096 bf16 took 197 us instead of @@). Above 8,192: 16 columns.
+int bwd_row_threads(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+
+// Workgroups of the walk: 1,024 threads a CU, and no more than leave each row slot four rows, so that the partial sums (2 D floats
+// a workgroup: 16 MiB at most) stay small beside the rows
 int64_t bwd_groups(int64_t M, int64_t D) {
     if (D > kLong) return M < 64 ? M : 64;
-    const int64_t R = rows_per_group(D), most = R > 1 ? 1024 : 512, need = (M + 4 * R - 1) / (4 * R);
+    const int64_t tpr = bwd_row_threads(D), threads = bwd_threads((int)tpr), R = threads / tpr, most = 256 * 1024 / threads, need = (M + 4 * R - 1) / (4 * R);
     return need < most ? need : most;
 }
 
@@ -395,6 +448,13 @@ int norm_fwd(const NormFwd<T, P>& a, hipStream_t s) {
     return launch_status();
 }
 
+template <typename T, typename P, bool PACKED, bool DZ>
+auto norm_bwd_for(int64_t D) {
+    return D <= 128 ? k_norm_bwd<T, P, 16, 8, PACKED, DZ> : D <= 512 ? k_norm_bwd<T, P, 64, 8, PACKED, DZ> : D <= 1024 ? k_norm_bwd<T, P, 128, 8, PACKED, DZ>
+         : D <= 2048 ? k_norm_bwd<T, P, 256, 8, PACKED, DZ> : D <= 4096 ? k_norm_bwd<T, P, 512, 8, PACKED, DZ>
+         : D <= 8192 ? k_norm_bwd<T, P, 1024, 8, PACKED, DZ> : k_norm_bwd<T, P, 1024, 16, PACKED, DZ>;
+}
+
 template <typename T, typename P>
 int norm_bwd(const NormBwd<T, P>& a, P* dgamma, P* dbeta, hipStream_t s) {
     const int64_t D = a.D;
@@ -405,10 +465,9 @@ int norm_bwd(const NormBwd<T, P>& a, P* dgamma, P* dbeta, hipStream_t s) {
         if ((rc = launch_status())) return rc;
         if (a.partial) hipLaunchKernelGGL((k_norm_columns_long<T, P>), dim3((unsigned)((D + 256 * Piece<T>::kN - 1) / (256 * Piece<T>::kN)), groups), dim3(256), 0, s, a);
     } else {
-        void (*fn)(NormBwd<T, P>) = D <= 128 ? k_norm_bwd<T, P, 16, 8> : D <= 512 ? k_norm_bwd<T, P, 64, 8> : D <= 1024 ? k_norm_bwd<T, P, 64, 16>
-                                  : D <= 2048 ? k_norm_bwd<T, P, 64, 32> : D <= 4096 ? k_norm_bwd<T, P, 256, 16> : D <= 8192 ? k_norm_bwd<T, P, 256, 32>
-                                  : k_norm_bwd<T, P, 1024, 16>;
-        hipLaunchKernelGGL(fn, dim3(groups), dim3(D <= 8192 ? 256 : 1024), 0, s, a);
+        void (*fn)(NormBwd<T, P>) = a.q ? (a.dz ? norm_bwd_for<T, P, true, true>(D) : norm_bwd_for<T, P, true, false>(D))
+                                        : (a.dz ? norm_bwd_for<T, P, false, true>(D) : norm_bwd_for<T, P, false, false>(D));
+        hipLaunchKernelGGL(fn, dim3(groups), dim3(bwd_threads(bwd_row_threads(D))), 0, s, a);
     }
     if ((rc = launch_status()) || !a.partial) return rc;
     hipLaunchKernelGGL(k_norm_join<P>, dim3((unsigned)((2 * D + 31) / 32)), dim3(256), 0, s, (const float*)a.partial, groups, D, dgamma, dbeta);
