@@ -398,6 +398,12 @@ struct WideTile {
     }
 };
 
+// memory from `at` to `end`: reads behind it give 0
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(uint64_t at, uint64_t end) {
+    const int64_t left = (int64_t)(end - at);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff, 0x00027000);
+}
+
 // a kAcross8 operand: 8 bytes and their exponent a piece through registers, one stage ahead of the others; LDS holds what a kAcross
 // stage would
 template <typename T, int R, int THREADS>
@@ -416,15 +422,11 @@ struct WideTile<T, kAcross8, R, THREADS> {
         at_e = (uint64_t)o.e + (uint64_t)k_begin * pe + r0 / kBlock8, end_e = (uint64_t)o.e + (uint64_t)K * pe;
         to = (kr >> 1) * pair_pitch<R>() + (kr & 1) * R + (slot_of<R>(piece >> 1, kr) << 4) + (piece & 1) * 8;
     }
-    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(uint64_t at, uint64_t end) {
-        const int64_t left = (int64_t)(end - at);
-        return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff, 0x00027000);
-    }
     // piece i of the next stage; behind the last k: zeros
     __device__ __forceinline__ void load(int i) {
-        const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(buffer(at, end), offset + i * step, 0, 0));
+        const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(buffer_of(at, end), offset + i * step, 0, 0));
         __builtin_memcpy(c[i].v, &b, 8);
-        c[i].e = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buffer(at_e, end_e), offset_e + i * step_e, 0, 0);
+        c[i].e = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buffer_of(at_e, end_e), offset_e + i * step_e, 0, 0);
         if (i == kPieces - 1) at += (uint64_t)step * kPieces, at_e += (uint64_t)step_e * kPieces;
     }
     __device__ __forceinline__ void put(short* stage, int i) {
@@ -445,6 +447,32 @@ __device__ __forceinline__ s16x8 wide_fragment(const short* stage, int row0, int
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2 * pair_pitch<R>()));
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// A wave's 16 FX x 64 outputs through LDS, 16 rows of fp32 sums at a time, so that a lane stores 8 neighbours and a row is stored whole:
+// a lane of an accumulator holds m = l % 16, n = 4 (l / 16) .. + 3. Each wave has its own 16 x 68 floats (the pitch spreads the banks).
+template <typename T, int FX>
+__device__ __forceinline__ void store_tile(const f32x4 (&acc)[4][FX], float* lds, int wave, int lane, int m0, int n0, const Shape& s, const Epilogue& ep) {
+    constexpr int P = 68;
+    float* tile = lds + wave * (16 * P);
+    const int n = n0 + 8 * (lane & 7);
+    float bias[8];
+    load_bias<T, 8>(ep, n, s.N, bias);
+#pragma unroll
+    for (int i = 0; i < FX; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(f32x4*)(tile + (lane & 15) * P + 16 * j + 4 * (lane >> 4)) = acc[j][i];
+#pragma unroll 1
+        for (int r = 0; r < 2; ++r) {
+            const int row = 8 * r + (lane >> 3), m = m0 + 16 * i + row;
+            const float* from = tile + row * P + 8 * (lane & 7);
+            const f32x4 a = *(const f32x4*)from, b = *(const f32x4*)(from + 4);
+            float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            if (m >= s.M || n >= s.N) continue;
+            if (ep.partial) store_piece<float, 8>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
+            else finish<T, 8>(ep, m, n, s.N, v, bias);
+        }
     }
 }
 
@@ -541,29 +569,131 @@ __global__ __launch_bounds__(R == 256 ? 512 : 256, 2) void k_product_wide(Operan
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // nothing is on its way to LDS any more, and nobody reads it
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    // Through LDS, 16 rows of 64 fp32 sums of a wave at a time, so that a lane stores 16 bytes and a row 128: a lane of an accumulator
-    // holds m = l % 16, n = 4 (l / 16) .. + 3. Each wave has its own 16 x 68 (the pitch spreads the banks).
     static_assert(FY == 4, "64 columns a wave");
-    constexpr int P = 68;
-    float* tile = (float*)&lds[0][0][0] + wave * (16 * P);
-    const int n = n0 + wn + 8 * (lane & 7);
-    float bias[8];
-    load_bias<T, 8>(ep, n, s.N, bias);
-#pragma unroll
-    for (int i = 0; i < FX; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *(f32x4*)(tile + (lane & 15) * P + 16 * j + 4 * (lane >> 4)) = acc[j][i];
-#pragma unroll 1
-        for (int r = 0; r < 2; ++r) {
-            const int row = 8 * r + (lane >> 3), m = m0 + wm + 16 * i + row;
-            const float* from = tile + row * P + 8 * (lane & 7);
-            const f32x4 a = *(const f32x4*)from, b = *(const f32x4*)(from + 4);
-            float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-            if (m >= s.M || n >= s.N) continue;
-            if (ep.partial) store_piece<float, 8>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
-            else finish<T, 8>(ep, m, n, s.N, v, bias);
+    store_tile<T, FX>(acc, (float*)&lds[0][0][0], wave, lane, m0 + wm, n0 + wn, s, ep);
+}
+
+// ---- fp32: 256 x 128 outputs by eight waves, the operands split while they are staged ---------------------------------------
+// A wave owns 64 x 64 outputs; 24 fragment reads (three planes of each operand) feed 96 matrix instructions. Two stages of 32 k: while
+// one is multiplied, the numbers of the next, which are in registers already, are split and stored to the other, and those of the
+// one after it are fetched; one barrier a stage. 24 numbers a thread and stage take about 220 vector instructions, hidden by the matrix
+// instructions of the other wave of the SIMD. Buffer loads, as above; rows of at most 2^21 numbers, kFlat ones a multiple of 8.
+constexpr int kSplitM = 256, kSplitN = 128, kSplitK = 32, kSplitThreads = 512;
+constexpr int64_t kSplitMaxPitch = 1 << 21;
+
+template <int KIND, int R>
+struct SplitTile {
+    static constexpr int kPieces = R * kSplitK / 8 / kSplitThreads, P = KIND == kAcross8 ? 1 : 3, kShorts = P * R * kSplitK;
+    static constexpr int kSize = KIND == kAcross8 ? 1 : 4;
+    Chunk<float, KIND> c[kPieces];
+    uint64_t at, end, at_e, end_e;
+    uint32_t offset, step, offset_e, step_e;
+    int k0, to;                   // k of the pieces (kFlat) within the stage; where piece 0 goes
+    int64_t advance, advance_e;
+    __device__ __forceinline__ SplitTile(const Operand& o, int r0, int k_begin, int K, int tid) {
+        const uint64_t p = (uint64_t)o.p;
+        at_e = end_e = 0, offset_e = step_e = 0, advance_e = 0, k0 = 0;
+        if constexpr (KIND == kFlat) {
+            const int row = tid / (kSplitK / 8), piece = tid % (kSplitK / 8);               // piece i: 128 rows further
+            k0 = piece * 8, to = flat_at<kSplitK>(row, piece);
+            offset = (uint32_t)(row * o.pitch + k0) * 4, step = (uint32_t)(kSplitThreads / (kSplitK / 8) * o.pitch * 4), advance = kSplitK * 4;
+            at = p + ((uint64_t)r0 * o.pitch + k_begin) * 4, end = p + (uint64_t)o.rows * o.pitch * 4;
+        } else {
+            const int k = tid / (R / 8), piece = tid % (R / 8);                             // piece i: kSplitThreads / (R / 8) k further
+            to = across_at<R>(k, piece >> 1) + (piece & 1) * 8;
+            offset = (uint32_t)(k * o.pitch + piece * 8) * kSize, step = (uint32_t)(kSplitThreads / (R / 8) * o.pitch) * kSize;
+            advance = (int64_t)kSplitK * o.pitch * kSize;
+            at = p + ((uint64_t)k_begin * o.pitch + r0) * kSize, end = p + (uint64_t)K * o.pitch * kSize;
+            if constexpr (KIND == kAcross8) {
+                const int64_t pe = o.pitch / kBlock8;
+                offset_e = (uint32_t)(k * pe + piece / 4), step_e = (uint32_t)(kSplitThreads / (R / 8) * pe), advance_e = kSplitK * pe;
+                at_e = (uint64_t)o.e + (uint64_t)k_begin * pe + r0 / kBlock8, end_e = (uint64_t)o.e + (uint64_t)K * pe;
+            }
         }
     }
+    // piece i of the stage from k
+    __device__ __forceinline__ void load(int i, int k, int K) {
+        const __amdgpu_buffer_rsrc_t b = buffer_of(at, end);
+        uint32_t from = offset + i * step;
+        if constexpr (KIND == kFlat)
+            if (k + kSplitK > K) from = k + k0 < K ? from : 0x80000000u;                    // the row goes on with other numbers
+        if constexpr (KIND == kAcross8) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b64(b, from, 0, 0);
+            __builtin_memcpy(c[i].v, &v, 8);
+            c[i].e = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buffer_of(at_e, end_e), offset_e + i * step_e, 0, 0);
+        } else {
+            const auto lo = __builtin_amdgcn_raw_buffer_load_b128(b, from, 0, 0), hi = __builtin_amdgcn_raw_buffer_load_b128(b, from + 16, 0, 0);
+            __builtin_memcpy(c[i].v, &lo, 16);
+            __builtin_memcpy(c[i].v + 4, &hi, 16);
+        }
+        if (i == kPieces - 1) at += advance, at_e += advance_e;
+    }
+    __device__ __forceinline__ void put(short* stage, int i) {
+        constexpr int kMore = KIND == kFlat ? kSplitThreads / (kSplitK / 8) * kSplitK : kSplitThreads / (R / 8) * R;   // shorts from piece to piece
+        static_assert(KIND == kFlat || kPieces == 1 || kSplitThreads / (R / 8) % 8 == 0, "the permutation repeats");
+        s16x8 out[3];
+        split_chunk<float, KIND>(c[i], out);
+#pragma unroll
+        for (int p = 0; p < P; ++p) *(s16x8*)(stage + p * (R * kSplitK) + to + i * kMore) = out[p];
+    }
+};
+
+template <int XK, int YK>
+__global__ __launch_bounds__(kSplitThreads, 2) void k_product_split(Operand X, Operand Y, Shape s, Epilogue ep) {
+    typedef SplitTile<XK, kSplitM> TileX;
+    typedef SplitTile<YK, kSplitN> TileY;
+    constexpr int BK = kSplitK, PX = TileX::P, PY = TileY::P;
+    static_assert(TileX::kPieces == 2 && TileY::kPieces == 1, "three pieces a thread");
+    __shared__ __attribute__((aligned(16))) short lds[2][TileX::kShorts + TileY::kShorts];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, s, tm, tn);
+    const int m0 = tm * kSplitM, n0 = tn * kSplitN;
+    const int k_begin = blockIdx.y * s.k_slice, k_end = s.K - k_begin < s.k_slice ? s.K : k_begin + s.k_slice;
+    const int steps = (k_end - k_begin + BK - 1) / BK;
+    const int wm = (wave & 3) * 64, wn = (wave >> 2) * 64;
+    TileX tx(X, m0, k_begin, s.K, tid);
+    TileY ty(Y, n0, k_begin, s.K, tid);
+    f32x4 acc[4][4] = {};                                 // [n][m]
+    tx.load(0, k_begin, s.K), tx.load(1, k_begin, s.K), ty.load(0, k_begin, s.K);
+    tx.put(lds[0], 0), tx.put(lds[0], 1), ty.put(lds[0] + TileX::kShorts, 0);
+    tx.load(0, k_begin + BK, s.K), tx.load(1, k_begin + BK, s.K), ty.load(0, k_begin + BK, s.K);
+    for (int t = 0; t < steps; ++t) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                     // this stage is stored, and nobody reads the other one
+        asm volatile("" ::: "memory");
+        const short *xs = lds[t & 1], *ys = xs + TileX::kShorts;
+        short* next = lds[(t + 1) & 1];
+        const int k = k_begin + (t + 2) * BK;
+        s16x8 fx[PX][4], fy[2][PY];
+#pragma unroll
+        for (int p = 0; p < PY; ++p) fy[0][p] = fragment<YK, BK, kSplitN>(ys + p * (kSplitN * BK), wn, 0, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int p = 0; p < PX; ++p) fx[p][i] = fragment<XK, BK, kSplitM>(xs + p * (kSplitM * BK), wm + 16 * i, 0, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j < 3) {
+#pragma unroll
+                for (int p = 0; p < PY; ++p) fy[(j + 1) & 1][p] = fragment<YK, BK, kSplitN>(ys + p * (kSplitN * BK), wn + 16 * (j + 1), 0, lane);
+            }
+            // past the last step nobody uses what these bring
+            if (j < 2) tx.put(next, j), tx.load(j, k, s.K);
+            if (j == 2) ty.put(next + TileX::kShorts, 0), ty.load(0, k, s.K);
+#pragma unroll
+            for (int px = PX - 1; px >= 0; --px)          // small products first
+#pragma unroll
+                for (int py = PY - 1; py >= 0; --py)
+                    if (px + py <= 2)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[j][i] = mfma<bf16>(fy[j & 1][py], fx[px][i], acc[j][i]);
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    store_tile<float, 4>(acc, (float*)&lds[0][0], wave, lane, m0 + wm, n0 + wn, s, ep);
 }
 
 // the slices of a cut contraction, added in ascending order, and the epilogue
@@ -647,35 +777,36 @@ __global__ __launch_bounds__(256) void k_columns_join(const float* __restrict__ 
 
 // ---- plans ----------------------------------------------------------------------------------
 struct Plan {
-    int tile;
-    bool wide;
+    int tm, tn;                  // outputs of a workgroup
+    bool wide;                   // the large forms: k_product_wide, k_product_split
     Shape s;
     int64_t ws() const { return s.slices > 1 ? (int64_t)s.slices * s.M * s.N * 4 : 0; }
 };
 
-// 128 x 128 tiles where they give every CU one, 64 x 64 otherwise; a contraction is cut while there are fewer than 512 workgroups
-// (two for each CU) and each keeps eight k steps. `wide`: the operands suit the 256 x 256 form, taken where it gives 192 CUs a tile.
-Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide = false, bool packed = false) {
+// The form by the number of workgroups that it gives the 256 CUs, and the cut of the contraction where there are fewer than one (two
+// of the smaller forms) for each: at most 16 slices of at least eight k steps. `wide`: the operands suit the large forms (see there);
+// `packed`: one of them comes in 8 bits.
+Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide, bool packed) {
     Plan p;
     const int bk = dtype == URSA_F32 ? 32 : 64;
-    const int64_t big = ((M + 127) / 128) * ((N + 127) / 128), huge = ((M + 255) / 256) * ((N + 255) / 256);
-    p.tile = big >= 256 ? 128 : 64;
-#ifdef NO256
-    wide = wide;
-    const bool no256 = true;
-#else
-    const bool no256 = false;
-#endif
-    const int64_t most = (K + bk - 1) / bk / 8 < 16 ? (K + bk - 1) / bk / 8 : 16;
-    if (!no256 && wide && (huge >= 192 || (packed && huge * most >= 192))) p.tile = 256;
-    p.wide = wide && p.tile >= 128;
+    const int64_t steps = (K + bk - 1) / bk, most = steps / 8 < 16 ? steps / 8 : 16;
+    const auto tiles_of = [&](int tm, int tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
+    const int64_t big = tiles_of(128, 128);
+    p.tm = p.tn = big >= 256 ? 128 : 64;
+    p.wide = false;
+    if (wide && dtype == URSA_F32) {
+        const int64_t n = tiles_of(kSplitM, kSplitN);
+        if (n >= 192 || (n >= 96 && n * most >= 192)) p.tm = kSplitM, p.tn = kSplitN, p.wide = true;
+    } else if (wide) {
+        const int64_t n = tiles_of(256, 256);
+        if (n >= 192 || (packed && n * most >= 192)) p.tm = p.tn = 256;
+        p.wide = p.tm >= 128;
+    }
     p.s.M = (int)M, p.s.N = (int)N, p.s.K = (int)K;
-    p.s.tiles_m = (int)((M + p.tile - 1) / p.tile), p.s.tiles_n = (int)((N + p.tile - 1) / p.tile);
-    const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, steps = (K + bk - 1) / bk;
-    const int64_t want = p.tile == 256 ? 256 : 512;
+    p.s.tiles_m = (int)((M + p.tm - 1) / p.tm), p.s.tiles_n = (int)((N + p.tn - 1) / p.tn);
+    const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, want = p.tm == 256 ? 256 : 512;
     int64_t cut = tiles < want && tiles ? want / tiles : 1;
-    if (cut > steps / 8) cut = steps / 8;
-    if (cut > 16) cut = 16;
+    if (cut > most) cut = most;
     if (cut < 1) cut = 1;
     const int64_t per = (steps + cut - 1) / cut;
     p.s.k_slice = (int)((per > 0 ? per : 1) * bk);
@@ -690,25 +821,26 @@ int join(const Plan& p, const Epilogue& ep, hipStream_t st) {
     return launch_status();
 }
 
-// whether an operand's rows (of `pitch` elements) and start suit 16-byte pieces
-bool whole_pieces(int32_t dtype, const void* p, int64_t pitch) { return dtype != URSA_F32 && pitch % 8 == 0 && pitch <= kWideMaxPitch && ((uintptr_t)p & 15) == 0; }
+// whether an operand (rows of `pitch` elements) suits the large forms
+bool suits(int32_t dtype, int kind, const void* p, int64_t pitch) {
+    return dtype == URSA_F32 ? pitch <= kSplitMaxPitch && (kind != kFlat || pitch % 8 == 0) : pitch % 8 == 0 && pitch <= kWideMaxPitch && ((uintptr_t)p & 15) == 0;
+}
 
 template <typename T, int XK, int YK>
 int product(const Operand& x, const Operand& y, const Plan& p, Epilogue ep, hipStream_t st) {
     if (p.s.slices == 1) ep.partial = nullptr;
     const dim3 grid((unsigned)(p.s.tiles_m * p.s.tiles_n), (unsigned)p.s.slices);
-    if constexpr (!__is_same(T, float))
-        if (p.wide) {
-            if (p.tile == 256) hipLaunchKernelGGL((k_product_wide<T, XK, YK, 256>), grid, dim3(512), 0, st, x, y, p.s, ep);
-            else hipLaunchKernelGGL((k_product_wide<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
-            const int rc = launch_status();
-            return rc || p.s.slices == 1 ? rc : join<T>(p, ep, st);
-        }
-    if (p.tile == 128) hipLaunchKernelGGL((k_product<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
-    else hipLaunchKernelGGL((k_product<T, XK, YK, 64>), grid, dim3(256), 0, st, x, y, p.s, ep);
-    int rc = launch_status();
-    if (rc || p.s.slices == 1) return rc;
-    return join<T>(p, ep, st);
+    if (p.wide) {
+        if constexpr (__is_same(T, float)) hipLaunchKernelGGL((k_product_split<XK, YK>), grid, dim3(kSplitThreads), 0, st, x, y, p.s, ep);
+        else if (p.tm == 256) hipLaunchKernelGGL((k_product_wide<T, XK, YK, 256>), grid, dim3(512), 0, st, x, y, p.s, ep);
+        else hipLaunchKernelGGL((k_product_wide<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
+    } else if (p.tm == 128) {
+        hipLaunchKernelGGL((k_product<T, XK, YK, 128>), grid, dim3(256), 0, st, x, y, p.s, ep);
+    } else {
+        hipLaunchKernelGGL((k_product<T, XK, YK, 64>), grid, dim3(256), 0, st, x, y, p.s, ep);
+    }
+    const int rc = launch_status();
+    return rc || p.s.slices == 1 ? rc : join<T>(p, ep, st);
 }
 
 #define URSA_LINEAR_TYPES(dtype, call) (dtype == URSA_F32 ? call(float) : dtype == URSA_BF16 ? call(bf16) : call(f16))
@@ -755,12 +887,12 @@ int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T*
     const T* g = dz ? dz : dy;
     if (dx && M && K) {
         const Operand X{g, nullptr, N, (int)M}, Y{w, nullptr, K, (int)K};
-        if ((rc = product<T, kFlat, kAcross>(X, Y, plan_of(M, K, N, dtype, whole_pieces(dtype, g, N) && whole_pieces(dtype, w, K)), {dx, nullptr, nullptr, nullptr, scratch, URSA_ACT_NONE}, st))) return rc;
+        if ((rc = product<T, kFlat, kAcross>(X, Y, plan_of(M, K, N, dtype, suits(dtype, kFlat, g, N) && suits(dtype, kAcross, w, K), false), {dx, nullptr, nullptr, nullptr, scratch, URSA_ACT_NONE}, st))) return rc;
     }
     if (dw && K) {
         const Epilogue ep{dw, nullptr, nullptr, nullptr, scratch, URSA_ACT_NONE};
         const Operand X{g, nullptr, N, (int)N}, Y{q ? (const void*)q : x, e, q ? (K + kBlock8 - 1) / kBlock8 * kBlock8 : K, (int)K};
-        const Plan p = plan_of(N, K, M, dtype, whole_pieces(dtype, g, N) && (q || whole_pieces(dtype, x, K)), q);
+        const Plan p = plan_of(N, K, M, dtype, suits(dtype, kAcross, g, N) && (q ? K <= kSplitMaxPitch : suits(dtype, kAcross, x, K)), q != nullptr);
         rc = q ? product<T, kAcross, kAcross8>(X, Y, p, ep, st) : product<T, kAcross, kAcross>(X, Y, p, ep, st);
     }
     return rc;
@@ -768,8 +900,7 @@ int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T*
 
 // scratch: what either form of a plan takes (alignment decides). Of a backward call: dz (with an activation), then what one of its launches needs at a time - they run one after another
 int64_t most_ws(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-    const bool wide = dtype != URSA_F32;
-    const int64_t a = plan_of(M, N, K, dtype).ws(), b = plan_of(M, N, K, dtype, wide).ws(), c = plan_of(M, N, K, dtype, wide, true).ws();
+    const int64_t a = plan_of(M, N, K, dtype, false, false).ws(), b = plan_of(M, N, K, dtype, true, false).ws(), c = plan_of(M, N, K, dtype, true, true).ws();
     return a > b ? (a > c ? a : c) : (b > c ? b : c);
 }
 
@@ -799,7 +930,7 @@ extern "C" int ursa_linear_act(const void* x, const void* w, const void* bias, c
                                int64_t N, int64_t K, int32_t dtype, int32_t act, ursa_stream_t stream) {
     if (act < URSA_ACT_NONE || act > URSA_ACT_SILU) return URSA_EFLAGS;
     if (int rc = check(M, N, K, dtype)) return rc > 0 ? URSA_OK : rc;
-    const Plan p = plan_of(M, N, K, dtype, whole_pieces(dtype, x, K) && whole_pieces(dtype, w, K));
+    const Plan p = plan_of(M, N, K, dtype, suits(dtype, kFlat, x, K) && suits(dtype, kFlat, w, K), false);
     if ((K && (!x || !w)) || !y || (p.ws() && !ws)) return URSA_ENULL;
     if (misaligned(dtype, (uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)z) || (uintptr_t)ws & 3) return URSA_EALIGN;
     const Operand X{x, nullptr, K, (int)M}, Y{w, nullptr, K, (int)N};
