@@ -35,8 +35,8 @@ def test_linear_entries_refuse_bad_arguments(lib, p):
     assert fwd(p + 2, p, None, None, p, None, None, 4, 4, 4, F32, 0, None) == -3
     assert fwd(p, p, p + 1, None, p, None, None, 4, 4, 4, BF16, 0, None) == -3
     assert fwd(None, None, None, None, None, None, None, 0, 4, 4, F32, 0, None) == 0  # no rows: nothing to do
-    assert ws(64, 64, 1 << 16, F32) > 0
-    assert fwd(p, p, None, None, p, None, None, 64, 64, 1 << 16, F32, 0, None) == -1  # a cut contraction without its scratch
+    assert ws(65, 64, 1 << 16, F32) > 0 and ws(4, 64, 1 << 16, F32) > 0 and ws(4, 64, 1 << 10, F32) == 0
+    assert fwd(p, p, None, None, p, None, None, 65, 64, 1 << 16, F32, 0, None) == -1  # a cut contraction without its scratch
     ok = dict(dy=p, x=p, q=None, e=None, w=p, z=p, dx=p, dw=p, db=p, ws=p, M=4, N=4, K=4, t=F16, act=2)
     back = lambda **k: bwd(*{**ok, **k}.values(), None)                               # noqa: E731
     assert back(t=3) == -4 and back(act=4) == -4 and back(M=-1) == -2 and back(N=1 << 31) == -2 and back(K=1 << 31) == -2

@@ -232,6 +232,17 @@ def _tptr(t, name, dtype, n=None, device=None, optional=False):
     return t.data_ptr()
 
 
+def _addr(t, name, dtype, n, like):
+    """The address of an operand of n elements of `dtype` on the device of `like` (None: 0): the checks of _tptr in their cheapest
+    form, and _tptr itself for what they find."""
+    if t is None:
+        return None
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_contiguous() and t.numel() == n and t.get_device() == like.get_device()
+            and t.is_cuda):
+        return t.data_ptr()
+    return _tptr(t, name, dtype, n, like.device)
+
+
 def _raw_stream(index):
     """torch's current stream on device `index`, as the address the C ABI takes (0.1 us; current_stream().cuda_stream: 1.9)."""
     return torch._C._cuda_getCurrentRawStream(index)
@@ -953,12 +964,14 @@ class HipKernels:
         _check(self.lib, rc, 'ursa_bn_relu_pool_bwd_f32')
 
     # K15 -----------------------------------------------------------------------------
-    def _launch(self, fn, dev, *args):
-        if torch.cuda.current_device() == dev.index:
-            rc = fn(*args, _raw_stream(dev.index))
+    def _launch(self, fn, on, *args):
+        """fn(*args, torch's current stream) on the device of the tensor `on`."""
+        index = on.get_device()
+        if torch.cuda.current_device() == index:
+            rc = fn(*args, _raw_stream(index))
         else:
-            with torch.cuda.device(dev):
-                rc = fn(*args, _raw_stream(dev.index))
+            with torch.cuda.device(index):
+                rc = fn(*args, _raw_stream(index))
         if rc:
             _check(self.lib, rc, fn.__name__)
 
@@ -974,15 +987,13 @@ class HipKernels:
         dt, act = _element_type(x, 'x'), self._act(activation)
         if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
             raise ValueError(f'x {tuple(x.shape)} and w {tuple(w.shape)} should be [M, K] and [N, K]')
-        (M, K), N, t, dev = x.shape, w.shape[0], x.dtype, x.device
-        px, pw = _tptr(x, 'x', t), _tptr(w, 'w', t, None, dev)
-        pb = None if bias is None else _tptr(bias, 'bias', t, N, dev)
-        pr = None if residual is None else _tptr(residual, 'residual', t, M * N, dev)
+        (M, K), N, t, lib = x.shape, w.shape[0], x.dtype, self.lib
+        px, pw, pb, pr = _addr(x, 'x', t, M * K, x), _addr(w, 'w', t, N * K, x), _addr(bias, 'bias', t, N, x), _addr(residual, 'residual', t, M * N, x)
         y = x.new_empty((M, N))
         z = x.new_empty((M, N)) if save_z else None
-        n = self.lib.ursa_linear_ws_bytes(M, N, K, dt)
+        n = lib.ursa_linear_ws_bytes(M, N, K, dt)
         ws = x.new_empty(n, dtype=torch.uint8) if n else None
-        self._launch(self.lib.ursa_linear_act, dev, px, pw, pb, pr, y.data_ptr(), None if z is None else z.data_ptr(),
+        self._launch(lib.ursa_linear_act, x, px, pw, pb, pr, y.data_ptr(), None if z is None else z.data_ptr(),
                      None if ws is None else ws.data_ptr(), M, N, K, dt, act)
         return y, z
 
@@ -991,25 +1002,27 @@ class HipKernels:
         """(dx, dw, db) of linear_act from dy [M, N], None for what is not wanted. w is read for dx; x - or its 8-bit form (q, e) of
         `in_features` columns - for dw; z with an activation."""
         dt, act = _element_type(dy, 'dy'), self._act(activation)
-        (M, N), t, dev = dy.shape, dy.dtype, dy.device
+        (M, N), t, lib = dy.shape, dy.dtype, self.lib
         K = int(in_features) if in_features is not None else (x if x is not None else w).shape[1]
         if need_dw and (x is None) == (q is None):
             raise ValueError('linear_backward wants x or its 8-bit form')
-        pd = _tptr(dy, 'dy', t)
+        if (need_dx and w is None) or (act and z is None):
+            raise ValueError('linear_backward wants w for dx, and z with an activation')
+        pd = _addr(dy, 'dy', t, M * N, dy)
         px = pq = pe = None
         if need_dw:
             if q is None:
-                px = _tptr(x, 'x', t, M * K, dev)
+                px = _addr(x, 'x', t, M * K, dy)
             else:
-                pq, pe = self._act8_ptrs(q, e, M, K, dev)
-        pw = _tptr(w, 'w', t, N * K, dev) if need_dx else None
-        pz = _tptr(z, 'z', t, M * N, dev) if act else None
+                pq, pe = self._act8_ptrs(q, e, M, K, dy)
+        pw = _addr(w, 'w', t, N * K, dy) if need_dx else None
+        pz = _addr(z, 'z', t, M * N, dy) if act else None
         dx = dy.new_empty((M, K)) if need_dx else None
         dw = dy.new_empty((N, K)) if need_dw else None
         db = dy.new_empty(N) if need_db else None
-        n = self.lib.ursa_linear_bwd_ws_bytes(M, N, K, dt, act, need_dx, need_dw, need_db)
+        n = lib.ursa_linear_bwd_ws_bytes(M, N, K, dt, act, need_dx, need_dw, need_db)
         ws = dy.new_empty(n, dtype=torch.uint8) if n else None
-        self._launch(self.lib.ursa_linear_bwd, dev, pd, px, pq, pe, pw, pz, None if dx is None else dx.data_ptr(),
+        self._launch(lib.ursa_linear_bwd, dy, pd, px, pq, pe, pw, pz, None if dx is None else dx.data_ptr(),
                      None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
                      M, N, K, dt, act)
         return dx, dw, db
@@ -1025,28 +1038,33 @@ class HipKernels:
         return dt, pt
 
     def layer_norm(self, x, gamma=None, beta=None, *, eps, addend=None, stats=False, save8=False):
-        """x [M, D] -> (z, y, mean, rstd, q, e): z the sum with `addend` (x without one); mean / rstd with `stats`, q / e (the
-        8-bit form of z) with `save8`, None otherwise."""
+        """x [M, D] -> (z, y, stats, q, e): z the sum with `addend` (x without one); [2, M] mean and 1 / std with `stats`, q / e
+        (the 8-bit form of z) with `save8`, None otherwise."""
         dt, pt = self._norm_param_type(x, gamma, beta)
         if x.dim() != 2 or x.shape[1] < 1:
             raise ValueError(f'x {tuple(x.shape)} should be [M, D]')
-        (M, D), t, dev = x.shape, x.dtype, x.device
-        px, pa = _tptr(x, 'x', t), _tptr(addend, 'addend', t, M * D, dev, True)
-        pg, pb = _tptr(gamma, 'gamma', pt, D, dev, True), _tptr(beta, 'beta', pt, D, dev, True)
-        z = x if addend is None else torch.empty_like(x)
-        y = torch.empty_like(x)
-        ms = x.new_empty((2, M), dtype=torch.float32) if stats else None
-        q, e = self._act8_empty(x, M, D) if save8 else (None, None)
-        pm = None if ms is None else ms.data_ptr()
-        self._launch(self.lib.ursa_layer_norm_fwd, dev, px, pa, None if addend is None else z.data_ptr(), y.data_ptr(), pg, pb, pm,
-                     None if ms is None else pm + 4 * M, None if q is None else q.data_ptr(), None if q is None else e.data_ptr(),
-                     M, D, float(eps), dt, DTYPES[pt])
-        return z, y, (None if ms is None else ms[0]), (None if ms is None else ms[1]), q, e
+        (M, D), t = x.shape, x.dtype
+        px, pa, pg, pb = _addr(x, 'x', t, M * D, x), _addr(addend, 'addend', t, M * D, x), _addr(gamma, 'gamma', pt, D, x), _addr(beta, 'beta', pt, D, x)
+        z = x if addend is None else x.new_empty((M, D))
+        y = x.new_empty((M, D))
+        ms, pm, pr = None, None, None
+        if stats:
+            ms = x.new_empty((2, M), dtype=torch.float32)
+            pm = ms.data_ptr()
+            pr = pm + 4 * M
+        q = e = pq = pe = None
+        if save8:
+            q, e = self._act8_empty(x, M, D)
+            pq, pe = q.data_ptr(), e.data_ptr()
+        self._launch(self.lib.ursa_layer_norm_fwd, x, px, pa, None if addend is None else z.data_ptr(), y.data_ptr(), pg, pb, pm, pr, pq, pe,
+                     M, D, eps, dt, DTYPES[pt])
+        return z, y, ms, q, e
 
-    def layer_norm_backward(self, dy, mean, rstd, gamma=None, *, x=None, q=None, e=None, dz=None, need_dx=True, param_type=None,
+    def layer_norm_backward(self, dy, stats, gamma=None, *, x=None, q=None, e=None, dz=None, need_dx=True, param_type=None,
                             need_dgamma=False, need_dbeta=False):
-        """(dx, dgamma, dbeta), None for what is not wanted; dgamma / dbeta of `param_type` (gamma's)."""
-        dt, t, dev = _element_type(dy, 'dy'), dy.dtype, dy.device
+        """(dx, dgamma, dbeta) from dy [M, D] and the forward's `stats`, None for what is not wanted; dgamma / dbeta of `param_type`
+        (gamma's). x: what was normalised, as itself or as its 8-bit form (q, e)."""
+        dt, t = _element_type(dy, 'dy'), dy.dtype
         pt = gamma.dtype if gamma is not None else (param_type or t)
         if pt not in (t, torch.float32):
             raise TypeError(f'gamma / beta must be {str(t)[6:]} or float32, got {pt}')
@@ -1055,14 +1073,16 @@ class HipKernels:
         M, D = dy.shape
         pq = pe = None
         if q is not None:
-            pq, pe = self._act8_ptrs(q, e, M, D, dev)
-        args = (None if x is None else _tptr(x, 'x', t, M * D, dev), pq, pe, _tptr(dy, 'dy', t), _tptr(dz, 'dz', t, M * D, dev, True),
-                _tptr(gamma, 'gamma', pt, D, dev, True), _ptr(mean, 'mean', M, dev), _ptr(rstd, 'rstd', M, dev))
-        dx = torch.empty_like(dy) if need_dx else None
+            pq, pe = self._act8_ptrs(q, e, M, D, dy)
+        pm = _addr(stats, 'stats', torch.float32, 2 * M, dy)
+        px, pd, pz, pg = _addr(x, 'x', t, M * D, dy), _addr(dy, 'dy', t, M * D, dy), _addr(dz, 'dz', t, M * D, dy), _addr(gamma, 'gamma', pt, D, dy)
+        dx = dy.new_empty((M, D)) if need_dx else None
         dg = dy.new_empty(D, dtype=pt) if need_dgamma else None
         db = dy.new_empty(D, dtype=pt) if need_dbeta else None
         ws = dy.new_empty(self.lib.ursa_layer_norm_ws_floats(M, D), dtype=torch.float32) if need_dgamma or need_dbeta else None
-        self._launch(self.lib.ursa_layer_norm_bwd, dev, *args, *(None if o is None else o.data_ptr() for o in (dx, dg, db, ws)), M, D, dt, DTYPES[pt])
+        self._launch(self.lib.ursa_layer_norm_bwd, dy, px, pq, pe, pd, pz, pg, pm, pm + 4 * M, None if dx is None else dx.data_ptr(),
+                     None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
+                     M, D, dt, DTYPES[pt])
         return dx, dg, db
 
     # K17 -----------------------------------------------------------------------------
@@ -1072,9 +1092,11 @@ class HipKernels:
         return x.new_empty((M, blocks * ACT8_BLOCK), dtype=torch.int8), x.new_empty((M, blocks), dtype=torch.int8)
 
     @staticmethod
-    def _act8_ptrs(q, e, M, D, dev):
+    def _act8_ptrs(q, e, M, D, like):
+        if q is None or e is None:
+            raise ValueError('the 8-bit form is q and e')
         blocks = -(-D // ACT8_BLOCK)
-        return (_tptr(q, 'q', torch.int8, M * blocks * ACT8_BLOCK, dev), _tptr(e, 'e', torch.int8, M * blocks, dev))
+        return _addr(q, 'q', torch.int8, M * blocks * ACT8_BLOCK, like), _addr(e, 'e', torch.int8, M * blocks, like)
 
     def act8_pack(self, x):
         """x [M, D] -> (q [M, P], e [M, P / 32]), P = D rounded up to a multiple of 32."""
@@ -1083,16 +1105,16 @@ class HipKernels:
             raise ValueError(f'x {tuple(x.shape)} should be [M, D]')
         M, D = x.shape
         q, e = self._act8_empty(x, M, D)
-        self._launch(self.lib.ursa_act8_pack, x.device, px, q.data_ptr(), e.data_ptr(), M, D, dt)
+        self._launch(self.lib.ursa_act8_pack, x, px, q.data_ptr(), e.data_ptr(), M, D, dt)
         return q, e
 
     def act8_unpack(self, q, e, D, dtype):
         if dtype not in DTYPES:
             raise TypeError(f'an activation must be float32, bfloat16 or float16, got {dtype}')
         M = q.shape[0]
-        pq, pe = self._act8_ptrs(q, e, M, D, q.device)
+        pq, pe = self._act8_ptrs(q, e, M, D, q)
         x = q.new_empty((M, D), dtype=dtype)
-        self._launch(self.lib.ursa_act8_unpack, q.device, pq, pe, x.data_ptr(), M, D, DTYPES[dtype])
+        self._launch(self.lib.ursa_act8_unpack, q, pq, pe, x.data_ptr(), M, D, DTYPES[dtype])
         return x
 
 

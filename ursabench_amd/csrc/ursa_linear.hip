@@ -696,6 +696,86 @@ __global__ __launch_bounds__(kSplitThreads, 2) void k_product_split(Operand X, O
     store_tile<float, 4>(acc, (float*)&lds[0][0], wave, lane, m0 + wm, n0 + wn, s, ep);
 }
 
+// ---- few rows: y for M <= 16 MT, the weights read once ----------------------------------------------------------------------
+// Bound by the weights' bytes. A workgroup owns 16 features; its waves take turns at 32 kAhead k, whose pieces of 16 rows of W it
+// fetches together, straight into the registers of the matrix instruction - no LDS on the way, no barrier until the waves' sums
+// are added up, in their order, by LDS. fp32: the fp32 instruction, eight times for 32 k (lane l has k = 8 (l / 16) + i for the i-th, in
+// both operands); there is time for it beside the loads, and the split would cost more vector work than that.
+template <typename T, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_rows(Operand X, Operand Y, Shape s, Epilogue ep) {
+    constexpr int kAhead = __is_same(T, float) ? (MT == 1 ? 4 : 2) : (MT == 1 ? 8 : MT == 2 ? 4 : 2);
+    __shared__ __attribute__((aligned(16))) float sums[WAVES][MT][16][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, kl = 8 * (lane >> 4);
+    const int n0 = blockIdx.x * 16;
+    const int k_begin = blockIdx.y * s.k_slice, k_end = s.K - k_begin < s.k_slice ? s.K : k_begin + s.k_slice;
+    // rows past the end: the last one again, its sums are not stored
+    const T* w = (const T*)Y.p + (int64_t)(n0 + r < s.N ? n0 + r : s.N - 1) * Y.pitch + kl;
+    const T* x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = (const T*)X.p + (int64_t)(16 * i + r < s.M ? 16 * i + r : s.M - 1) * X.pitch + kl;
+    f32x4 acc[MT] = {};
+    struct Piece8 { T v[8]; };
+    const auto multiply = [&](const Piece8& a, const Piece8& b, f32x4& c) {
+        if constexpr (__is_same(T, float)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+        } else {
+            c = mfma<T>(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c);
+        }
+    };
+    int k = k_begin + wave * 32 * kAhead;
+    for (; k + 32 * kAhead <= k_end; k += WAVES * 32 * kAhead) {
+        Piece8 pw[kAhead], px[kAhead][MT];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) __builtin_memcpy(&pw[u], w + k + 32 * u, sizeof(Piece8));
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) __builtin_memcpy(&px[u][i], x[i] + k + 32 * u, sizeof(Piece8));
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) multiply(pw[u], px[u][i], acc[i]);
+    }
+    for (const int turn = k + 32 * kAhead; k < k_end && k < turn; k += 32) {      // the slice's end, by the wave whose turn it is
+        Piece8 pw, px;
+        const auto part = [&](const T* from, Piece8& p) {
+            if (k + kl + 8 <= k_end) {
+                __builtin_memcpy(&p, from + k, sizeof p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p.v[i] = k + kl + i < k_end ? from[k + i] : (T)0.f;
+            }
+        };
+        part(w, pw);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            part(x[i], px);
+            multiply(pw, px, acc[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *(f32x4*)&sums[wave][i][r][4 * (lane >> 4)] = acc[i];      // [m][n]
+    __syncthreads();
+    for (int id = tid; id < 64 * MT; id += 64 * WAVES) {
+        const int m = id >> 2, n = n0 + 4 * (id & 3);
+        if (m >= s.M || n >= s.N) continue;
+        float v[4] = {}, b[4];
+#pragma unroll
+        for (int u = 0; u < WAVES; ++u) {
+            const f32x4 t = *(const f32x4*)&sums[u][m >> 4][m & 15][4 * (id & 3)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += t[i];
+        }
+        if (ep.partial) {
+            store_piece<float, 4>(ep.partial + ((int64_t)blockIdx.y * s.M + m) * s.N + n, s.N - n, v);
+        } else {
+            load_bias<T, 4>(ep, n, s.N, b);
+            finish<T, 4>(ep, m, n, s.N, v, b);
+        }
+    }
+}
+
 // the slices of a cut contraction, added in ascending order, and the epilogue
 template <typename T>
 __global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
@@ -720,7 +800,7 @@ __global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
 constexpr int kRows = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, float* __restrict__ partial,
-                                                  int64_t M, int N, int act, int rows) {
+                                                  T* __restrict__ db, int64_t M, int N, int act, int rows) {
     constexpr int V = Piece<T>::kN;
     __shared__ float red[8][32 * V];
     const int piece = threadIdx.x & 31, strand = threadIdx.x >> 5;
@@ -746,7 +826,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
                 for (int i = 0; i < V; ++i) s[i] += g[r][i];                // before dz is rounded to its type
             }
         }
-    if (!partial) return;
+    if (!partial && !db) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) red[strand][piece * V + i] = s[i];
     __syncthreads();
@@ -755,7 +835,9 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
 #pragma unroll
         for (int w = 1; w < 8; ++w) t += red[w][c];
         const int64_t col = (int64_t)blockIdx.x * 32 * V + c;
-        if (col < N) partial[(int64_t)blockIdx.y * N + col] = t;
+        if (col >= N) continue;
+        if (db) db[col] = (T)t;                                             // one slice: nothing to add up
+        else partial[(int64_t)blockIdx.y * N + col] = t;
     }
 }
 
@@ -815,15 +897,46 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide, bool pac
 }
 
 template <typename T>
-int join(const Plan& p, const Epilogue& ep, hipStream_t st) {
-    const int64_t quads = (int64_t)p.s.M * ((p.s.N + 3) / 4), blocks = (quads + 255) / 256;
-    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, p.s, ep);
+int join(const Shape& s, const Epilogue& ep, hipStream_t st) {
+    const int64_t quads = (int64_t)s.M * ((s.N + 3) / 4), blocks = (quads + 255) / 256;
+    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, s, ep);
     return launch_status();
 }
 
 // whether an operand (rows of `pitch` elements) suits the large forms
 bool suits(int32_t dtype, int kind, const void* p, int64_t pitch) {
     return dtype == URSA_F32 ? pitch <= kSplitMaxPitch && (kind != kFlat || pitch % 8 == 0) : pitch % 8 == 0 && pitch <= kWideMaxPitch && ((uintptr_t)p & 15) == 0;
+}
+
+// Few rows: 16, 32 or 64 of them. Four waves a workgroup of 16 features where those give two workgroups a CU, up to sixteen where
+// there are fewer, and the contraction cut (at least 2,048 k a slice) where sixteen waves do not fill the CUs either.
+int rows_form(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 4 : 0; }
+
+Shape rows_shape(int64_t M, int64_t N, int64_t K) {
+    Shape s = {};
+    s.M = (int)M, s.N = (int)N, s.K = (int)K;
+    const int64_t groups = (N + 15) / 16;
+    int64_t cut = groups < 128 ? 256 / groups : 1;
+    if (cut > K / 2048) cut = K / 2048;
+    if (cut > 16) cut = 16;
+    if (cut < 1) cut = 1;
+    s.k_slice = (int)(((K + cut - 1) / cut + 31) / 32 * 32);
+    if (s.k_slice < 32) s.k_slice = 32;
+    s.slices = (int)((K + s.k_slice - 1) / s.k_slice);
+    if (s.slices < 1) s.slices = 1;
+    return s;
+}
+
+template <typename T, int MT>
+int rows_product(const Operand& x, const Operand& y, const Shape& s, Epilogue ep, hipStream_t st) {
+    if (s.slices == 1) ep.partial = nullptr;
+    const unsigned groups = (unsigned)((s.N + 15) / 16);
+    const dim3 grid(groups, (unsigned)s.slices);
+    if (groups >= 512) hipLaunchKernelGGL((k_rows<T, MT, 4>), grid, dim3(256), 0, st, x, y, s, ep);
+    else if (groups >= 128) hipLaunchKernelGGL((k_rows<T, MT, 8>), grid, dim3(512), 0, st, x, y, s, ep);
+    else hipLaunchKernelGGL((k_rows<T, MT, 16>), grid, dim3(1024), 0, st, x, y, s, ep);
+    const int rc = launch_status();
+    return rc || s.slices == 1 ? rc : join<T>(s, ep, st);
 }
 
 template <typename T, int XK, int YK>
@@ -840,7 +953,7 @@ int product(const Operand& x, const Operand& y, const Plan& p, Epilogue ep, hipS
         hipLaunchKernelGGL((k_product<T, XK, YK, 64>), grid, dim3(256), 0, st, x, y, p.s, ep);
     }
     const int rc = launch_status();
-    return rc || p.s.slices == 1 ? rc : join<T>(p, ep, st);
+    return rc || p.s.slices == 1 ? rc : join<T>(p.s, ep, st);
 }
 
 #define URSA_LINEAR_TYPES(dtype, call) (dtype == URSA_F32 ? call(float) : dtype == URSA_BF16 ? call(bf16) : call(f16))
@@ -856,14 +969,13 @@ int check(int64_t M, int64_t N, int64_t K, int32_t dtype) {
 
 bool misaligned(int32_t dtype, uintptr_t pointers) { return pointers & (uintptr_t)(element_size(dtype) - 1); }
 
-int act_rows(int64_t M, int64_t N, int32_t dtype) {       // rows of a slice of k_act_grad: about 2,048 workgroups, 8 rows at least
+int act_rows(int64_t M, int64_t N, int32_t dtype) {       // rows of a slice of k_act_grad: about 2,048 workgroups, 32 rows at least
     const int64_t cols = (N + 32 * 16 / element_size(dtype) - 1) / (32 * 16 / element_size(dtype));
     int64_t slices = 2048 / (cols ? cols : 1);
     if (slices < 1) slices = 1;
     if (slices > 256) slices = 256;
-    int64_t rows = (M + slices - 1) / slices;
-    rows = (rows + 7) / 8 * 8;
-    return (int)(rows < 8 ? 8 : rows);
+    const int64_t rows = ((M + slices - 1) / slices + 7) / 8 * 8;
+    return (int)(M <= 256 ? 256 : rows < 32 ? 32 : rows);         // few rows: one slice, which spares the second launch
 }
 
 template <typename T>
@@ -876,10 +988,10 @@ int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T*
         const int rows = act_rows(M, N, dtype), slices = (int)((M + rows - 1) / rows), per = 32 * Piece<T>::kN;
         if (M) {
             hipLaunchKernelGGL(k_act_grad<T>, dim3((unsigned)((N + per - 1) / per), (unsigned)slices), dim3(256), 0, st, dy, act ? z : nullptr, dz,
-                               db ? scratch : nullptr, M, (int)N, act, rows);
+                               db && slices > 1 ? scratch : nullptr, slices == 1 ? db : nullptr, M, (int)N, act, rows);
             if ((rc = launch_status())) return rc;
         }
-        if (db) {
+        if (db && slices != 1) {
             hipLaunchKernelGGL(k_columns_join<T>, dim3((unsigned)((N + 31) / 32)), dim3(256), 0, st, (const float*)scratch, slices, (int)N, db);
             if ((rc = launch_status())) return rc;
         }
@@ -917,7 +1029,10 @@ struct BwdScratch {
 }  // namespace
 
 extern "C" int64_t ursa_linear_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-    return check(M, N, K, dtype) ? 0 : most_ws(M, N, K, dtype);
+    if (check(M, N, K, dtype)) return 0;
+    if (!rows_form(M)) return most_ws(M, N, K, dtype);
+    const Shape s = rows_shape(M, N, K);
+    return s.slices > 1 ? (int64_t)s.slices * M * N * 4 : 0;
 }
 
 extern "C" int64_t ursa_linear_bwd_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t act, int32_t dx, int32_t dw, int32_t db) {
@@ -931,10 +1046,18 @@ extern "C" int ursa_linear_act(const void* x, const void* w, const void* bias, c
     if (act < URSA_ACT_NONE || act > URSA_ACT_SILU) return URSA_EFLAGS;
     if (int rc = check(M, N, K, dtype)) return rc > 0 ? URSA_OK : rc;
     const Plan p = plan_of(M, N, K, dtype, suits(dtype, kFlat, x, K) && suits(dtype, kFlat, w, K), false);
-    if ((K && (!x || !w)) || !y || (p.ws() && !ws)) return URSA_ENULL;
+    const int form = rows_form(M);
+    const Shape few = rows_shape(M, N, K);
+    if ((K && (!x || !w)) || !y || ((form ? few.slices > 1 : p.s.slices > 1) && !ws)) return URSA_ENULL;
     if (misaligned(dtype, (uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)z) || (uintptr_t)ws & 3) return URSA_EALIGN;
     const Operand X{x, nullptr, K, (int)M}, Y{w, nullptr, K, (int)N};
     const Epilogue ep{y, z, bias, residual, (float*)ws, act};
+    if (form) {
+#define URSA_CALL(T) (form == 1 ? rows_product<T, 1>(X, Y, few, ep, (hipStream_t)stream) : form == 2 ? rows_product<T, 2>(X, Y, few, ep, (hipStream_t)stream) \
+                                                                                         : rows_product<T, 4>(X, Y, few, ep, (hipStream_t)stream))
+        return URSA_LINEAR_TYPES(dtype, URSA_CALL);
+#undef URSA_CALL
+    }
 #define URSA_CALL(T) product<T, kFlat, kFlat>(X, Y, p, ep, (hipStream_t)stream)
     return URSA_LINEAR_TYPES(dtype, URSA_CALL);
 #undef URSA_CALL

@@ -79,13 +79,13 @@ class _LinearAct(torch.autograd.Function):
 
 
 def _fusable(fc, w, b, x, residual):
-    t, dev = x.dtype, x.device
-    return (_on and dev.type == 'cuda' and t in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
+    t, dev = x.dtype, x.get_device()
+    return (_on and x.is_cuda and t in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
             and type(fc).forward is nn.Linear.forward
             and not (fc._forward_hooks or fc._forward_pre_hooks or fc._backward_hooks or fc._backward_pre_hooks)
-            and w.dtype == t and w.device == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
-            and (b is None or (b.dtype == t and b.device == dev))
-            and (residual is None or (residual.dtype == t and residual.device == dev)))
+            and w.dtype is t and w.get_device() == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
+            and (b is None or (b.dtype is t and b.get_device() == dev))
+            and (residual is None or (residual.dtype is t and residual.get_device() == dev)))
 
 
 def linear_act(fc, x, activation=None, residual=None, *, save8=False):
@@ -95,7 +95,9 @@ def linear_act(fc, x, activation=None, residual=None, *, save8=False):
         raise ValueError(f'activation must be one of {list(_STOCK)}, got {activation!r}')
     if not isinstance(fc, nn.Linear):
         raise TypeError(f'linear_act wants an nn.Linear, got {type(fc).__name__}')
-    w, b = fc.weight, fc.bias
+    own = fc._parameters                                  # (a parametrised weight is a property instead)
+    w = own['weight'] if 'weight' in own else fc.weight
+    b = own['bias'] if 'bias' in own else fc.bias
     shape = x.shape[:-1] + (w.shape[0],)
     if residual is not None and residual.shape != shape:
         raise ValueError(f'residual {tuple(residual.shape)} should have the result\'s shape {tuple(shape)}')

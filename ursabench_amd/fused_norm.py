@@ -39,9 +39,9 @@ def enabled(flag=None):
 
 
 def _gradients(ctx, dy, dz, need_x, need_w, need_b):
-    z, q, e, mean, rstd, w = ctx.saved_tensors
+    z, q, e, stats, w = ctx.saved_tensors
     return _native.default_kernels().layer_norm_backward(
-        dy.contiguous(), mean, rstd, w, x=z, q=q, e=e, dz=None if dz is None else dz.contiguous(), need_dx=need_x,
+        dy.contiguous(), stats, w, x=z, q=q, e=e, dz=None if dz is None else dz.contiguous(), need_dx=need_x,
         param_type=ctx.param_type, need_dgamma=need_w, need_dbeta=need_b)
 
 
@@ -50,8 +50,8 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, eps, save8):
-        z, y, mean, rstd, q, e = _native.default_kernels().layer_norm(x, w, b, eps=eps, stats=True, save8=save8)
-        ctx.save_for_backward(None if save8 else z, q, e, mean, rstd, w)
+        z, y, ms, q, e = _native.default_kernels().layer_norm(x, w, b, eps=eps, stats=True, save8=save8)
+        ctx.save_for_backward(None if save8 else z, q, e, ms, w)
         ctx.param_type = None if b is None else b.dtype
         return y
 
@@ -67,8 +67,8 @@ class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, w, bias, eps, save8):
         ctx.set_materialize_grads(False)                 # an unused output's gradient arrives as None, not as zeros
-        z, y, mean, rstd, q, e = _native.default_kernels().layer_norm(a, w, bias, eps=eps, addend=b, stats=True, save8=save8)
-        ctx.save_for_backward(None if save8 else z, q, e, mean, rstd, w)
+        z, y, ms, q, e = _native.default_kernels().layer_norm(a, w, bias, eps=eps, addend=b, stats=True, save8=save8)
+        ctx.save_for_backward(None if save8 else z, q, e, ms, w)
         ctx.param_type = None if bias is None else bias.dtype
         return z, y
 
@@ -83,13 +83,13 @@ class _AddNorm(torch.autograd.Function):
 
 
 def _fusable(ln, w, b, x):
-    t, dev, shape = x.dtype, x.device, ln.normalized_shape
-    return (_on and dev.type == 'cuda' and t in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
+    t, dev, shape = x.dtype, x.get_device(), ln.normalized_shape
+    return (_on and x.is_cuda and t in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
             and type(ln).forward is nn.LayerNorm.forward
             and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks or ln._backward_pre_hooks)
-            and x.dim() >= len(shape) and tuple(x.shape[x.dim() - len(shape):]) == tuple(shape) and ln.eps >= 0
-            and (w is None or (w.device == dev and (w.dtype == t or w.dtype == torch.float32)))
-            and (b is None or (b.device == dev and (b.dtype == t or b.dtype == torch.float32) and (w is None or w.dtype == b.dtype))))
+            and x.shape[-len(shape):] == shape and ln.eps >= 0
+            and (w is None or (w.get_device() == dev and (w.dtype is t or w.dtype is torch.float32)))
+            and (b is None or (b.get_device() == dev and (b.dtype is t or b.dtype is torch.float32) and (w is None or w.dtype is b.dtype))))
 
 
 def _rows(n, x):
@@ -103,15 +103,21 @@ def _flat(p):
     return p if p is None or (p.dim() == 1 and p.is_contiguous()) else p.reshape(-1).contiguous()
 
 
-def _recorded(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _params(ln):
+    own = ln._parameters                                  # (a parametrised weight is a property instead)
+    return own['weight'] if 'weight' in own else ln.weight, own['bias'] if 'bias' in own else ln.bias
+
+
+def _recorded(x, w, b, addend=None):
+    return torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad) or (b is not None and b.requires_grad)
+                                        or (addend is not None and addend.requires_grad))
 
 
 def layer_norm(ln, x, *, save8=False):
     """ln(x). save8: keep x in 8 bits for the backward pass (module docstring)."""
     if not isinstance(ln, nn.LayerNorm):
         raise TypeError(f'layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
-    w, b = ln.weight, ln.bias
+    w, b = _params(ln)
     if not _fusable(ln, w, b, x):
         return ln(x)
     n = len(ln.normalized_shape)
@@ -132,14 +138,14 @@ def add_layer_norm(ln, x, *, save8=False):
     if not isinstance(ln, nn.LayerNorm):
         raise TypeError(f'add_layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
     a, b = x
-    w, bias = ln.weight, ln.bias
-    if not (_fusable(ln, w, bias, a) and b.shape == a.shape and b.dtype == a.dtype and b.device == a.device):
+    w, bias = _params(ln)
+    if not (_fusable(ln, w, bias, a) and b.shape == a.shape and b.dtype is a.dtype and b.device == a.device):
         z = a + b
         return z, layer_norm(ln, z, save8=save8)
     n = len(ln.normalized_shape)
     flat = n == 1 and a.dim() == 2
     a2, b2, w, bias = _rows(n, a), _rows(n, b), _flat(w), _flat(bias)
-    if _recorded(a, b, w, bias):
+    if _recorded(a, w, bias, b):
         z, y = _AddNorm.apply(a2, b2, w, bias, ln.eps, save8)
     else:
         z, y = _native.default_kernels().layer_norm(a2, w, bias, eps=ln.eps, addend=b2)[:2]
