@@ -238,6 +238,31 @@ def test_large_and_small_magnitudes_fp32():
     assert ((got - want).abs() <= 1e-6 * want).all()
 
 
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes of y, z and dy (and 2^31 elements): the last rows and features, and the column sums over all rows."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    M, K, N = 70000, 8, 32768
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    w = torch.randn(N, K, generator=g, device=DEV).bfloat16()
+    y, z = k.linear_act(x, w, activation='silu', save_z=True)
+    assert y.numel() > 2 ** 31
+    tail = slice(M - 300, M)
+    B.check(dict(y=y[tail]), *B.linear(x[tail], w, None, None, 'silu'))
+    del z
+    dx, dw, db = k.linear_backward(y, x, w)
+    yt = y[tail].double()
+    want = yt @ w.double()
+    bound = B.product_error(yt.abs() @ w.double().abs(), N, torch.bfloat16) + B.last_rounding(want, torch.bfloat16)
+    assert ((dx[tail].double() - want).abs() <= bound).all()
+    cols = slice(N - 64, N)
+    yc = y[:, cols].double()
+    want, s = yc.t() @ x.double(), yc.abs().t() @ x.double().abs()
+    assert ((dw[cols].double() - want).abs() <= B.product_error(s, M, torch.bfloat16) + B.last_rounding(want, torch.bfloat16)).all()
+    assert ((db[cols].double() - yc.sum(0)).abs() <= (M + 16) * B.F * yc.abs().sum(0) + B.last_rounding(yc.sum(0), torch.bfloat16)).all()
+
+
 def test_the_same_call_gives_the_same_bits():
     for M, K, N, dtype in ((300, 4096, 300, 'bfloat16'), (300, 1000, 200, 'float32')):
         x, w, b, r, dy = _case(M, K, N, dtype, residual=True)

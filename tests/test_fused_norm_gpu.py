@@ -190,6 +190,28 @@ def test_infinities_and_nans_stay_in_their_rows(dtype):
         assert torch.equal(y[keep], clean[keep]) and not torch.isfinite(y[7]).any()
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows have the bits that they have in a small call of the same width."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    M, D = 530000, 4096
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(1000, D, generator=g, device=DEV).bfloat16().repeat(M // 1000, 1)
+    assert x.numel() > 2 ** 31
+    w = torch.randn(D, generator=g, device=DEV).bfloat16()
+    z, y, ms, q, e = k.layer_norm(x, w, eps=1e-5, stats=True, save8=True)
+    _, y0, ms0, q0, e0 = k.layer_norm(x[:1000], w, eps=1e-5, stats=True, save8=True)
+    for big, small in ((y, y0), (q, q0), (e, e0)):
+        assert torch.equal(big[-1000:], small)
+    assert torch.equal(ms[:, -1000:], ms0)
+    for kept, kept0 in ((dict(x=x), dict(x=x[:1000])), (dict(q=q, e=e), dict(q=q0, e=e0))):
+        dx = k.layer_norm_backward(y, ms, w, **kept)[0]
+        assert torch.equal(dx[-1000:], k.layer_norm_backward(y0, ms0, w, **kept0)[0])
+    assert torch.equal(k.act8_unpack(q, e, D, torch.bfloat16)[-1000:], k.act8_unpack(q0, e0, D, torch.bfloat16))
+    qp, ep = k.act8_pack(x)
+    assert torch.equal(qp, q) and torch.equal(ep, e)
+
+
 def test_the_same_call_gives_the_same_bits():
     for M, D, dtype in ((5000, 300, 'float32'), (3000, 4096, 'bfloat16')):
         x, r, w, b, dy, dz = _case(M, D, dtype)

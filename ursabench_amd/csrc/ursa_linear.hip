@@ -344,9 +344,10 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes from each lane's `offset` in the buffer to LDS at `dst` + 16 lane (dst the same in the whole wave). Not the compiler's
 // builtin: that one makes it wait for every such load before the next LDS read of any address. Whoever reads the LDS waits
-// (vmcnt(0), then a barrier). m0 has no other use here; one wait state between its write and its use.
+// (vmcnt(0), then a barrier). m0 has no other use here. The compiler does not look into the block for hazards: the wait states
+// cover a scalar register that a vector instruction wrote just before (five) and m0 (one).
 __device__ __forceinline__ void memory_to_lds(i32x4 buffer, uint32_t offset, const short* dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  ::"s"((uint32_t)(uintptr_t)(lptr)dst), "v"(offset), "s"(buffer) : "memory");
 }
 

@@ -191,10 +191,23 @@ template <typename T, typename P, int TPR, int CV, bool PACKED, bool DZ>
 __global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) {
     constexpr int V = Piece<T>::kN, C = CV / V, R = bwd_threads(TPR) / TPR;
     constexpr int kJoin = R > 1 ? R * TPR * CV : 32;
+    constexpr bool kEarly = DZ && CV == 8;                       // dz with the rest of a row: 16 columns leave no registers for it
     __shared__ float red[kJoin];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const int64_t qpitch = (a.D + kBlock8 - 1) / kBlock8 * kBlock8, stride = (int64_t)gridDim.x * R;
-    float dg[C][V] = {}, db[C][V] = {};
+    float dg[C][V] = {}, db[C][V] = {}, g[C][V];
+    const auto load_gamma = [&](int c) {
+        const int d = (c * TPR + t) * V;
+        if (a.gamma) {
+            load_piece<P, V>(a.gamma + d, (int)a.D - d, g[c]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) g[c][i] = 1.f;
+        }
+    };
+    if constexpr (CV == 8)
+#pragma unroll
+        for (int c = 0; c < C; ++c) load_gamma(c);
     Raw<T, C> rx, rd, rz;
     Raw8<V, C> rq;
     float mean = 0.f, rstd = 0.f;
@@ -202,7 +215,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) 
         if constexpr (PACKED) rq.template load<TPR>(a.q + row * qpitch, a.e + row * (qpitch / kBlock8), t, qpitch);
         else rx.template load<TPR>(a.x + row * a.D, t, a.D);
         rd.template load<TPR>(a.dy + row * a.D, t, a.D);
-        if constexpr (DZ) rz.template load<TPR>(a.dz + row * a.D, t, a.D);
+        if constexpr (kEarly) rz.template load<TPR>(a.dz + row * a.D, t, a.D);
         mean = a.mean[row], rstd = a.rstd[row];
     };
     for (int64_t row = (int64_t)blockIdx.x * R + sub; row < a.M; row += stride) {
@@ -213,20 +226,19 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) 
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int64_t d = (int64_t)(c * TPR + t) * V, left = a.D - d;
-            float g[V];
-            if (a.gamma) load_piece<P, V>(a.gamma + d, left, g);
+            const int left = (int)a.D - (c * TPR + t) * V;
+            if constexpr (CV != 8) load_gamma(c);                // 16 columns: once for every row, for want of registers
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float x;
                 if constexpr (PACKED) x = value8(rq.v[c][i], rq.e[c]);
                 else x = (float)rx.v[c][i];
-                if constexpr (DZ) z[c][i] = (float)rz.v[c][i];
+                if constexpr (kEarly) z[c][i] = (float)rz.v[c][i];
                 tt[c][i] = (float)rd.v[c][i];
                 xh[c][i] = (x - mean) * rs;                      // behind the row's end dy is 0, so these never count
                 dg[c][i] += i < left ? tt[c][i] * xh[c][i] : 0.f;
                 db[c][i] += tt[c][i];
-                if (a.gamma) tt[c][i] *= g[i];
+                tt[c][i] *= g[c][i];
                 s1 += tt[c][i];
                 s2 += i < left ? tt[c][i] * xh[c][i] : 0.f;
             }
@@ -236,6 +248,8 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) 
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int64_t d = (int64_t)(c * TPR + t) * V, left = a.D - d;
+            if constexpr (CV != 8) asm volatile("" ::: "memory");
+            if constexpr (DZ && !kEarly) load_piece<T, V>(a.dz + base + d, left, z[c]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 tt[c][i] = rs * (tt[c][i] - m1 - xh[c][i] * m2);
@@ -427,7 +441,7 @@ constexpr int64_t kLong = 16384;         // features that the register forms hol
 int rows_per_group(int64_t D) { return D <= 128 ? 16 : D <= 2048 ? 4 : 1; }
 
 // Threads of a row in the backward's walk: 8 columns each, so that their sums leave registers for many waves (with 16 or 32 a CU holds
-// few, and 16,384 x 4,096 bf16 took 197 us instead of @@). Above 8,192: 16 columns.
+// few, and 16,384 x 4,096 bf16 with a gradient past the norm took 197 us instead of 125). Above 8,192: 16 columns.
 int bwd_row_threads(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 
 // Workgroups of the walk: 1,024 threads a CU, and no more than leave each row slot four rows, so that the partial sums (2 D floats
