@@ -866,31 +866,38 @@ struct Plan {
     int64_t ws() const { return s.slices > 1 ? (int64_t)s.slices * s.M * s.N * 4 : 0; }
 };
 
-// The form by the number of workgroups that it gives the 256 CUs, and the cut of the contraction where there are fewer than one (two
-// of the smaller forms) for each: at most 16 slices of at least eight k steps. `wide`: the operands suit the large forms (see there);
-// `packed`: one of them comes in 8 bits.
+// The form, by the number of workgroups that it gives the 256 CUs, and the cut of the contraction where there are fewer than one
+// (two of the smaller forms) for each: at most 16 slices of at least eight k steps. `wide`: the operands suit the large forms (see
+// there); `packed`: one of them comes in 8 bits. Measured, both sides of each border:
+//   16 bits, 256 x 256 from 192 tiles on: 8192 x 1024 outputs, K 4096 (128 tiles): 64 us in 128 x 128, 79 cut in two;
+//            8192 x 8192, K 2048: 219 against 267. With an operand in 8 bits, whose conversion the larger tile halves, also cut:
+//            1024 x 4096, K 8192: 97 against 118
+//   16 bits, 128 x 128 where they reach 256 workgroups, cut in four at most: 2048^3: 28 us against 37 in 64 x 64; 1024^3 (too few):
+//            16.8 against 14.6. Two workgroups a CU where each has 48 steps left: 1024 x 4096, K 8192: 79 us against 92
+//   fp32, 256 x 128 where they reach 192 workgroups, cut or not: 4096 x 1024 outputs, K 1024: 67 us both ways; 1024 x 1024, K 4096: 67
+//            against 93; 1024^3 (128 workgroups at most): 34 against 29 in 64 x 64
 Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide, bool packed) {
     Plan p;
     const int bk = dtype == URSA_F32 ? 32 : 64;
-    const int64_t steps = (K + bk - 1) / bk, most = steps / 8 < 16 ? steps / 8 : 16;
+    const int64_t steps = (K + bk - 1) / bk, most = steps / 8 < 1 ? 1 : steps / 8 < 16 ? steps / 8 : 16;
     const auto tiles_of = [&](int tm, int tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
     const int64_t big = tiles_of(128, 128);
     p.tm = p.tn = big >= 256 ? 128 : 64;
     p.wide = false;
     if (wide && dtype == URSA_F32) {
         const int64_t n = tiles_of(kSplitM, kSplitN);
-        if (n >= 192 || (n >= 96 && n * most >= 192)) p.tm = kSplitM, p.tn = kSplitN, p.wide = true;
+        if (n * most >= 192) p.tm = kSplitM, p.tn = kSplitN, p.wide = true;
     } else if (wide) {
         const int64_t n = tiles_of(256, 256);
         if (n >= 192 || (packed && n * most >= 192)) p.tm = p.tn = 256;
+        else if (big * (most < 4 ? most : 4) >= 256) p.tm = p.tn = 128;
         p.wide = p.tm >= 128;
     }
     p.s.M = (int)M, p.s.N = (int)N, p.s.K = (int)K;
     p.s.tiles_m = (int)((M + p.tm - 1) / p.tm), p.s.tiles_n = (int)((N + p.tn - 1) / p.tn);
-    const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, want = p.tm == 256 ? 256 : 512;
+    const int64_t tiles = (int64_t)p.s.tiles_m * p.s.tiles_n, want = p.wide && (p.tm == 256 || tiles < 256 || steps < 96) ? 256 : 512;
     int64_t cut = tiles < want && tiles ? want / tiles : 1;
     if (cut > most) cut = most;
-    if (cut < 1) cut = 1;
     const int64_t per = (steps + cut - 1) / cut;
     p.s.k_slice = (int)((per > 0 ? per : 1) * bk);
     p.s.slices = per > 0 ? (int)((steps + per - 1) / per) : 1;
