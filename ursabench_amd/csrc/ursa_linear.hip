@@ -874,8 +874,8 @@ struct Plan {
 //            1024 x 4096, K 8192: 97 against 118
 //   16 bits, 128 x 128 where they reach 256 workgroups, cut in four at most: 2048^3: 28 us against 37 in 64 x 64; 1024^3 (too few):
 //            16.8 against 14.6. Two workgroups a CU where each has 48 steps left: 1024 x 4096, K 8192: 79 us against 92
-//   fp32, 256 x 128 where they reach 192 workgroups, cut or not: 4096 x 1024 outputs, K 1024: 67 us both ways; 1024 x 1024, K 4096: 67
-//            against 93; 1024^3 (128 workgroups at most): 34 against 29 in 64 x 64
+//   fp32, 256 x 128 where they reach 192 workgroups, cut from 96 tiles or K 2048 on: 1024 x 1024 outputs, K 4096: 64 us against 93;
+//            4096 x 1024, K 1024: 62 against 66; 2048 x 1024, K 1024 (64 tiles): 44 against 40 in 64 x 64; 1024^3: 34 against 29
 Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide, bool packed) {
     Plan p;
     const int bk = dtype == URSA_F32 ? 32 : 64;
@@ -886,7 +886,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide, bool pac
     p.wide = false;
     if (wide && dtype == URSA_F32) {
         const int64_t n = tiles_of(kSplitM, kSplitN);
-        if (n * most >= 192) p.tm = kSplitM, p.tn = kSplitN, p.wide = true;
+        if (n >= 192 || (n * most >= 192 && (n >= 96 || steps >= 64))) p.tm = kSplitM, p.tn = kSplitN, p.wide = true;
     } else if (wide) {
         const int64_t n = tiles_of(256, 256);
         if (n >= 192 || (packed && n * most >= 192)) p.tm = p.tn = 256;
