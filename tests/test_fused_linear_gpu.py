@@ -185,6 +185,45 @@ def test_only_the_gradients_that_are_wanted(frozen):
         assert torch.equal(t, full[k]), k
 
 
+def test_differentiable_once_and_no_changes_in_place():
+    """create_graph gives the same gradients, differentiating them raises; so does a backward pass over an operand that changed."""
+    from ursabench_amd.fused_linear import linear_act
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    fc, ln = nn.Linear(40, 40, device=DEV), nn.LayerNorm(40, device=DEV)
+    x = torch.randn(3, 9, 40, device=DEV, requires_grad=True)
+    for f in (lambda: linear_act(fc, x, 'gelu', x), lambda: layer_norm(ln, x), lambda: sum(add_layer_norm(ln, (x, 2 * x)))):
+        want = torch.autograd.grad(f().square().sum(), x)[0]
+        g = torch.autograd.grad(f().square().sum(), x, create_graph=True)[0]
+        assert torch.equal(g, want)
+        with pytest.raises(RuntimeError, match='double backward'):
+            torch.autograd.grad(g.sum(), x)
+    y = linear_act(fc, x, 'gelu')
+    with torch.no_grad():
+        fc.weight.mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace'):
+        y.sum().backward()
+    z, y = add_layer_norm(ln, (x, 2 * x))
+    z.mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace'):
+        y.sum().backward()
+
+
+def test_nothing_is_kept_behind_a_dropped_graph():
+    from ursabench_amd.fused_linear import linear_act
+    from ursabench_amd.fused_norm import add_layer_norm
+    fc, ln = nn.Linear(512, 512, device=DEV), nn.LayerNorm(512, device=DEV)
+    x = torch.randn(4, 256, 512, device=DEV, requires_grad=True)
+    held = []
+    for _ in range(4):
+        for save8 in (False, True):
+            z, y = add_layer_norm(ln, (x, x), save8=save8)
+            linear_act(fc, y, 'gelu', z, save8=save8).sum().backward()
+            del z, y
+        torch.cuda.synchronize()
+        held.append(torch.cuda.memory_allocated())
+    assert held[-1] == held[0], held
+
+
 def test_empty_batches():
     from ursabench_amd.fused_linear import linear_act
     for t in B.TYPES.values():

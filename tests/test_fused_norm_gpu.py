@@ -119,7 +119,7 @@ def test_gradients_against_differences():
     side, err = [], 0.0
     for s in (h, -h):
         moved = x + s * v
-        side.append(float((_run(moved, w, b, c)[1]['y'].double().cpu() * c.double()).sum()))
+        side.append(float((_run(moved, w, b, c)[1]['y'].detach().double().cpu() * c.double()).sum()))
         values, bounds = B.norm(moved, w, b, 1e-5)
         err += float((bounds['y'] * c.double().abs()).sum())
         # the rounding of the moved input: 2^-24 |x| an element, through a map whose slope is at most 2 rstd |g| in the largest norm

@@ -1,4 +1,4 @@
-"""ctypes binding of the gfx950 kernel library (include/ursa_hip.h).
+"""ctypes binding of the gfx950 kernel library (include/ursa_hip.h), and the loader of the autograd nodes that call it from C++.
 
 This is the only way the package computes an MCMC update or a BMA reduction. There is no CPU
 or eager-PyTorch fallback: if ``csrc/libursa_hip.so`` is missing, or a tensor is not a
@@ -10,6 +10,7 @@ loader resolve our NEEDED entry to the runtime torch already initialised, so the
 handles torch hands us are valid in the runtime our launches go through.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -17,6 +18,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libursa_hip.so')
 KNOBS_LIB_PATH = os.path.join(_HERE, 'csrc', 'libursa_hip_knobs.so')   # -DURSA_DEBUG_KNOBS build: tests / tools only
+NODES_PATH = os.path.join(_HERE, 'csrc', '_ursa_torch.so')                 # autograd nodes of K15 / K16
 
 ABI_VERSION = 9
 
@@ -1116,6 +1118,26 @@ class HipKernels:
         x = q.new_empty((M, D), dtype=dtype)
         self._launch(self.lib.ursa_act8_unpack, q, pq, pe, x.data_ptr(), M, D, DTYPES[dtype])
         return x
+
+
+_nodes = None
+
+
+def nodes():
+    """The autograd nodes of K15 / K16 (csrc/ursa_torch.cpp): raises NativeLibraryMissing if they are not built."""
+    global _nodes
+    if _nodes is None:
+        load_library()
+        if not os.path.exists(NODES_PATH):
+            raise NativeLibraryMissing(f'{NODES_PATH} not found: the autograd nodes are not built. Run '
+                                       f'`python -c "import __graft_entry__ as g; g.build()"`. ursabench_amd has no fallback for them.')
+        spec = importlib.util.spec_from_file_location('_ursa_torch', NODES_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        if mod.abi_version != ABI_VERSION:
+            raise NativeLibraryMissing(f'{NODES_PATH}: ABI version {mod.abi_version}, binding expects {ABI_VERSION}; rebuild it')
+        _nodes = mod
+    return _nodes
 
 
 def knobs_kernels():

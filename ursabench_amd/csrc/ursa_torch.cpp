@@ -1,0 +1,278 @@
+// ursa_torch.cpp — K15 / K16 (include/ursa_hip.h) as autograd nodes. The backward pass of a node runs on autograd's device thread:
+// written in Python it has to wait there for the interpreter, which costs more than the launches of a small layer (mnist's first
+// layer, forward + backward: 138 us with Python nodes, @@ with these). What may be called and with what is checked by the Python callers
+// (fused_linear, fused_norm); this file allocates, launches on the current stream of the tensors' device and keeps what the
+// backward pass needs.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "../../include/ursa_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Maybe;
+
+int32_t type_of(const Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return URSA_F32;
+        case at::kBFloat16: return URSA_BF16;
+        case at::kHalf: return URSA_F16;
+        default: TORCH_CHECK_TYPE(false, "float32, bfloat16 or float16 wanted, got ", t.scalar_type());
+    }
+}
+
+void ok(int rc, const char* what) {
+    if (rc < 0) TORCH_CHECK_VALUE(false, what, ": ", ursa_strerror(rc), " (ursa error ", rc, ")");
+    TORCH_CHECK(rc == 0, what, ": HIP error ", rc, ": ", ursa_strerror(rc));
+}
+
+ursa_stream_t stream_of(const Tensor& t) { return (ursa_stream_t)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+void* at_(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+Tensor bytes(const Tensor& like, int64_t n) { return n ? at::empty({n}, like.options().dtype(at::kByte)) : Tensor(); }
+
+Tensor given(const Maybe& t) { return t.has_value() && t->defined() ? *t : Tensor(); }
+
+Tensor packed(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// x as rows of `width`
+Tensor rows_of(const Tensor& x, int64_t width) { return (x.dim() == 2 && x.size(1) == width ? x : x.reshape({width ? x.numel() / width : 0, width})).contiguous(); }
+
+struct Packed8 { Tensor q, e; };
+
+Packed8 pack8(const Tensor& x2) {
+    const int64_t blocks = (x2.size(1) + 31) / 32;
+    Packed8 p{at::empty({x2.size(0), 32 * blocks}, x2.options().dtype(at::kChar)), at::empty({x2.size(0), blocks}, x2.options().dtype(at::kChar))};
+    return p;
+}
+
+// Gradients of a node that is differentiable once: further differentiation raises when it gets there.
+variable_list once(variable_list grads, bool tracked) {
+    if (!tracked) return grads;
+    size_t n = 0;
+    for (auto& g : grads) n += g.defined();
+    if (!n) return grads;
+    variable_list in;
+    for (auto& g : grads)
+        if (g.defined()) in.push_back(g.detach().requires_grad_());
+    const at::AutoGradMode record(true);
+    auto out = (*std::make_shared<torch::autograd::DelayedError>("ursabench_amd: double backward is not offered", (int)n))(std::move(in));
+    size_t k = 0;
+    for (auto& g : grads)
+        if (g.defined()) g = out[k++];
+    return grads;
+}
+
+bool tracked(const variable_list& grads) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (auto& g : grads)
+        if (wants(g)) return true;
+    return false;
+}
+
+// y (, z) = act(x w' + b) + r for 2-d contiguous operands
+Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act, at::IntArrayRef shape, Tensor* z) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), N = w.size(0), K = w.size(1);
+    const int32_t dt = type_of(x);
+    Tensor y = at::empty(shape, x.options());
+    if (z) *z = at::empty({M, N}, x.options());
+    const Tensor ws = bytes(x, ursa_linear_ws_bytes(M, N, K, dt));
+    ok(ursa_linear_act(at_(x), at_(w), at_(b), at_(r), at_(y), z ? at_(*z) : nullptr, at_(ws), M, N, K, dt, (int32_t)act, stream_of(x)), "ursa_linear_act");
+    return y;
+}
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b_, const Maybe& r_, int64_t act, bool save8) {
+        const Tensor b = given(b_), r = given(r_);
+        const bool nx = wants(x), nw = wants(w), nb = wants(b);
+        at::NoGradGuard no_grad;
+        const int64_t N = w.size(0), K = w.size(1);
+        const Tensor x2 = rows_of(x, K), wc = w.contiguous();
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.back() = N;
+        Tensor z;
+        const Tensor y = linear_forward(x2, wc, packed(b), r.defined() ? rows_of(r, N) : r, act, shape, act && (nx || nw || nb) ? &z : nullptr);
+        Packed8 p;
+        if (nw && save8) {
+            p = pack8(x2);
+            const c10::DeviceGuard guard(x.device());
+            ok(ursa_act8_pack(at_(x2), (int8_t*)at_(p.q), (int8_t*)at_(p.e), x2.size(0), K, type_of(x2), stream_of(x2)), "ursa_act8_pack");
+        }
+        ctx->save_for_backward({nw && !save8 ? x2 : Tensor(), nx ? wc : Tensor(), z, p.q, p.e});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["needs"] = (int64_t)(nx + 2 * nw + 4 * nb + 8 * wants(r));
+        ctx->saved_data["x"] = x.sizes().vec();
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const bool again = tracked(grads);
+        at::NoGradGuard no_grad;
+        const int64_t needs = ctx->saved_data["needs"].toInt(), act = ctx->saved_data["act"].toInt();
+        const bool nx = needs & 1, nw = needs & 2, nb = needs & 4;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &z = saved[2], &q = saved[3], &e = saved[4], &dy_ = grads[0];
+        variable_list out(6);
+        if (nx || nw || nb) {
+            const std::vector<int64_t> shape = ctx->saved_data["x"].toIntVector();
+            const int64_t K = shape.back(), N = dy_.size(-1);
+            const Tensor dy = rows_of(dy_, N);
+            const int64_t M = dy.size(0);
+            const c10::DeviceGuard guard(dy.device());
+            const int32_t dt = type_of(dy);
+            if (nx) out[0] = at::empty(shape, dy.options());
+            if (nw) out[1] = at::empty({N, K}, dy.options());
+            if (nb) out[2] = at::empty({N}, dy.options());
+            const Tensor ws = bytes(dy, ursa_linear_bwd_ws_bytes(M, N, K, dt, (int32_t)act, nx, nw, nb));
+            ok(ursa_linear_bwd(at_(dy), at_(x), (const int8_t*)at_(q), (const int8_t*)at_(e), at_(w), at_(z), at_(out[0]), at_(out[1]), at_(out[2]), at_(ws), M,
+                               N, K, dt, (int32_t)act, stream_of(dy)), "ursa_linear_bwd");
+        }
+        if (needs & 8) out[3] = dy_;
+        return once(std::move(out), again);
+    }
+};
+
+Tensor linear_act(const Tensor& x, const Tensor& w, const Maybe& b_, const Maybe& r_, int64_t act, bool save8) {
+    const Tensor b = given(b_), r = given(r_);
+    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) return LinearAct::apply(x, w, b_, r_, act, save8);
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = w.size(0);
+    return linear_forward(rows_of(x, w.size(1)), w.contiguous(), packed(b), r.defined() ? rows_of(r, w.size(0)) : r, act, shape, nullptr);
+}
+
+struct NormOut { Tensor z, y, stats, q, e; };
+
+// of 2-d contiguous x (and addend); z and y in `shape`
+NormOut norm_forward(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b, double eps, at::IntArrayRef shape, bool stats, bool save8) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), D = x.size(1);
+    NormOut o;
+    if (r.defined()) o.z = at::empty(shape, x.options());
+    o.y = at::empty(shape, x.options());
+    if (stats) o.stats = at::empty({2, M}, x.options().dtype(at::kFloat));
+    Packed8 p;
+    if (save8) p = pack8(x);
+    float* m = (float*)at_(o.stats);
+    ok(ursa_layer_norm_fwd(at_(x), at_(r), at_(o.z), at_(o.y), at_(w), at_(b), m, m ? m + M : nullptr, (int8_t*)at_(p.q), (int8_t*)at_(p.e), M, D, (float)eps,
+                           type_of(x), w.defined() ? type_of(w) : b.defined() ? type_of(b) : type_of(x), stream_of(x)), "ursa_layer_norm_fwd");
+    o.q = p.q, o.e = p.e;
+    return o;
+}
+
+// z: what was normalised, in any shape (of an output: that tensor itself, so that changes in place are noticed)
+void norm_keep(AutogradContext* ctx, const Tensor& z, const NormOut& o, const Tensor& w, const Tensor& b, const Tensor& x, int64_t width, int64_t needs, bool save8) {
+    ctx->save_for_backward({save8 ? Tensor() : z, o.q, o.e, o.stats, w});
+    ctx->saved_data["needs"] = needs;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["width"] = width;
+    ctx->saved_data["type"] = (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : z.scalar_type());
+}
+
+// dx in the input's shape, dgamma and dbeta [D]
+std::array<Tensor, 3> norm_backward(AutogradContext* ctx, const Tensor& dy_, const Tensor& dz_, bool nx, bool nw, bool nb) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t D = ctx->saved_data["width"].toInt();
+    const auto ptype = (at::ScalarType)ctx->saved_data["type"].toInt();
+    const Tensor dy = rows_of(dy_, D), dz = dz_.defined() ? rows_of(dz_, D) : dz_;
+    const int64_t M = dy.size(0);
+    const c10::DeviceGuard guard(dy.device());
+    std::array<Tensor, 3> out;
+    if (nx) out[0] = at::empty(ctx->saved_data["shape"].toIntVector(), dy.options());
+    if (nw) out[1] = at::empty({D}, dy.options().dtype(ptype));
+    if (nb) out[2] = at::empty({D}, dy.options().dtype(ptype));
+    const Tensor ws = nw || nb ? bytes(dy, 4 * ursa_layer_norm_ws_floats(M, D)) : Tensor();
+    const float* m = (const float*)at_(saved[3]);
+    ok(ursa_layer_norm_bwd(at_(saved[0]), (const int8_t*)at_(saved[1]), (const int8_t*)at_(saved[2]), at_(dy), at_(dz), at_(saved[4]), m, m + M, at_(out[0]),
+                           at_(out[1]), at_(out[2]), (float*)at_(ws), M, D, type_of(dy), ptype == at::kFloat ? URSA_F32 : ptype == at::kHalf ? URSA_F16 : URSA_BF16,
+                           stream_of(dy)), "ursa_layer_norm_bwd");
+    return out;
+}
+
+// w, b: [D] contiguous
+struct Norm : torch::autograd::Function<Norm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
+        const Tensor w = given(w_), b = given(b_);
+        const int64_t needs = wants(x) + 2 * wants(w) + 4 * wants(b);
+        at::NoGradGuard no_grad;
+        const Tensor x2 = rows_of(x, width);
+        const NormOut o = norm_forward(x2, Tensor(), w, b, eps, x.sizes(), true, save8);
+        norm_keep(ctx, x2, o, w, b, x, width, needs, save8);
+        return o.y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const bool again = tracked(grads);
+        at::NoGradGuard no_grad;
+        const int64_t needs = ctx->saved_data["needs"].toInt();
+        const auto g = norm_backward(ctx, grads[0], Tensor(), needs & 1, needs & 2, needs & 4);
+        return once({g[0], g[1], g[2], Tensor(), Tensor(), Tensor()}, again);
+    }
+};
+
+struct AddNorm : torch::autograd::Function<AddNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& a, const Tensor& r, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
+        const Tensor w = given(w_), b = given(b_);
+        const int64_t needs = wants(a) + 2 * wants(w) + 4 * wants(b) + 8 * wants(r);
+        at::NoGradGuard no_grad;
+        ctx->set_materialize_grads(false);                     // an unused output's gradient arrives undefined, not as zeros
+        const NormOut o = norm_forward(rows_of(a, width), rows_of(r, width), w, b, eps, a.sizes(), true, save8);
+        norm_keep(ctx, o.z, o, w, b, a, width, needs, save8);
+        return {o.z, o.y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const bool again = tracked(grads);
+        at::NoGradGuard no_grad;
+        const int64_t needs = ctx->saved_data["needs"].toInt();
+        const bool na = needs & 1, nr = needs & 8;
+        variable_list out(7);
+        const Tensor &dz = grads[0], &dy = grads[1];
+        if (!dy.defined()) {                                   // y unused: only the sum's own gradient flows
+            if (na) out[0] = dz;
+            if (nr) out[1] = dz;
+            return once(std::move(out), again);
+        }
+        const auto g = norm_backward(ctx, dy, dz, na || nr, needs & 2, needs & 4);
+        if (na) out[0] = g[0];
+        if (nr) out[1] = g[0];
+        out[2] = g[1], out[3] = g[2];
+        return once(std::move(out), again);
+    }
+};
+
+bool recorded(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b) {
+    return at::GradMode::is_enabled() && (wants(x) || wants(r) || wants(w) || wants(b));
+}
+
+Tensor layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, int64_t width, double eps, bool save8) {
+    if (recorded(x, Tensor(), given(w), given(b))) return Norm::apply(x, w, b, width, eps, save8);
+    return norm_forward(rows_of(x, width), Tensor(), given(w), given(b), eps, x.sizes(), false, false).y;
+}
+
+std::pair<Tensor, Tensor> add_layer_norm(const Tensor& a, const Tensor& r, const Maybe& w, const Maybe& b, int64_t width, double eps, bool save8) {
+    if (recorded(a, r, given(w), given(b))) {
+        auto out = AddNorm::apply(a, r, w, b, width, eps, save8);
+        return {out[0], out[1]};
+    }
+    const NormOut o = norm_forward(rows_of(a, width), rows_of(r, width), given(w), given(b), eps, a.sizes(), false, false);
+    return {o.z, o.y};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ursa_torch, m) {
+    namespace py = pybind11;
+    m.attr("abi_version") = URSA_ABI_VERSION;
+    m.def("linear_act", &linear_act, py::call_guard<py::gil_scoped_release>());
+    m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
+    m.def("add_layer_norm", &add_layer_norm, py::call_guard<py::gil_scoped_release>());
+}

@@ -9,8 +9,8 @@ launches differ:
 
 float32, bfloat16 and float16, any sizes and leading dimensions, on a HIP device. Operands that are not contiguous are copied first.
 Anything else - host tensors, other or mixed types, autocast, a subclass with a forward of its own, hooks on `fc` - takes
-`fc(x)`, the activation and the sum as stock ops, where `save8` keeps x itself. Double backward is not offered. On a HIP tensor the
-fused path needs csrc/libursa_hip.so (no silent fallback: a missing library raises).
+`fc(x)`, the activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises. On a HIP tensor
+the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the x that the weight gradient needs in 8 bits (K17, `act8`) instead of the tensor: a quarter / half of its
 memory, dW as if x had been rounded to 8 bits per block of 32 features; y, dx and db do not change.
@@ -23,7 +23,6 @@ import os
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -48,34 +47,6 @@ def in_models(flag=None):
     if flag is not None:
         _models = bool(flag)
     return old
-
-
-class _LinearAct(torch.autograd.Function):
-    """y = act(x w' + b) + r for 2-d contiguous x."""
-
-    @staticmethod
-    def forward(ctx, x, w, b, r, activation, save8):
-        K = _native.default_kernels()
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        y, z = K.linear_act(x, w, b, r, activation=activation, save_z=activation is not None and (need_x or need_w or need_b))
-        q = e = None
-        if need_w and save8:
-            q, e = K.act8_pack(x)
-        ctx.save_for_backward(x if need_w and not save8 else None, w if need_x else None, z, q, e)
-        ctx.activation, ctx.in_features = activation, x.shape[1]
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w, z, q, e = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dy = dy.contiguous()
-        dx = dw = db = None
-        if need_x or need_w or need_b:
-            dx, dw, db = _native.default_kernels().linear_backward(
-                dy, x, w, z, q=q, e=e, in_features=ctx.in_features, activation=ctx.activation, need_dx=need_x, need_dw=need_w, need_db=need_b)
-        return dx, dw, db, (dy if need_r else None), None, None
 
 
 def _fusable(fc, w, b, x, residual):
@@ -104,13 +75,4 @@ def linear_act(fc, x, activation=None, residual=None, *, save8=False):
     if not _fusable(fc, w, b, x, residual):
         y = _STOCK[activation](fc(x))
         return y if residual is None else y + residual
-    flat = x.dim() == 2
-    x2 = (x if flat else x.reshape(-1, x.shape[-1])).contiguous()
-    r2 = None if residual is None else (residual if flat else residual.reshape(-1, shape[-1])).contiguous()
-    w, b = w.contiguous(), None if b is None else b.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        y = _LinearAct.apply(x2, w, b, r2, activation, save8)
-    else:
-        y = _native.default_kernels().linear_act(x2, w, b, r2, activation=activation)[0]
-    return y if flat else y.view(shape)
+    return _native.nodes().linear_act(x, w, b, residual, _native.ACTIVATIONS[activation], save8)
