@@ -27,18 +27,29 @@ class Packed8(NamedTuple):
         return self.q.numel() + self.e.numel()
 
 
+_LIKE = {t: torch.empty(0, dtype=t) for t in _native.DTYPES}
+
+
 def pack(x):
     """The 8-bit form of x (at least one dimension; a copy is made first if x is not contiguous)."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError('pack wants a tensor with at least one dimension')
-    with torch.no_grad():
-        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        q, e = _native.default_kernels().act8_pack(x.detach().reshape(rows, x.shape[-1]).contiguous())
-    return Packed8(q, e, x.shape, x.dtype)
+    if x.dtype not in _native.DTYPES:
+        raise TypeError(f'an activation must be float32, bfloat16 or float16, got {x.dtype}')
+    if not x.is_cuda:
+        raise RuntimeError(f'x must live on a HIP device (got {x.device}); ursabench_amd has no CPU path')
+    return Packed8(*_native.nodes().act8_pack(x), x.shape, x.dtype)
 
 
 def unpack(packed):
     """The tensor that `packed` stands for."""
-    features = packed.shape[-1]
-    with torch.no_grad():
-        return _native.default_kernels().act8_unpack(packed.q, packed.e, features, packed.dtype).view(packed.shape)
+    q, e, shape, dtype = packed
+    if dtype not in _native.DTYPES:
+        raise TypeError(f'an activation must be float32, bfloat16 or float16, got {dtype}')
+    features = shape[-1]
+    rows, blocks = (shape.numel() // features if features else 0), -(-features // _native.ACT8_BLOCK)
+    if not (q.is_cuda and e.device == q.device and q.dtype == e.dtype == torch.int8 and q.is_contiguous() and e.is_contiguous()):
+        raise ValueError('q and e must be contiguous int8 tensors on one HIP device')
+    if q.shape != (rows, blocks * _native.ACT8_BLOCK) or e.shape != (rows, blocks):
+        raise ValueError(f'q {tuple(q.shape)} and e {tuple(e.shape)} do not have the elements of a tensor of shape {tuple(shape)}')
+    return _native.nodes().act8_unpack(q, e, shape, _LIKE[dtype])

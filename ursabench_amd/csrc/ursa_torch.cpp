@@ -1,4 +1,4 @@
-// ursa_torch.cpp — K15 / K16 (include/ursa_hip.h) as autograd nodes. The backward pass of a node runs on autograd's device thread:
+// ursa_torch.cpp — K15 / K16 (include/ursa_hip.h) as autograd nodes, and K17's two calls. The backward pass of a node runs on autograd's device thread:
 // written in Python it has to wait there for the interpreter, which costs more than the launches of a small layer (mnist's first
 // layer, forward + backward: 138 us with Python nodes, @@ with these). What may be called and with what is checked by the Python callers
 // (fused_linear, fused_norm); this file allocates, launches on the current stream of the tensors' device and keeps what the
@@ -267,11 +267,31 @@ std::pair<Tensor, Tensor> add_layer_norm(const Tensor& a, const Tensor& r, const
     return {o.z, o.y};
 }
 
+std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
+    at::NoGradGuard no_grad;
+    const int64_t D = x.size(-1);
+    const Tensor x2 = rows_of(x, D);
+    const c10::DeviceGuard guard(x.device());
+    const Packed8 p = pack8(x2);
+    ok(ursa_act8_pack(at_(x2), (int8_t*)at_(p.q), (int8_t*)at_(p.e), x2.size(0), D, type_of(x2), stream_of(x2)), "ursa_act8_pack");
+    return {p.q, p.e};
+}
+
+// q, e: contiguous, of `shape`'s rows and features
+Tensor act8_unpack(const Tensor& q, const Tensor& e, const std::vector<int64_t>& shape, const Tensor& like) {
+    const c10::DeviceGuard guard(q.device());
+    Tensor x = at::empty(shape, like.options().device(q.device()));
+    ok(ursa_act8_unpack((const int8_t*)at_(q), (const int8_t*)at_(e), at_(x), q.size(0), shape.back(), type_of(x), stream_of(q)), "ursa_act8_unpack");
+    return x;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ursa_torch, m) {
     namespace py = pybind11;
     m.attr("abi_version") = URSA_ABI_VERSION;
+    m.def("act8_pack", &act8_pack, py::call_guard<py::gil_scoped_release>());
+    m.def("act8_unpack", &act8_unpack, py::call_guard<py::gil_scoped_release>());
     m.def("linear_act", &linear_act, py::call_guard<py::gil_scoped_release>());
     m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
     m.def("add_layer_norm", &add_layer_norm, py::call_guard<py::gil_scoped_release>());
