@@ -257,6 +257,26 @@ def test_infinities_and_nans_stay_in_their_rows(dtype):
         assert torch.isnan(dw[:, :32]).all() and torch.isfinite(dw[:, 32:]).all()     # the block of 32 features, no other
 
 
+@pytest.mark.parametrize('act', ['gelu', 'silu', 'relu'])
+def test_sums_beyond_the_type_have_their_slope(act):
+    """z = -96,000 is -inf in fp16 where it is kept: y = 0 and the gradient 0, not NaN; z = 96,000: y = inf, the gradient's factor 1;
+    a NaN in z stays one."""
+    from ursabench_amd import _native
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(8, 2, bias=False, device=DEV, dtype=torch.float16)
+    with torch.no_grad():
+        fc.weight.copy_(torch.tensor([[-6000.0] * 8, [6000.0] * 8]))
+    x = torch.full((3, 8), 2.0, device=DEV, dtype=torch.float16, requires_grad=True)
+    y = linear_act(fc, x, act)
+    assert torch.equal(y[:, 0], torch.zeros_like(y[:, 0])) and torch.isinf(y[:, 1]).all()
+    dy = torch.tensor([[1.0, 2.0 ** -10]] * 3, device=DEV, dtype=torch.float16)
+    dx, dw = torch.autograd.grad(y, (x, fc.weight), dy)
+    assert torch.equal(dx, torch.full_like(dx, 6000 / 1024)) and torch.equal(dw, torch.tensor([[0.0] * 8, [6 / 1024] * 8], device=DEV, dtype=torch.float16))
+    z = torch.full((3, 2), float('nan'), device=DEV)
+    db = _native.default_kernels().linear_backward(torch.ones(3, 2, device=DEV), in_features=8, z=z, activation=act, need_dx=False, need_dw=False)[2]
+    assert torch.isnan(db).all() or act == 'relu'
+
+
 def test_large_and_small_magnitudes_fp32():
     """The three-way split holds over fp32's exponents: products of 2^100 and 2^-100, of the largest numbers, and of numbers
     whose low parts are subnormal."""

@@ -83,13 +83,13 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
         for (int i = 0; i < N; ++i) {
             float e;
             const float phi = normal_cdf(z[i], e);
-            g[i] *= fmaf(z[i] * 0.39894228040143268f, e, phi);
+            g[i] *= e > 0.f ? fmaf(z[i] * 0.39894228040143268f, e, phi) : phi;       // z that was rounded to an infinity: 0 or 1
         }
     } else if (act == URSA_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float s = sigmoid(z[i]);
-            g[i] *= s * fmaf(z[i], 1.f - s, 1.f);
+            const float s = sigmoid(z[i]), p = s * (1.f - s);
+            g[i] *= p > 0.f ? fmaf(p, z[i], s) : s;                                   // likewise; a NaN stays one
         }
     } else if (act == URSA_ACT_RELU) {
 #pragma unroll

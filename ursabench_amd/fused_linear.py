@@ -15,6 +15,9 @@ the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd n
 `save8=True` keeps the x that the weight gradient needs in 8 bits (K17, `act8`) instead of the tensor: a quarter / half of its
 memory, dW as if x had been rounded to 8 bits per block of 32 features; y, dx and db do not change.
 
+In a captured step take gradients with `torch.autograd.grad`, or drop every eager graph of the same parameters before the capture:
+their accumulation nodes are bound to the stream of the first graph that uses them, whichever operator that is.
+
 `URSA_FUSED_LINEAR=0` / `enabled(False)` selects the stock ops in `linear_act` everywhere (A/B runs). `URSA_LINEAR_IN_MODELS=1` /
 `in_models(True)` makes `models.MLP` and `models.LeNet5` call it (off by default: their products stay the library's, bit for bit).
 """
