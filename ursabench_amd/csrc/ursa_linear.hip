@@ -175,11 +175,14 @@ __device__ __forceinline__ void split_chunk(const Chunk<T, KIND>& c, s16x8 (&out
 }
 
 // LDS places of a 16-byte piece. kFlat: [rows][BK], the pieces of a row permuted so that eight rows' reads of one k fall into
-// different banks; kAcross: [BK][R], 32-byte slots permuted by k so that the four rows of a transposing read do.
+// different banks; kAcross: [BK][R], 32-byte slots permuted by k so that the rows k .. k + 3 and k + 8 .. k + 11, which half a wave's
+// transposing read takes, do (256 bytes: with the first four alone apart, half of the LDS's active cycles were conflicts).
 template <int BK> __device__ __forceinline__ int flat_at(int row, int piece) {
     return BK == 64 ? row * 64 + ((piece ^ (row & 7)) << 3) : row * 32 + ((piece ^ ((row >> 1) & 3)) << 3);
 }
-template <int R> __device__ __forceinline__ int across_at(int k, int slot) { return k * R + ((slot ^ (k & (R >= 128 ? 7 : 3))) << 4); }
+template <int R> __device__ __forceinline__ int across_at(int k, int slot) {
+    return k * R + ((slot ^ (R >= 128 ? (k & 3) | ((k >> 1) & 4) : (k & 3) ^ ((k >> 3) & 1))) << 4);
+}
 
 // the fragment of 16 rows from row0, k .. k + 31: lane l holds row l % 16, k + 8 (l / 16) .. + 7
 template <int KIND, int BK, int R>
@@ -354,11 +357,12 @@ __device__ __forceinline__ void memory_to_lds(i32x4 buffer, uint32_t offset, con
 constexpr int kWideK = 64;
 constexpr int64_t kWideMaxPitch = 1 << 22;
 
-// A stage of R rows: kFlat [R][64], kAcross [64][R] with 64 bytes after every 1,024 where R = 256 (two k rows)
-template <int R> constexpr int pair_pitch() { return R == 256 ? 2 * R + 32 : 2 * R; }     // shorts from k to k + 2
-template <int R> constexpr int stage_shorts() { return kWideK / 2 * pair_pitch<R>(); }
+// A stage of R rows: kFlat [R][64], kAcross [64][R] with 64 bytes after every 1,024 where R = 256 (two k rows) and 128 after every 8 k
+template <int R> constexpr int pair_pitch() { return R == 256 ? 2 * R + 32 : 2 * R; }     // shorts from k to k + 2 (within 8 k)
+template <int R> constexpr int stage_shorts() { return kWideK / 2 * pair_pitch<R>() + kWideK / 8 * 64; }
+template <int R> __device__ __forceinline__ constexpr int row_at(int k) { return (k >> 1) * pair_pitch<R>() + (k & 1) * R + (k >> 3) * 64; }
 
-// where the 32-byte slot of 16 rows lies within a k row: four consecutive k have to fall into different banks
+// where the 32-byte slot of 16 rows lies within a k row: k .. k + 3 and k + 8 .. k + 11 have to fall into different banks
 template <int R> __device__ __forceinline__ int slot_of(int slot, int k) { return R == 256 ? slot ^ (k & 1) : slot ^ (k & 3); }
 
 // an operand's tile on its way: the buffer starts at (r0, k) and ends with the operand, so that rows and k behind it are out of range
@@ -392,8 +396,8 @@ struct WideTile {
         uint32_t from = offset + i * step;
         if constexpr (KIND == kFlat)
             if (k + kWideK > K) from = k + k0 < K ? from : 0x80000000u;                    // the row goes on with other numbers
-        constexpr int kGap = pair_pitch<R>() - 2 * R;                                      // a wave's 512 shorts: two k rows of 256
-        short* dst = stage + (i * (THREADS / 64) + wave) * (512 + (KIND == kFlat ? 0 : kGap));
+        const int load = i * (THREADS / 64) + wave;                                        // 512 shorts: 512 / R k rows of kAcross
+        short* dst = stage + (KIND == kFlat ? load * 512 : row_at<R>(load * (512 / R)));
         memory_to_lds(buffer, from, dst);
         if (i == kPieces - 1) at += advance;
     }
@@ -421,7 +425,7 @@ struct WideTile<T, kAcross8, R, THREADS> {
         step = (uint32_t)(kRows * o.pitch), step_e = (uint32_t)(kRows * pe);
         at = (uint64_t)o.p + (uint64_t)k_begin * o.pitch + r0, end = (uint64_t)o.p + (uint64_t)K * o.pitch;
         at_e = (uint64_t)o.e + (uint64_t)k_begin * pe + r0 / kBlock8, end_e = (uint64_t)o.e + (uint64_t)K * pe;
-        to = (kr >> 1) * pair_pitch<R>() + (kr & 1) * R + (slot_of<R>(piece >> 1, kr) << 4) + (piece & 1) * 8;
+        to = row_at<R>(kr) + (slot_of<R>(piece >> 1, kr) << 4) + (piece & 1) * 8;
     }
     // piece i of the next stage; behind the last k: zeros
     __device__ __forceinline__ void load(int i) {
@@ -433,8 +437,8 @@ struct WideTile<T, kAcross8, R, THREADS> {
     __device__ __forceinline__ void put(short* stage, int i) {
         s16x8 out[3];
         split_chunk<T, kAcross8>(c[i], out);
-        static_assert(kRows % 4 == 0, "the permutation of the slots repeats every 4 k");
-        *(s16x8*)(stage + to + i * (kRows / 2) * pair_pitch<R>()) = out[0];
+        static_assert(kRows % 8 == 0, "the permutation of the slots repeats every 4 k, the gaps every 8");
+        *(s16x8*)(stage + to + row_at<R>(i * kRows)) = out[0];
     }
 };
 
@@ -444,7 +448,7 @@ __device__ __forceinline__ s16x8 wide_fragment(const short* stage, int row0, int
         return *(const s16x8*)(stage + flat_at<kWideK>(row0 + (lane & 15), (k >> 3) + (lane >> 4)));
     } else {
         const int kr = 8 * (lane >> 4) + ((lane & 15) >> 2);
-        const short* p = stage + ((k + kr) >> 1) * pair_pitch<R>() + (kr & 1) * R + (slot_of<R>(row0 >> 4, kr) << 4) + ((lane & 3) << 2);
+        const short* p = stage + row_at<R>(k) + row_at<R>(kr) + (slot_of<R>(row0 >> 4, kr) << 4) + ((lane & 3) << 2);
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2 * pair_pitch<R>()));
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
