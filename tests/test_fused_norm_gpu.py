@@ -94,6 +94,19 @@ def test_without_weight_or_bias(affine, dtype):
     B.check(_run(x, w, None, dy)[1], *B.norm(x, w, None, 1e-5, dy), where=(affine, dtype))
 
 
+def test_more_rows_than_one_dimension_of_a_launch():
+    """2^20 workgroups and some: the rows behind them are normalised too (narrow: 16 rows a workgroup; wide: one)."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    for M, D in ((2 ** 24 + 100, 3), (2 ** 20 + 37, 2056)):
+        t = torch.bfloat16
+        x = torch.randn(1 << 10, D, device=DEV).to(t).repeat(M // 1024 + 1, 1)[:M]
+        _, y, ms, _, _ = k.layer_norm(x, eps=1e-5, stats=True)
+        _, y0, ms0, _, _ = k.layer_norm(x[:1024].contiguous(), eps=1e-5, stats=True)
+        tail = torch.arange(M - 500, M, device=DEV) % 1024
+        assert torch.equal(y[-500:], y0[tail]) and torch.equal(ms[:, -500:], ms0[:, tail])
+
+
 def test_rows_far_from_zero_keep_their_variance():
     """Mean 1,000 times the deviation: the squares are summed around the mean, not as a difference of large numbers."""
     x, r, w, b, dy, dz = _case(20, 700, 'float32', offset=1500.0)
@@ -321,7 +334,7 @@ def test_pack_shapes_and_refusals():
     x = torch.randn(2, 3, 5, 70, device=DEV)
     assert torch.equal(act8.unpack(act8.pack(x)), act8.unpack(act8.pack(x.view(30, 70))).view_as(x))
     assert torch.equal(act8.unpack(act8.pack(x.transpose(0, 2))), act8.unpack(act8.pack(x)).transpose(0, 2))
-    assert act8.unpack(act8.pack(x[:0])).shape == (0, 3, 5, 70)
+    assert act8.unpack(act8.pack(x[:0])).shape == (0, 3, 5, 70) and act8.unpack(act8.pack(x[..., :0])).shape == (2, 3, 5, 0)
     with pytest.raises(TypeError, match='float32, bfloat16 or float16'):
         act8.pack(x.double())
     with pytest.raises(ValueError):

@@ -47,7 +47,7 @@ def unpack(packed):
     if dtype not in _native.DTYPES:
         raise TypeError(f'an activation must be float32, bfloat16 or float16, got {dtype}')
     features = shape[-1]
-    rows, blocks = (shape.numel() // features if features else 0), -(-features // _native.ACT8_BLOCK)
+    rows, blocks = (shape.numel() // features if features else q.shape[0]), -(-features // _native.ACT8_BLOCK)
     if not (q.is_cuda and e.device == q.device and q.dtype == e.dtype == torch.int8 and q.is_contiguous() and e.is_contiguous()):
         raise ValueError('q and e must be contiguous int8 tensors on one HIP device')
     if q.shape != (rows, blocks * _native.ACT8_BLOCK) or e.shape != (rows, blocks):

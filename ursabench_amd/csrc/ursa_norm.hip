@@ -11,6 +11,8 @@
 // fp32. A row belongs to TPR threads (16 for the narrowest, so that a wave holds four rows; one wave; one workgroup), CV values
 // per thread. dgamma / dbeta: a workgroup walks rows with a fixed stride and keeps its columns' sums in registers, stores them
 // once, and a second launch adds the workgroups' sums in a fixed order - no atomics, the same bits every time.
+// 16,384 x 4,096 bf16: the sum and its norm 107 us (537 MB, 5.0 TB/s), backward with a gradient past the norm 125 us (4.3 TB/s; a
+// large copy moves 4.8). One row of any width: the launch, 5 us.
 #include "ursa_ops.h"
 
 namespace {
@@ -75,7 +77,7 @@ template <typename T, typename P, int TPR, int CV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(NormFwd<T, P> a) {
     constexpr int V = Piece<T>::kN, C = CV / V, R = TPR < 256 ? 256 / TPR : 1;
     __shared__ float red[32];
-    const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * R + threadIdx.x / TPR;
     if (row >= a.M) return;                                  // TPR > 64: a workgroup is one row, so nobody waits for the leavers
     const int t = threadIdx.x % TPR;
     const int64_t base = row * a.D;
@@ -291,7 +293,8 @@ template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwd<T, P> a) {
     constexpr int V = Piece<T>::kN, TPR = 1024;
     __shared__ float red[32];
-    const int64_t row = blockIdx.x, base = row * a.D, step = (int64_t)TPR * V;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, base = row * a.D, step = (int64_t)TPR * V;
+    if (row >= a.M) return;                                  // the whole workgroup
     const int64_t qpitch = (a.D + kBlock8 - 1) / kBlock8 * kBlock8;
     const T* src = a.r ? a.z : a.x;
     float v[V], sum = 0.f;
@@ -341,7 +344,8 @@ template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwd<T, P> a) {
     constexpr int V = Piece<T>::kN, TPR = 1024;
     __shared__ float red[32];
-    const int64_t row = blockIdx.x, base = row * a.D, step = (int64_t)TPR * V;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, base = row * a.D, step = (int64_t)TPR * V;
+    if (row >= a.M) return;                                  // the whole workgroup
     const int64_t qpitch = (a.D + kBlock8 - 1) / kBlock8 * kBlock8;
     const float mean = a.mean[row], rstd = a.rstd[row];
     float m1 = 0.f, m2 = 0.f;
@@ -409,6 +413,7 @@ __global__ __launch_bounds__(256) void k_norm_join(const float* __restrict__ par
     if (out) out[j < D ? j : j - D] = (P)acc;
 }
 
+// one pass each way, 16 bytes of x a thread and turn: 8192 x 4096 bf16 (102 MB) 20 us to pack, 21 to unpack
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, int8_t* __restrict__ q, int8_t* __restrict__ e, int64_t M, int64_t D, int64_t qpitch) {
     constexpr int V = Piece<T>::kN;
@@ -440,6 +445,12 @@ constexpr int64_t kLong = 16384;         // features that the register forms hol
 // rows side by side in one workgroup of the forward, by width (the dispatch below)
 int rows_per_group(int64_t D) { return D <= 128 ? 16 : D <= 2048 ? 4 : 1; }
 
+// a launch has less than 2^32 threads in a dimension: many rows go over two
+dim3 grid_of(int64_t blocks) {
+    const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+
 // Threads of a row in the backward's walk: 8 columns each, so that their sums leave registers for many waves (with 16 or 32 a CU holds
 // few, and 16,384 x 4,096 bf16 with a gradient past the norm took 197 us instead of 125). Above 8,192: 16 columns.
 int bwd_row_threads(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
@@ -458,7 +469,7 @@ int norm_fwd(const NormFwd<T, P>& a, hipStream_t s) {
     void (*fn)(NormFwd<T, P>) = D <= 128 ? k_norm_fwd<T, P, 16, 8> : D <= 512 ? k_norm_fwd<T, P, 64, 8> : D <= 1024 ? k_norm_fwd<T, P, 64, 16>
                               : D <= 2048 ? k_norm_fwd<T, P, 64, 32> : D <= 4096 ? k_norm_fwd<T, P, 256, 16> : D <= 8192 ? k_norm_fwd<T, P, 256, 32>
                               : D <= kLong ? k_norm_fwd<T, P, 1024, 16> : k_norm_fwd_long<T, P>;
-    hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(D <= 8192 ? 256 : 1024), 0, s, a);
+    hipLaunchKernelGGL(fn, grid_of(blocks), dim3(D <= 8192 ? 256 : 1024), 0, s, a);
     return launch_status();
 }
 
@@ -475,7 +486,7 @@ int norm_bwd(const NormBwd<T, P>& a, P* dgamma, P* dbeta, hipStream_t s) {
     const int groups = (int)bwd_groups(a.M, D);
     int rc = URSA_OK;
     if (D > kLong) {
-        if (a.dx) hipLaunchKernelGGL((k_norm_bwd_long<T, P>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+        if (a.dx) hipLaunchKernelGGL((k_norm_bwd_long<T, P>), grid_of(a.M), dim3(1024), 0, s, a);
         if ((rc = launch_status())) return rc;
         if (a.partial) hipLaunchKernelGGL((k_norm_columns_long<T, P>), dim3((unsigned)((D + 256 * Piece<T>::kN - 1) / (256 * Piece<T>::kN)), groups), dim3(256), 0, s, a);
     } else {
@@ -492,7 +503,7 @@ bool bad_dtype(int32_t d) { return d < URSA_F32 || d > URSA_F16; }
 
 int sizes_ok(int64_t M, int64_t D) {
     if (M < 0 || D < 0) return URSA_ESIZE;
-    if (M > INT32_MAX || D > INT32_MAX || (M && D > (INT64_MAX >> 4) / M)) return URSA_ESIZE;
+    if (M > INT32_MAX || D > 1 << 27 || (M && D > (INT64_MAX >> 4) / M)) return URSA_ESIZE;
     return URSA_OK;
 }
 
