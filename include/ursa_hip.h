@@ -630,11 +630,12 @@ int ursa_bn_relu_pool_bwd_f32(const float* z, const float* dpooled, const float*
  *
  *   x [M][K], w [N][K], bias [N] or NULL, residual [M][N] or NULL, y [M][N]: contiguous, one element type (`dtype`), pointers
  *   aligned to an element. z [M][N] or NULL receives x W' + b, rounded to the type, for the backward pass. Sums are fp32; the
- *   activation sees the sum before it is rounded. fp32 operands are multiplied as three bf16 numbers each (exact split, products
- *   down to 2^-24 of |x w|): a non-finite one gives NaN in every sum that it enters.
+ *   activation sees the sum before it is rounded. fp32 operands are multiplied as three bf16 numbers each (exact split; what is dropped
+ *   is below 2^-21.9 of |x w|): a non-finite one gives NaN in every sum that it enters. y of up to 64 rows: fp32 products.
+ *   N, K at most 2^27, and less than 2^24 tiles of 128 x 128 in y, dx and dw (URSA_ESIZE).
  *   backward: dz = dy act'(z) (z as the forward call gave it; rounded to the type for the products, not for db), dx [M][K] = dz W,
  *   dw [N][K] = dz' x, db [N] = column sums of dz; each of dx, dw, db may be NULL: not wanted. x: as `x`, or as its 8-bit form (`q`,
- *   `e`; K17), the other NULL. w is read for dx, x for dw, z with an activation. M = 0: dw and db are zeros.
+ *   `e`; K17), the other NULL. w is read for dx, x for dw, z with an activation. M = 0: dw and db are zeros; N = 0: nothing is written.
  *   ws: ursa_linear_ws_bytes / ursa_linear_bwd_ws_bytes bytes of scratch, 16-byte aligned, private to the call (0: may be NULL); its
  *   contents need not be set.
  * The same call gives the same bits every time (no atomics).
@@ -661,7 +662,7 @@ int ursa_linear_bwd(const void* dy, const void* x /* or NULL */, const int8_t* q
  *   NULL: the 8-bit form of z, written in the same pass, from which ursa_layer_norm_bwd can take xhat instead of x.
  *   backward: dx (or NULL) = d(loss)/dz + dz (dz: the gradient that reaches z by another way, or NULL); dgamma, dbeta [D] (or NULL).
  *   x: what was normalised (z_out if there was an addend). ws: ursa_layer_norm_ws_floats(M, D) floats when dgamma or dbeta is given.
- *   Statistics and sums are fp32, summed in a fixed order.
+ *   M = 0 with dgamma or dbeta: URSA_EVALUE. Statistics and sums are fp32, summed in a fixed order. D at most 2^27.
  */
 int64_t ursa_layer_norm_ws_floats(int64_t M, int64_t D);
 int ursa_layer_norm_fwd(const void* x, const void* addend /* or NULL */, void* z_out /* iff addend */, void* y, const void* gamma,

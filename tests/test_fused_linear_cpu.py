@@ -29,6 +29,9 @@ def test_linear_entries_refuse_bad_arguments(lib, p):
     assert fwd(p, p, None, None, p, None, None, 4, 4, 4, F32, 4, None) == -4          # no such activation
     assert fwd(p, p, None, None, p, None, None, -1, 4, 4, F32, 0, None) == -2
     assert fwd(p, p, None, None, p, None, None, 1 << 31, 4, 4, F32, 0, None) == -2
+    assert fwd(p, p, None, None, p, None, None, 1 << 20, 1 << 20, 4, F32, 0, None) == -2    # more workgroups than a launch has
+    assert fwd(p, p, None, None, p, None, None, 4, 1 << 28, 4, F32, 0, None) == -2
+    assert fwd(p, p, None, None, p, None, None, 4, 4, 1 << 28, F32, 0, None) == -2
     assert fwd(None, p, None, None, p, None, None, 4, 4, 4, F32, 0, None) == -1
     assert fwd(p, None, None, None, p, None, None, 4, 4, 4, F32, 0, None) == -1
     assert fwd(p, p, None, None, None, None, None, 4, 4, 4, F32, 0, None) == -1
@@ -40,6 +43,7 @@ def test_linear_entries_refuse_bad_arguments(lib, p):
     ok = dict(dy=p, x=p, q=None, e=None, w=p, z=p, dx=p, dw=p, db=p, ws=p, M=4, N=4, K=4, t=F16, act=2)
     back = lambda **k: bwd(*{**ok, **k}.values(), None)                               # noqa: E731
     assert back(t=3) == -4 and back(act=4) == -4 and back(M=-1) == -2 and back(N=1 << 31) == -2 and back(K=1 << 31) == -2
+    assert back(M=1 << 20, K=1 << 20) == -2 and back(M=1 << 20, K=1 << 28) == -2 and back(N=1 << 20, K=1 << 20) == -2   # too many tiles of dx, of dw
     assert back(dy=None) == -1 and back(w=None) == -1 and back(ws=None) == -1
     assert back(z=None) == -1                                                         # an activation without z
     assert back(x=None) == -1 and back(q=p, e=p) == -1 and back(x=None, q=p) == -1    # neither x nor its 8-bit form; both; q without e
@@ -54,7 +58,7 @@ def test_norm_and_pack_entries_refuse_bad_arguments(lib, p):
     ok = dict(x=p, a=None, z=None, y=p, g=None, b=None, m=None, r=None, q=None, e=None, M=2, D=4, eps=1e-5, t=F32, pt=F32)
     call = lambda **k: fwd(*{**ok, **k}.values(), None)                               # noqa: E731
     assert call(t=3) == -4 and call(t=F32, pt=BF16) == -4 and call(t=BF16, pt=F16) == -4
-    assert call(M=-1) == -2 and call(M=1 << 31) == -2 and call(D=1 << 31) == -2
+    assert call(M=-1) == -2 and call(M=1 << 31) == -2 and call(D=1 << 28) == -2
     assert call(eps=-1.0) == -5 and call(eps=float('nan')) == -5
     assert call(x=None) == -1 and call(y=None) == -1 and call(a=p) == -1 and call(z=p) == -1 and call(m=p) == -1 and call(q=p) == -1
     assert call(x=p + 2) == -3 and call(g=p + 2) == -3 and call(q=p + 8, e=p) == -3

@@ -236,6 +236,20 @@ def test_empty_batches():
             assert dx.shape == (0, 40) and not dw.any() and not db.any() and dw.shape == (24, 40)
 
 
+def test_no_features_and_no_rows_at_the_kernels():
+    """An empty contraction is a sum of nothing: zeros, in every direction."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    z = lambda *s: torch.empty(s, device=DEV, dtype=torch.bfloat16)      # noqa: E731
+    dx, dw, db = k.linear_backward(z(300, 0), z(300, 40), z(0, 40))
+    assert dx.shape == (300, 40) and not dx.any() and dw.shape == (0, 40) and db.shape == (0,)
+    b = torch.randn(24, device=DEV).bfloat16()
+    for M in (5, 300):
+        assert torch.equal(k.linear_act(z(M, 0), z(24, 0), b)[0], b.expand(M, 24))
+    dx, dg, db = k.layer_norm_backward(z(0, 40), torch.empty(2, 0, device=DEV), x=z(0, 40), need_dgamma=True, need_dbeta=True)
+    assert dx.shape == (0, 40) and dg.shape == db.shape == (40,) and not dg.any() and not db.any()
+
+
 @pytest.mark.parametrize('dtype', list(B.TYPES))
 def test_infinities_and_nans_stay_in_their_rows(dtype):
     """Other rows keep their bits; the row itself is not finite."""
@@ -277,13 +291,14 @@ def test_sums_beyond_the_type_have_their_slope(act):
     assert torch.isnan(db).all() or act == 'relu'
 
 
-def test_large_and_small_magnitudes_fp32():
+@pytest.mark.parametrize('M', [40, 100])
+def test_large_and_small_magnitudes_fp32(M):
     """The three-way split holds over fp32's exponents: products of 2^100 and 2^-100, of the largest numbers, and of numbers
     whose low parts are subnormal."""
     from ursabench_amd import _native
     k = _native.default_kernels()
     g = torch.Generator().manual_seed(3)
-    x, w = torch.randn(40, 64, generator=g), torch.randn(48, 64, generator=g)
+    x, w = torch.randn(M, 64, generator=g), torch.randn(48, 64, generator=g)
     for sx, sw in ((2.0 ** 100, 2.0 ** -100), (2.0 ** -100, 2.0 ** 100), (2.0 ** 120, 2.0 ** -60), (2.0 ** -60, 2.0 ** -40)):
         a, c = x * sx, w * sw
         got = k.linear_act(a.to(DEV), c.to(DEV))[0].double().cpu()
@@ -291,7 +306,7 @@ def test_large_and_small_magnitudes_fp32():
         # below 2^-117 the low parts of an operand are subnormal bf16 numbers, kept to 2^-133: 2^-134 of each times the other
         low = 2.0 ** -134 * (a.abs().double().sum(1)[:, None] + c.abs().double().sum(1)[None, :])
         assert ((got - want['y']).abs() <= bound['y'] + low).all(), (sx, sw)
-    top = torch.full((16, 32), torch.finfo(torch.float32).max)
+    top = torch.full((M, 32), torch.finfo(torch.float32).max)
     got = k.linear_act(top.to(DEV), torch.full((16, 32), 2.0 ** -10, device=DEV))[0].double().cpu()
     want = float(top[0, 0]) * 2.0 ** -10 * 32
     assert ((got - want).abs() <= 1e-6 * want).all()

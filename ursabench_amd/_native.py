@@ -1019,7 +1019,7 @@ class HipKernels:
                 pq, pe = self._act8_ptrs(q, e, M, K, dy)
         pw = _addr(w, 'w', t, N * K, dy) if need_dx else None
         pz = _addr(z, 'z', t, M * N, dy) if act else None
-        dx = dy.new_empty((M, K)) if need_dx else None
+        dx = (dy.new_empty if N else dy.new_zeros)((M, K)) if need_dx else None
         dw = dy.new_empty((N, K)) if need_dw else None
         db = dy.new_empty(N) if need_db else None
         n = lib.ursa_linear_bwd_ws_bytes(M, N, K, dt, act, need_dx, need_dw, need_db)
@@ -1078,9 +1078,10 @@ class HipKernels:
             pq, pe = self._act8_ptrs(q, e, M, D, dy)
         pm = _addr(stats, 'stats', torch.float32, 2 * M, dy)
         px, pd, pz, pg = _addr(x, 'x', t, M * D, dy), _addr(dy, 'dy', t, M * D, dy), _addr(dz, 'dz', t, M * D, dy), _addr(gamma, 'gamma', pt, D, dy)
-        dx = dy.new_empty((M, D)) if need_dx else None
-        dg = dy.new_empty(D, dtype=pt) if need_dgamma else None
-        db = dy.new_empty(D, dtype=pt) if need_dbeta else None
+        new = dy.new_empty if M else dy.new_zeros             # no rows: the sums are zeros, and nothing is launched
+        dx, dg, db = (new(s, dtype=p) if need else None for s, p, need in (((M, D), t, need_dx), (D, pt, need_dgamma), (D, pt, need_dbeta)))
+        if not M:
+            return dx, dg, db
         ws = dy.new_empty(self.lib.ursa_layer_norm_ws_floats(M, D), dtype=torch.float32) if need_dgamma or need_dbeta else None
         self._launch(self.lib.ursa_layer_norm_bwd, dy, px, pq, pe, pd, pz, pg, pm, pm + 4 * M, None if dx is None else dx.data_ptr(),
                      None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),

@@ -1,6 +1,6 @@
 // ursa_torch.cpp — K15 / K16 (include/ursa_hip.h) as autograd nodes, and K17's two calls. The backward pass of a node runs on autograd's device thread:
 // written in Python it has to wait there for the interpreter, which costs more than the launches of a small layer (mnist's first
-// layer, forward + backward: 138 us with Python nodes, @@ with these). What may be called and with what is checked by the Python callers
+// layer, forward + backward: 138 us with Python nodes, 46 with these). What may be called and with what is checked by the Python callers
 // (fused_linear, fused_norm); this file allocates, launches on the current stream of the tensors' device and keeps what the
 // backward pass needs.
 #include <ATen/ATen.h>
@@ -50,7 +50,8 @@ Tensor rows_of(const Tensor& x, int64_t width) { return (x.dim() == 2 && x.size(
 
 struct Packed8 { Tensor q, e; };
 
-Packed8 pack8(const Tensor& x2) {
+// room for the 8-bit form of x2
+Packed8 room8(const Tensor& x2) {
     const int64_t blocks = (x2.size(1) + 31) / 32;
     Packed8 p{at::empty({x2.size(0), 32 * blocks}, x2.options().dtype(at::kChar)), at::empty({x2.size(0), blocks}, x2.options().dtype(at::kChar))};
     return p;
@@ -105,7 +106,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         const Tensor y = linear_forward(x2, wc, packed(b), r.defined() ? rows_of(r, N) : r, act, shape, act && (nx || nw || nb) ? &z : nullptr);
         Packed8 p;
         if (nw && save8) {
-            p = pack8(x2);
+            p = room8(x2);
             const c10::DeviceGuard guard(x.device());
             ok(ursa_act8_pack(at_(x2), (int8_t*)at_(p.q), (int8_t*)at_(p.e), x2.size(0), K, type_of(x2), stream_of(x2)), "ursa_act8_pack");
         }
@@ -162,7 +163,7 @@ NormOut norm_forward(const Tensor& x, const Tensor& r, const Tensor& w, const Te
     o.y = at::empty(shape, x.options());
     if (stats) o.stats = at::empty({2, M}, x.options().dtype(at::kFloat));
     Packed8 p;
-    if (save8) p = pack8(x);
+    if (save8) p = room8(x);
     float* m = (float*)at_(o.stats);
     ok(ursa_layer_norm_fwd(at_(x), at_(r), at_(o.z), at_(o.y), at_(w), at_(b), m, m ? m + M : nullptr, (int8_t*)at_(p.q), (int8_t*)at_(p.e), M, D, (float)eps,
                            type_of(x), w.defined() ? type_of(w) : b.defined() ? type_of(b) : type_of(x), stream_of(x)), "ursa_layer_norm_fwd");
@@ -272,7 +273,7 @@ std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
     const int64_t D = x.size(-1);
     const Tensor x2 = rows_of(x, D);
     const c10::DeviceGuard guard(x.device());
-    const Packed8 p = pack8(x2);
+    const Packed8 p = room8(x2);
     ok(ursa_act8_pack(at_(x2), (int8_t*)at_(p.q), (int8_t*)at_(p.e), x2.size(0), D, type_of(x2), stream_of(x2)), "ursa_act8_pack");
     return {p.q, p.e};
 }
