@@ -366,6 +366,51 @@ def test_side_streams_at_once():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_training_steps_on_side_streams_at_once():
+    """Forward and backward of one layer's copies on two streams: their scratch is their own."""
+    from ursabench_amd.fused_linear import linear_act
+    fcs = [nn.Linear(2048, 640, device=DEV) for _ in range(4)]
+    xs = [torch.randn(300, 2048, device=DEV, requires_grad=True) for _ in range(4)]
+    dy = torch.randn(300, 640, device=DEV)
+
+    def step(fc, x, save8):
+        return torch.autograd.grad(linear_act(fc, x, 'gelu', save8=save8), (x, fc.weight, fc.bias), dy)
+    want = [step(fc, x, i > 1) for i, (fc, x) in enumerate(zip(fcs, xs))]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, (fc, x) in enumerate(zip(fcs, xs)):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(step(fc, x, i > 1))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize('save8', [False, True])
+def test_one_tensor_in_both_places_and_one_layer_twice(save8):
+    """The input as its own residual: its gradient is the layer's and dy; a layer called twice: both calls' gradients."""
+    from ursabench_amd.fused_linear import linear_act
+    fc = nn.Linear(136, 136, device=DEV)
+    x, dy = torch.randn(100, 136, device=DEV, requires_grad=True), torch.randn(100, 136, device=DEV)
+    y = linear_act(fc, x, 'silu', x, save8=save8)
+    got = torch.autograd.grad(y, (x, fc.weight, fc.bias), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(y, (x, fc.weight, fc.bias), dy)))
+    r = x.detach().clone().requires_grad_()
+    yr = linear_act(fc, x, 'silu', r, save8=save8)
+    dx, dw, db, dr = torch.autograd.grad(yr, (x, fc.weight, fc.bias, r), dy)
+    assert torch.equal(y, yr) and torch.equal(dr, dy) and torch.equal(got[0], dx + dy) and torch.equal(got[1], dw) and torch.equal(got[2], db)
+    h = linear_act(fc, x, 'silu', save8=save8)
+    both = torch.autograd.grad(linear_act(fc, h, save8=save8), (x, fc.weight), dy)
+    h2 = h.detach().requires_grad_()
+    dh, dw2 = torch.autograd.grad(linear_act(fc, h2, save8=save8), (h2, fc.weight), dy)
+    dx1, dw1 = torch.autograd.grad(linear_act(fc, x, 'silu', save8=save8), (x, fc.weight), dh)
+    assert torch.equal(both[0], dx1) and torch.equal(both[1], dw1 + dw2)
+
+
 @pytest.mark.parametrize('dtype', list(B.TYPES))
 def test_captured_step_replays_like_the_eager_one(dtype):
     """Forward and backward of a layer (cut contractions among them) in a graph: several replays on new inputs with eager work and

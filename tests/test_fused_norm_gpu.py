@@ -189,6 +189,29 @@ def test_only_the_gradients_that_are_wanted():
     assert torch.equal(only_y, both)
 
 
+def test_one_tensor_in_both_places_and_gradients_of_their_own():
+    from ursabench_amd.fused_norm import add_layer_norm
+    x, r, w, b, dy, dz = (t.to(DEV) for t in _case(40, 200, 'float32'))
+    ln = _module(200, w, b)
+    X, R = x.clone().requires_grad_(), r.clone().requires_grad_()
+    z, y = add_layer_norm(ln, (X, R))
+    torch.autograd.backward((z, y), (dz, dy), retain_graph=True)
+    assert torch.equal(X.grad, R.grad) and X.grad.data_ptr() != R.grad.data_ptr()
+    once = X.grad.clone()
+    X.grad.zero_()                                                # leaves the other one alone
+    assert torch.equal(R.grad, once)
+    torch.autograd.backward((z, y), (dz, dy))
+    assert torch.equal(X.grad, once) and torch.equal(R.grad, 2 * once)
+    T = x.clone().requires_grad_()
+    zt, yt = add_layer_norm(ln, (T, T))
+    assert torch.equal(zt, 2 * x)
+    U, V = x.clone().requires_grad_(), x.clone().requires_grad_()
+    zu, yu = add_layer_norm(ln, (U, V))
+    gu, = torch.autograd.grad((zu, yu), U, (dz, dy))
+    gt, = torch.autograd.grad((zt, yt), T, (dz, dy))
+    assert torch.equal(yt, yu) and torch.equal(gt, 2 * gu)        # the same gradient by both ways
+
+
 @pytest.mark.parametrize('dtype', list(B.TYPES))
 def test_infinities_and_nans_stay_in_their_rows(dtype):
     from ursabench_amd.fused_norm import layer_norm
