@@ -121,11 +121,10 @@ template <typename T, int KIND> struct Chunk { T v[8]; };
 template <typename T> struct Chunk<T, kAcross8> { int8_t v[8]; int8_t e; };
 
 template <typename T, int KIND>
-__device__ __forceinline__ void load_chunk(Chunk<T, KIND>& c, const Operand& o, int64_t outer, int inner, bool in, int inner_end) {
-    // stored row `outer`, elements inner .. inner + 7, those below inner_end
+__device__ __forceinline__ void load_chunk(Chunk<T, KIND>& c, const Operand& o, int64_t outer, int inner, bool whole, bool in, int inner_end) {
+    // stored row `outer`, elements inner .. inner + 7: all of them (`whole`), or those below inner_end if `in`, and zeros
     if constexpr (KIND == kAcross8) {
-        const bool ok = in && inner < inner_end;              // rows are padded to whole blocks of 32 with zeros
-        if (ok) {
+        if (whole || (in && inner < inner_end)) {             // rows are padded to whole blocks of 32 with zeros
             __builtin_memcpy(c.v, (const int8_t*)o.p + outer * o.pitch + inner, 8);
             c.e = o.e[outer * (o.pitch / kBlock8) + inner / kBlock8];
         } else {
@@ -135,7 +134,7 @@ __device__ __forceinline__ void load_chunk(Chunk<T, KIND>& c, const Operand& o, 
         }
     } else {
         const T* p = (const T*)o.p + outer * o.pitch + inner;
-        if (in && inner + 8 <= inner_end) {
+        if (whole) {
             __builtin_memcpy(c.v, p, sizeof c.v);
         } else {
 #pragma unroll
@@ -235,7 +234,10 @@ __device__ __forceinline__ void tile_of(int id, const Shape& s, int& tm, int& tn
     tn = j / rows;
 }
 
-// TILE x TILE outputs by four waves (2 x 2), operands through registers (types that are converted, rows at any alignment)
+// TILE x TILE outputs by four waves (2 x 2), operands through registers (types that are converted, rows at any alignment). What lies
+// behind an operand's rows only enters outputs that are not stored, so whole chunks are read there too: the last row again (kFlat),
+// the next k's numbers (kAcross; there are TILE of them). Element by element, every step of a tile on the edge waited for each of its
+// chunks in turn (1000 x 777 outputs, K 1111, fp16: forward 19.1 -> 16.2 us, dx 19.6 -> 14.4, dW 19.1 -> 16.3).
 template <typename T, int XK, int YK, int TILE>
 __global__ __launch_bounds__(256) void k_product(Operand X, Operand Y, Shape s, Epilogue ep) {
     typedef typename Arith<T>::type A;
@@ -257,10 +259,11 @@ __global__ __launch_bounds__(256) void k_product(Operand X, Operand Y, Shape s, 
             const int id = i * 256 + tid;
             if constexpr (KIND == kFlat) {
                 const int row = r0 + id / (BK / 8), k = k0 + id % (BK / 8) * 8;
-                load_chunk<T, KIND>(c[i], o, row, k, row < o.rows, k_end);
+                load_chunk<T, KIND>(c[i], o, row < o.rows ? row : o.rows - 1, k, k + 8 <= k_end, true, k_end);
             } else {
                 const int k = k0 + id / (TILE / 8), row = r0 + id % (TILE / 8) * 8;
-                load_chunk<T, KIND>(c[i], o, k, row, k < k_end, o.rows);
+                const bool in = k < k_end;
+                load_chunk<T, KIND>(c[i], o, k, row, in && (row + 8 <= o.rows || (k < s.K - 1 && o.pitch >= TILE)), in, o.rows);
             }
         }
     };
