@@ -806,46 +806,64 @@ __global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
     }
 }
 
-// dz = dy act'(z) and the slices' sums of its columns: one pass, bound by its bytes. A workgroup: 32 column pieces x 8 rows at a time,
-// the loads of kRows of those together (8192 x 8192 bf16, gelu, from memory: 100 us for 402 MB, 4 TB/s).
+// dz = dy act'(z) and the slices' sums of its columns: one pass, bound by its bytes. A workgroup: PIECES column pieces x 256 / PIECES
+// rows at a time, the loads of kRows of those together. 32 pieces; 8 where one slice has all rows, so that the activation's
+// arithmetic is spread over more workgroups (gelu, 128 x 200 fp16: 14.9 -> 7.8 us, 256 x 4096 bf16: 28.7 -> 9.0). 8192 x 8192 bf16,
+// gelu, from memory: 100 us for 402 MB, 4 TB/s.
 constexpr int kRows = 4;
-template <typename T>
+
+// V elements from p as they are in memory, of which `room` are the tensor's: past a row's end those of the next one, whose sums are
+// not stored. No conversion in here: it would wait for this load before the next one starts.
+template <typename T, int V>
+__device__ __forceinline__ void load_raw(const T* __restrict__ p, int64_t room, T (&v)[V]) {
+    if (room >= V) {
+        __builtin_memcpy(v, p, sizeof v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = i < room ? p[i] : (T)0.f;
+    }
+}
+
+template <typename T, int PIECES>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, float* __restrict__ partial,
                                                   T* __restrict__ db, int64_t M, int N, int act, int rows) {
-    constexpr int V = Piece<T>::kN;
-    __shared__ float red[8][32 * V];
-    const int piece = threadIdx.x & 31, strand = threadIdx.x >> 5;
-    const int64_t n = ((int64_t)blockIdx.x * 32 + piece) * V, left = N - n;
+    constexpr int V = Piece<T>::kN, STRANDS = 256 / PIECES;
+    __shared__ float red[STRANDS][PIECES * V];
+    const int piece = threadIdx.x % PIECES, strand = threadIdx.x / PIECES;
+    const int64_t n = ((int64_t)blockIdx.x * PIECES + piece) * V, left = N - n;
     const int64_t begin = (int64_t)blockIdx.y * rows, end = begin + rows < M ? begin + rows : M;
     float s[V] = {};
     if (left > 0)
-        for (int64_t m0 = begin + strand; m0 < end; m0 += 8 * kRows) {
-            float g[kRows][V], a[kRows][V];
+        for (int64_t m0 = begin + strand; m0 < end; m0 += STRANDS * kRows) {
+            T raw[2][kRows][V];
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-                const int64_t m = m0 + 8 * r, have = m < end ? left : 0;
-                load_piece<T, V>(dy + m * N + n, have, g[r]);
-                if (z) load_piece<T, V>(z + m * N + n, have, a[r]);
+                const int64_t m = m0 + STRANDS * r, at = m * N + n, room = m < end ? M * N - at : 0;
+                load_raw<T, V>(dy + at, room, raw[0][r]);
+                if (z) load_raw<T, V>(z + at, room, raw[1][r]);
             }
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-                const int64_t m = m0 + 8 * r;
+                const int64_t m = m0 + STRANDS * r;
                 if (m >= end) break;
-                if (z) act_slopes(g[r], a[r], act);
-                if (dz) store_piece<T, V>(dz + m * N + n, left, g[r]);      // dz NULL: the column sums alone are wanted
+                float g[V], a[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) s[i] += g[r][i];                // before dz is rounded to its type
+                for (int i = 0; i < V; ++i) g[i] = (float)raw[0][r][i], a[i] = z ? (float)raw[1][r][i] : 0.f;
+                if (z) act_slopes(g, a, act);
+                if (dz) store_piece<T, V>(dz + m * N + n, left, g);         // dz NULL: the column sums alone are wanted
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] += g[i];                   // before dz is rounded to its type
             }
         }
     if (!partial && !db) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) red[strand][piece * V + i] = s[i];
     __syncthreads();
-    for (int c = threadIdx.x; c < 32 * V; c += 256) {
+    for (int c = threadIdx.x; c < PIECES * V; c += 256) {
         float t = red[0][c];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) t += red[w][c];
-        const int64_t col = (int64_t)blockIdx.x * 32 * V + c;
+        for (int w = 1; w < STRANDS; ++w) t += red[w][c];
+        const int64_t col = (int64_t)blockIdx.x * PIECES * V + c;
         if (col >= N) continue;
         if (db) db[col] = (T)t;                                             // one slice: nothing to add up
         else partial[(int64_t)blockIdx.y * N + col] = t;
@@ -1005,9 +1023,9 @@ int backward(const T* dy, const T* x, const int8_t* q, const int8_t* e, const T*
     T* dz = dz_bytes ? (T*)ws : nullptr;
     float* scratch = (float*)(ws + dz_bytes);
     if (dz || db) {
-        const int rows = act_rows(M, N, dtype), slices = (int)((M + rows - 1) / rows), per = 32 * Piece<T>::kN;
+        const int rows = act_rows(M, N, dtype), slices = (int)((M + rows - 1) / rows), per = (slices == 1 ? 8 : 32) * Piece<T>::kN;
         if (M) {
-            hipLaunchKernelGGL(k_act_grad<T>, dim3((unsigned)((N + per - 1) / per), (unsigned)slices), dim3(256), 0, st, dy, act ? z : nullptr, dz,
+            hipLaunchKernelGGL((slices == 1 ? k_act_grad<T, 8> : k_act_grad<T, 32>), dim3((unsigned)((N + per - 1) / per), (unsigned)slices), dim3(256), 0, st, dy, act ? z : nullptr, dz,
                                db && slices > 1 ? scratch : nullptr, slices == 1 ? db : nullptr, M, (int)N, act, rows);
             if ((rc = launch_status())) return rc;
         }
