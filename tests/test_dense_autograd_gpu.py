@@ -1,0 +1,69 @@
+"""What autograd may ask of the dense blocks' nodes (K15, K16): second derivatives, single gradients, saved tensors that a hook hands
+back, outputs that need no gradient. Operands are small; values are compared bit for bit with the plain call."""
+import itertools
+
+import pytest
+import torch
+import torch.nn as nn
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+ACTS = [None, 'relu', 'gelu', 'silu']
+
+
+def _ops():
+    """name -> (modules, f(x)) for x [., 40]; add_layer_norm's two outputs are added up."""
+    from ursabench_amd.fused_linear import linear_act
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    torch.manual_seed(0)
+    fc, ln = nn.Linear(40, 40, device=DEV), nn.LayerNorm(40, device=DEV)
+    with torch.no_grad():
+        ln.weight.normal_(), ln.bias.normal_()
+    ops = {f'linear {a}': (fc, lambda x, a=a, s=False: linear_act(fc, x, a, x, save8=s)) for a in ACTS}
+    ops['norm'] = (ln, lambda x, s=False: layer_norm(ln, x, save8=s))
+    ops['add'] = (ln, lambda x, s=False: sum(add_layer_norm(ln, (x, 2 * x), save8=s)))
+    ops['z alone'] = (ln, lambda x, s=False: add_layer_norm(ln, (x, 2 * x), save8=s)[0])
+    return ops
+
+
+# ---- second derivatives: they are not offered, so asking for one raises -----------------------
+OPS = [f'linear {a}' for a in ACTS] + ['norm', 'add', 'z alone']
+
+
+@pytest.mark.parametrize('save8', [False, True])
+@pytest.mark.parametrize('op', OPS)
+def test_gradients_under_create_graph_raise_when_differentiated(op, save8):
+    """Also where the incoming gradient is a constant (a loss linear in the output): the gradient of the layer depends on x and the
+    weights all the same, so it must not come back as a constant."""
+    mod, f = _ops()[op]
+    x = torch.randn(9, 40, device=DEV, requires_grad=True)
+    leaves = [x] if op == 'z alone' else [x, mod.weight, mod.bias]
+    for dy in (None, torch.randn(9, 40, device=DEV), torch.randn(9, 40, device=DEV, requires_grad=True)):
+        call = lambda **k: torch.autograd.grad(f(x, s=save8).sum() if dy is None else f(x, s=save8), leaves, dy, **k)      # noqa: E731
+        want, got = call(), call(create_graph=True)
+        for a, b in zip(want, got):
+            assert torch.equal(a, b) and b.requires_grad and not a.requires_grad
+            for t in leaves if dy is None or not dy.requires_grad else [*leaves, dy]:
+                with pytest.raises(RuntimeError, match='double backward'):
+                    torch.autograd.grad(b.sum() + t.sum(), t, retain_graph=True)
+            with pytest.raises(RuntimeError, match='double backward'):
+                b.sum().backward(retain_graph=True)
+
+
+@pytest.mark.parametrize('op', OPS)
+def test_penalties_and_hessians_raise(op):
+    mod, f = _ops()[op]
+    x = torch.randn(3, 40, device=DEV, requires_grad=True)
+    loss = lambda: f(x).square().mean() + torch.autograd.grad(f(x).sum(), x, create_graph=True)[0].square().sum()      # noqa: E731
+    with pytest.raises(RuntimeError, match='double backward'):
+        torch.autograd.grad(loss(), x)
+    with pytest.raises(RuntimeError, match='double backward'):
+        loss().backward()
+    with pytest.raises(RuntimeError, match='double backward'):
+        torch.autograd.functional.hessian(lambda v: f(v).sum(), x.detach())
+    with pytest.raises(RuntimeError, match='double backward'):
+        torch.autograd.functional.jvp(f, x.detach(), torch.ones(3, 40, device=DEV))      # differentiates the gradient with respect to dy
+    x.grad = None                                        # what the refused pass had brought so far
+    f(x).sum().backward(create_graph=True)            # kept gradients carry the refusal
+    with pytest.raises(RuntimeError, match='double backward'):
+        x.grad.sum().backward()

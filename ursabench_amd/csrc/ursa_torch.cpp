@@ -7,7 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/ursa_hip.h"
@@ -57,28 +57,31 @@ Packed8 room8(const Tensor& x2) {
     return p;
 }
 
-// Gradients of a node that is differentiable once: further differentiation raises when it gets there.
-variable_list once(variable_list grads, bool tracked) {
-    if (!tracked) return grads;
-    size_t n = 0;
-    for (auto& g : grads) n += g.defined();
-    if (!n) return grads;
-    variable_list in;
-    for (auto& g : grads)
-        if (g.defined()) in.push_back(g.detach().requires_grad_());
-    const at::AutoGradMode record(true);
-    auto out = (*std::make_shared<torch::autograd::DelayedError>("ursabench_amd: double backward is not offered", (int)n))(std::move(in));
-    size_t k = 0;
-    for (auto& g : grads)
-        if (g.defined()) g = out[k++];
-    return grads;
-}
+// What a gradient of a once differentiable node is a function of when a graph is recorded: whoever differentiates it any further comes
+// through here.
+struct DoubleBackward : torch::autograd::Node {
+    variable_list apply(variable_list&&) override { TORCH_CHECK(false, "ursabench_amd: double backward is not offered"); }
+};
 
-bool tracked(const variable_list& grads) {
-    if (!at::GradMode::is_enabled()) return false;
+// Gradients of a node that is differentiable once. Under create_graph each depends on all the node's
+// inputs and on the incoming gradients, whether or not one of those is tracked: a gradient of a sum has a constant coming in, and
+// depends on the weights all the same. The edges to them are what makes a second differentiation with respect to one of them arrive.
+variable_list once(variable_list grads, const variable_list& incoming, bool create_graph) {
+    if (!create_graph) return grads;
+    torch::autograd::edge_list edges;
+    if (const auto self = torch::autograd::get_current_node())
+        for (const auto& e : self->next_edges())
+            if (e.is_valid()) edges.push_back(e);
+    for (const auto& g : incoming)
+        if (wants(g)) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    const auto refusal = std::make_shared<DoubleBackward>();
+    refusal->set_next_edges(std::move(edges));
     for (auto& g : grads)
-        if (wants(g)) return true;
-    return false;
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::create_gradient_edge(g, refusal);
+        }
+    return grads;
 }
 
 // y (, z) = act(x w' + b) + r for 2-d contiguous operands
@@ -118,7 +121,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const bool again = tracked(grads);
+        const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const int64_t needs = ctx->saved_data["needs"].toInt(), act = ctx->saved_data["act"].toInt();
         const bool nx = needs & 1, nw = needs & 2, nb = needs & 4;
@@ -140,7 +143,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
                                N, K, dt, (int32_t)act, stream_of(dy)), "ursa_linear_bwd");
         }
         if (needs & 8) out[3] = dy_;
-        return once(std::move(out), again);
+        return once(std::move(out), grads, create_graph);
     }
 };
 
@@ -212,11 +215,11 @@ struct Norm : torch::autograd::Function<Norm> {
         return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const bool again = tracked(grads);
+        const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const int64_t needs = ctx->saved_data["needs"].toInt();
         const auto g = norm_backward(ctx, grads[0], Tensor(), needs & 1, needs & 2, needs & 4);
-        return once({g[0], g[1], g[2], Tensor(), Tensor(), Tensor()}, again);
+        return once({g[0], g[1], g[2], Tensor(), Tensor(), Tensor()}, grads, create_graph);
     }
 };
 
@@ -231,7 +234,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         return {o.z, o.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const bool again = tracked(grads);
+        const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const int64_t needs = ctx->saved_data["needs"].toInt();
         const bool na = needs & 1, nr = needs & 8;
@@ -240,13 +243,13 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         if (!dy.defined()) {                                   // y unused: only the sum's own gradient flows
             if (na) out[0] = dz;
             if (nr) out[1] = dz;
-            return once(std::move(out), again);
+            return once(std::move(out), grads, create_graph);
         }
         const auto g = norm_backward(ctx, dy, dz, na || nr, needs & 2, needs & 4);
         if (na) out[0] = g[0];
         if (nr) out[1] = g[0];
         out[2] = g[1], out[3] = g[2];
-        return once(std::move(out), again);
+        return once(std::move(out), grads, create_graph);
     }
 };
 
