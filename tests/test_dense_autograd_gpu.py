@@ -67,3 +67,42 @@ def test_penalties_and_hessians_raise(op):
     f(x).sum().backward(create_graph=True)            # kept gradients carry the refusal
     with pytest.raises(RuntimeError, match='double backward'):
         x.grad.sum().backward()
+
+
+# ---- saved tensors that a hook hands back -------------------------------------------------------
+def _strided(t):
+    """Equal values, other places."""
+    wide = t.new_zeros(t.shape[:-1] + (2 * t.shape[-1],))
+    wide[..., ::2] = t
+    return wide[..., ::2]
+
+
+@pytest.mark.parametrize('save8', [False, True])
+@pytest.mark.parametrize('op', OPS)
+def test_saved_tensors_come_back_in_other_places(op, save8):
+    """Unpack hooks may return equal tensors of any strides (offloading, compression): the same gradients, bit for bit."""
+    mod, f = _ops()[op]
+    x, dy = torch.randn(9, 40, device=DEV, requires_grad=True), torch.randn(9, 40, device=DEV)
+    leaves = [x] if op == 'z alone' else [x, mod.weight, mod.bias]
+    want = torch.autograd.grad(f(x, s=save8), leaves, dy)
+    for pack, unpack in ((lambda t: t, _strided), (lambda t: (t.device, t.cpu()), lambda p: p[1].to(p[0])),
+                         (lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t)):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = f(x, s=save8)
+        assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, leaves, dy)))
+    with torch.autograd.graph.save_on_cpu():
+        y = f(x, s=save8)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, leaves, dy)))
+
+
+@pytest.mark.parametrize('save8', [False, True])
+@pytest.mark.parametrize('op', [o for o in OPS if o != 'z alone'])
+@pytest.mark.parametrize('unpack', [lambda t: t.cpu(), lambda t: t.double(), lambda t: t.flatten()[1:], lambda t: torch.cat([t, t])],
+                         ids=['host', 'type', 'short', 'long'])
+def test_saved_tensors_that_are_not_what_was_saved_raise(unpack, op, save8):
+    mod, f = _ops()[op]
+    x = torch.randn(9, 40, device=DEV, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = f(x, s=save8)
+    with pytest.raises((RuntimeError, ValueError), match='saved'):
+        torch.autograd.grad(y, [x, mod.weight, mod.bias], torch.randn(9, 40, device=DEV))

@@ -43,6 +43,15 @@ Tensor given(const Maybe& t) { return t.has_value() && t->defined() ? *t : Tenso
 
 Tensor packed(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
+// What a backward pass finds of a tensor that its forward kept: a saved_tensors_hooks pair may hand back another one. The same values
+// in other places (strides, a copy) are laid out again; anything that the launch would misread raises.
+Tensor kept(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const Tensor& dy) {
+    if (!t.defined()) return t;
+    TORCH_CHECK(t.layout() == at::kStrided && t.device() == dy.device() && t.scalar_type() == type && t.sizes() == sizes,
+                "ursabench_amd: a saved tensor came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", saved was ", type, " ", sizes, " on ", dy.device());
+    return t.contiguous();
+}
+
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // x as rows of `width`
@@ -126,7 +135,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         const int64_t needs = ctx->saved_data["needs"].toInt(), act = ctx->saved_data["act"].toInt();
         const bool nx = needs & 1, nw = needs & 2, nb = needs & 4;
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &z = saved[2], &q = saved[3], &e = saved[4], &dy_ = grads[0];
+        const Tensor& dy_ = grads[0];
         variable_list out(6);
         if (nx || nw || nb) {
             const std::vector<int64_t> shape = ctx->saved_data["x"].toIntVector();
@@ -135,6 +144,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             const int64_t M = dy.size(0);
             const c10::DeviceGuard guard(dy.device());
             const int32_t dt = type_of(dy);
+            const at::ScalarType t = dy.scalar_type();
+            const int64_t blocks = (K + 31) / 32;
+            const Tensor x = kept(saved[0], {M, K}, t, dy), w = kept(saved[1], {N, K}, t, dy), z = kept(saved[2], {M, N}, t, dy),
+                         q = kept(saved[3], {M, 32 * blocks}, at::kChar, dy), e = kept(saved[4], {M, blocks}, at::kChar, dy);
             if (nx) out[0] = at::empty(shape, dy.options());
             if (nw) out[1] = at::empty({N, K}, dy.options());
             if (nb) out[2] = at::empty({N}, dy.options());
@@ -179,6 +192,7 @@ void norm_keep(AutogradContext* ctx, const Tensor& z, const NormOut& o, const Te
     ctx->save_for_backward({save8 ? Tensor() : z, o.q, o.e, o.stats, w});
     ctx->saved_data["needs"] = needs;
     ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["kept"] = z.sizes().vec();
     ctx->saved_data["width"] = width;
     ctx->saved_data["type"] = (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : z.scalar_type());
 }
@@ -190,14 +204,17 @@ std::array<Tensor, 3> norm_backward(AutogradContext* ctx, const Tensor& dy_, con
     const auto ptype = (at::ScalarType)ctx->saved_data["type"].toInt();
     const Tensor dy = rows_of(dy_, D), dz = dz_.defined() ? rows_of(dz_, D) : dz_;
     const int64_t M = dy.size(0);
+    const int64_t blocks = (D + 31) / 32;
+    const Tensor x = kept(saved[0], ctx->saved_data["kept"].toIntVector(), dy.scalar_type(), dy), q = kept(saved[1], {M, 32 * blocks}, at::kChar, dy),
+                 e = kept(saved[2], {M, blocks}, at::kChar, dy), stats = kept(saved[3], {2, M}, at::kFloat, dy), w = kept(saved[4], {D}, ptype, dy);
     const c10::DeviceGuard guard(dy.device());
     std::array<Tensor, 3> out;
     if (nx) out[0] = at::empty(ctx->saved_data["shape"].toIntVector(), dy.options());
     if (nw) out[1] = at::empty({D}, dy.options().dtype(ptype));
     if (nb) out[2] = at::empty({D}, dy.options().dtype(ptype));
     const Tensor ws = nw || nb ? bytes(dy, 4 * ursa_layer_norm_ws_floats(M, D)) : Tensor();
-    const float* m = (const float*)at_(saved[3]);
-    ok(ursa_layer_norm_bwd(at_(saved[0]), (const int8_t*)at_(saved[1]), (const int8_t*)at_(saved[2]), at_(dy), at_(dz), at_(saved[4]), m, m + M, at_(out[0]),
+    const float* m = (const float*)at_(stats);
+    ok(ursa_layer_norm_bwd(at_(x), (const int8_t*)at_(q), (const int8_t*)at_(e), at_(dy), at_(dz), at_(w), m, m + M, at_(out[0]),
                            at_(out[1]), at_(out[2]), (float*)at_(ws), M, D, type_of(dy), ptype == at::kFloat ? URSA_F32 : ptype == at::kHalf ? URSA_F16 : URSA_BF16,
                            stream_of(dy)), "ursa_layer_norm_bwd");
     return out;
