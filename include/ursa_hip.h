@@ -630,8 +630,9 @@ int ursa_bn_relu_pool_bwd_f32(const float* z, const float* dpooled, const float*
  *
  *   x [M][K], w [N][K], bias [N] or NULL, residual [M][N] or NULL, y [M][N]: contiguous, one element type (`dtype`), pointers
  *   aligned to an element. z [M][N] or NULL receives x W' + b, rounded to the type, for the backward pass. Sums are fp32; the
- *   activation sees the sum before it is rounded. fp32 operands are multiplied as three bf16 numbers each (exact split; what is dropped
- *   is below 2^-21.9 of |x w|): a non-finite one gives NaN in every sum that it enters. y of up to 64 rows: fp32 products.
+ *   activation sees the sum before it is rounded. fp32 operands are multiplied as three bf16 numbers each (exact from 2^-110 up, below
+ *   off by at most 2^-134; of the products what is dropped is below 2^-21.9 of |x w|); y of up to 64 rows and sums that are not finite:
+ *   fp32 products. Infinities, NaNs and sums past the range are fp32's in every form (a cut contraction adds its slices).
  *   N, K at most 2^27, and less than 2^24 tiles of 128 x 128 in y, dx and dw (URSA_ESIZE).
  *   backward: dz = dy act'(z) (z as the forward call gave it; rounded to the type for the products, not for db), dx [M][K] = dz W,
  *   dw [N][K] = dz' x, db [N] = column sums of dz; each of dx, dw, db may be NULL: not wanted. x: as `x`, or as its 8-bit form (`q`,

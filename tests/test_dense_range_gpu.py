@@ -1,0 +1,121 @@
+"""The dense blocks (K15, K16) at the ends of their types' range and precision, against the definition in fp64."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+import dense_bounds as B
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+INF, NAN = math.inf, math.nan
+
+
+# ---- fp32 sums past the range -------------------------------------------------------------------
+# Every form of the fp32 product: (M, K, N) whose forward is 64 x 64 tiles, 64 x 64 with the contraction cut, 128 x 128 (rows that the
+# large form does not take), the large form, the large form with the contraction cut; and, for comparison, up to 64 rows.
+FORMS = [(100, 40, 72), (100, 2040, 72), (2100, 33, 2052), (4104, 72, 2056), (1032, 4104, 1040), (40, 72, 72)]
+
+
+def _signed(M, K, N):
+    """x with a tenth of its rows near 2^100, w near 2^100 with one sign a feature: a sum of the large rows is above 2^200 in
+    magnitude, of that sign - and so are, past the range each, the products with the operands' low parts, which have either sign. The
+    others are inside the range."""
+    g = torch.Generator(device=DEV).manual_seed(M + K + N)
+    x, w = 1 + torch.rand(M, K, generator=g, device=DEV), 1 + torch.rand(N, K, generator=g, device=DEV)
+    big = torch.arange(M, device=DEV) % 10 == 3
+    x[big] *= 2.0 ** 100
+    w *= 2.0 ** 100 * (1 - 2 * (torch.arange(N, device=DEV) % 2).float())[:, None]
+    return x, w, big
+
+
+def _agrees(got, want, k):
+    """Infinities and NaNs of `want` (fp32's: |sum| >= 2^128) exactly, the rest to an fp32 sum's rounding; all terms of a sum have one sign."""
+    want = torch.where(want.abs() >= 2.0 ** 128, want.sign() * INF, want)
+    got = got.double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    fine = want.isfinite()
+    assert ((got - want)[fine].abs() <= B.product_error(want[fine].abs(), k, torch.float32)).all()
+
+
+@pytest.mark.parametrize('M,K,N', FORMS)
+def test_fp32_sums_past_the_range_are_infinite(M, K, N):
+    """Finite operands whose sum fp32 cannot hold: the infinity of its sign in every form and direction, whatever the low parts' signs;
+    relu of -inf is 0. The other rows keep their values."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    x, w, big = _signed(M, K, N)
+    want = x.double() @ w.double().t()
+    assert (want[big].abs() > 2.0 ** 128).all()
+    _agrees(k.linear_act(x, w)[0], want, K)
+    _agrees(k.linear_act(x, w, activation='relu')[0], want.clamp(min=0), K)
+    # dx = dy w: dy takes x's place, [M, N'] with N' = K, w as it is stored for the other direction
+    wt = w.t().contiguous()
+    _agrees(k.linear_backward(x, None, wt, need_dw=False, need_db=False)[0], want, K)
+    # dw = dy' x
+    xt = x.t().contiguous()
+    _agrees(k.linear_backward(xt, wt, need_dx=False, need_db=False)[1], want, K)
+
+
+@pytest.mark.parametrize('M,K,N', [(70, 100, 72), (4104, 72, 2056), (1032, 4104, 1040)])
+def test_fp32_sums_past_the_range_with_the_input_in_8_bits(M, K, N):
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    x, w, _ = _signed(M, K, N)
+    q, e = k.act8_pack(w.t().contiguous())                                  # dw [M, N] = x (as dy' [K, M]) times the kept [K, N]
+    kept = B.unpacked(w.t().contiguous())
+    got = k.linear_backward(x.t().contiguous(), None, None, q=q, e=e, in_features=N, need_dx=False, need_db=False)[1]
+    _agrees(got, x.double() @ kept, K)
+
+
+@pytest.mark.parametrize('M,K,N', FORMS)
+def test_fp32_infinities_and_nans_enter_sums_as_they_do_in_fp32(M, K, N):
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    g = torch.Generator(device=DEV).manual_seed(K)
+    x, w = 1 + torch.rand(M, K, generator=g, device=DEV), 1 + torch.rand(N, K, generator=g, device=DEV)
+    w *= (1 - 2 * (torch.arange(N, device=DEV) % 2).float())[:, None]
+    x[5, K - 1], x[7, 3], x[8, 0], x[M - 1, K // 2] = INF, -INF, NAN, INF
+    w[2, K - 1], w[4, 3], w[N - 1, 1] = 0, INF, NAN
+    want = x.double() @ w.double().t()
+    assert want[5, 2].isnan() and want[5, 3] == -INF and want[7, 4] == -INF and want[8].isnan().all() and want[0, 4] == INF
+    for act, f in ((None, lambda z: z), ('relu', torch.relu)):
+        _agrees(k.linear_act(x, w, activation=act)[0], f(want), K)
+    wt = w.t().contiguous()
+    _agrees(k.linear_backward(x, None, wt, need_dw=False, need_db=False)[0], want, K)
+    _agrees(k.linear_backward(x.t().contiguous(), wt, need_dx=False, need_db=False)[1], want, K)
+
+
+def test_fp32_the_largest_numbers_and_a_row_among_many():
+    """The largest number times one, sums that end exactly at it, and a row's answer beside 3 rows and beside 300."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    top = torch.finfo(torch.float32).max
+    x, w, big = _signed(300, 72, 72)
+    few = k.linear_act(x[:4].contiguous(), w)[0]
+    many = k.linear_act(x, w)[0]
+    assert torch.equal(few.isfinite(), many[:4].isfinite()) and torch.equal(few[3], many[3]) and few[3].isinf().all()
+    x, w = torch.zeros(300, 72, device=DEV), torch.zeros(72, 72, device=DEV)
+    x[:, 5], w[:, 5] = top, 1
+    x[:, 9], w[1::2, 9] = 1, top                                            # 2 top: past the range
+    y = k.linear_act(x, w)[0]
+    assert (y[:, 0::2] == top).all() and (y[:, 1::2] == INF).all()
+
+
+@pytest.mark.parametrize('M,K,N', FORMS)
+def test_fp32_operands_near_the_smallest(M, K, N):
+    """From 2^-110 up the three parts of an operand hold all of it; below, its low part ends at the smallest bf16 number, 2^-133: half of
+    that is lost of each operand, times the other. Subnormal operands among them."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    g = torch.Generator(device=DEV).manual_seed(N)
+    for scale in (-110, -113, -118, -126, -131):
+        x = (1 + torch.rand(M, K, generator=g, device=DEV)) * 2.0 ** scale
+        w = (1 + torch.rand(N, K, generator=g, device=DEV)) * 2.0 ** 100
+        want = x.double() @ w.double().t()
+        bound = B.product_error(want, K, torch.float32) + (0 if scale >= -110 else 2.0 ** -134 * w.double().abs().sum(1))
+        for got in (k.linear_act(x, w)[0], k.linear_backward(x, None, w.t().contiguous(), need_dw=False, need_db=False)[0],
+                    k.linear_backward(x.t().contiguous(), w.t().contiguous(), need_dx=False, need_db=False)[1]):
+            assert ((got.double() - want).abs() <= bound).all(), scale

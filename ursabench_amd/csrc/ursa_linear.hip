@@ -7,9 +7,9 @@
 // contiguous: x and W forward) or across it (W in dx; dz and x in dW). Both go to LDS as rows of 16-bit numbers; the first kind is
 // read as eight consecutive k of a row (ds_read_b128), the second by the transposing LDS read (ds_read_b64_tr_b16), which hands
 // each lane four k of its column. fp32 operands are split while they are staged, v = hi + mid + lo with three bf16 numbers
-// (8 + 8 + 8 bits: exact), and six of the nine partial products are summed in fp32: what is left out (mid lo twice, lo lo) is below
-// 2^-21.9 of |x w| and 2^-25 on average, of either sign, and the bf16 matrix instruction does 16 times the work of the fp32 one. A
-// non-finite fp32 operand makes the sums it enters NaN (its remainder is inf - inf).
+// (8 + 8 + 8 bits: exact from 2^-110 up; below, lo ends at 2^-133 and half of that is lost), and six of the nine partial products are
+// summed in fp32: what is left out (mid lo twice, lo lo) is below 2^-21.9 of |x w| and 2^-25 on average, of either sign, and the bf16
+// matrix instruction does 16 times the work of the fp32 one. Sums that come out not finite are taken once more without the split.
 //
 // Sums are fp32; a contraction is cut over workgroups where there are few tiles, and a second launch adds the pieces in order.
 #include "ursa_ops.h"
@@ -196,6 +196,67 @@ __device__ __forceinline__ s16x8 fragment(const short* plane, int row0, int k, i
     }
 }
 
+// numbers (row, k) .. (row, k + U - 1) of an fp32 operand; zeros from k_end on
+template <int KIND, int U>
+__device__ __forceinline__ void numbers_at(const Operand& o, int row, int k, int k_end, float (&v)[U]) {
+    if constexpr (KIND == kFlat) {
+        load_piece<float, U>((const float*)o.p + row * o.pitch + k, k_end - k, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t at = k + i < k_end ? k + i : k_end - 1;
+            if constexpr (KIND == kAcross8) v[i] = value8(((const int8_t*)o.p)[at * o.pitch + row], o.e[at * (o.pitch / kBlock8) + row / kBlock8]);
+            else v[i] = ((const float*)o.p)[at * o.pitch + row];
+            if (k + i >= k_end) v[i] = 0.f;
+        }
+    }
+}
+
+// The split's sums that are not finite, again. The parts of a number may differ in sign, so where hi hi is past the range and hi lo past
+// the other end of it they make a NaN of an infinite sum; and the remainder of an infinite operand is one. Either way the sum is not
+// finite and stays so. A wave that holds such a sum takes the 16 columns around it once more by the fp32 instruction, straight from
+// memory (k as in k_rows), and keeps what that has in the place of it: infinities and NaNs as fp32 has them. 4096^3 (715 us): a row of
+// them 1.9 ms, nothing else 2.7 ms; none of them: within 1 % of the kernels without this.
+template <int XK, int YK, int FY, int FX>
+__device__ __forceinline__ void sums_again(f32x4 (&acc)[FY][FX], const Operand& X, const Operand& Y, int m0, int n0, int k_begin, int k_end, int lane) {
+    constexpr int U = FX > 2 ? 8 : 4;                     // k a lane and turn; the smaller tile keeps its registers
+    float top[FY], most = 0.f;                            // the largest magnitude; a NaN is larger than all (two sums an instruction)
+#pragma unroll
+    for (int j = 0; j < FY; ++j) {
+        top[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < FX; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) top[j] = __builtin_elementwise_maximum(top[j], fabsf(acc[j][i][v]));
+        most = __builtin_elementwise_maximum(most, top[j]);
+    }
+    if (!__any(!(most < INFINITY))) return;
+#pragma unroll
+    for (int j = 0; j < FY; ++j) {
+        if (!__any(!(top[j] < INFINITY))) continue;               // the whole wave goes on: the instruction takes every lane's numbers
+        const int n = n0 + 16 * j + (lane & 15), ry = n < Y.rows ? n : Y.rows - 1;      // behind the last row: not stored
+        f32x4 c[FX] = {};
+        for (int k0 = k_begin; k0 < k_end; k0 += 4 * U) {
+            const int k = k0 + U * (lane >> 4);
+            float y[U], x[FX][U];
+            numbers_at<YK>(Y, ry, k, k_end, y);
+#pragma unroll
+            for (int i = 0; i < FX; ++i) {
+                const int m = m0 + 16 * i + (lane & 15);
+                numbers_at<XK>(X, m < X.rows ? m : X.rows - 1, k, k_end, x[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < FX; ++i)
+#pragma unroll
+                for (int u = 0; u < U; ++u) c[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[u], x[i][u], c[i], 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < FX; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[j][i][v] = fabsf(acc[j][i][v]) < INFINITY ? acc[j][i][v] : c[i][v];
+    }
+}
+
 // C consecutive n of one m through the epilogue; `bias`: those of the bias, or zeros
 template <typename T, int C>
 __device__ __forceinline__ void finish(const Epilogue& ep, int64_t m, int n, int N, float (&v)[C], const float (&bias)[C]) {
@@ -317,6 +378,7 @@ __global__ __launch_bounds__(256) void k_product(Operand X, Operand Y, Shape s, 
             }
         }
     }
+    if constexpr (PX > 1) sums_again<XK, YK>(acc, X, Y, m0 + wm, n0 + wn, k_begin, k_end, lane);
     // accumulator of (fy, fx): lane l holds m = l % 16 and n = 4 (l / 16) .. + 3
 #pragma unroll
     for (int i = 0; i < F; ++i) {
@@ -703,6 +765,7 @@ __global__ __launch_bounds__(kSplitThreads, 2) void k_product_split(Operand X, O
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    sums_again<XK, YK>(acc, X, Y, m0 + wm, n0 + wn, k_begin, k_end, lane);
     store_tile<float, 4>(acc, (float*)&lds[0][0], wave, lane, m0 + wm, n0 + wn, s, ep);
 }
 
