@@ -119,3 +119,85 @@ def test_fp32_operands_near_the_smallest(M, K, N):
         for got in (k.linear_act(x, w)[0], k.linear_backward(x, None, w.t().contiguous(), need_dw=False, need_db=False)[0],
                     k.linear_backward(x.t().contiguous(), w.t().contiguous(), need_dx=False, need_db=False)[1]):
             assert ((got.double() - want).abs() <= bound).all(), scale
+
+
+# ---- rows far from zero -------------------------------------------------------------------------
+def _norm_bound(z, eps, g, b, stored_mean):
+    """(y, bound on y or on what follows from xhat) of a row-wise norm whose mean is corrected by the mean of what it leaves. n roundings a
+    sum as in dense_bounds.norm. First mean: off by d1 <= (n + 1) F max|z|. v = z - mean: F |v|. The mean of v: off by (n + 1) F mean|v|,
+    with mean|v| <= deviation + d1. The variance around it: (n + 4) F (var + d1^2). `stored_mean`: the backward pass has the mean
+    rounded once more, to fp32: F |mean|."""
+    Z = z.double()
+    n = 64 + 2 * Z.shape[1] / 8192
+    mean = Z.mean(1, keepdim=True)
+    var = ((Z - mean) ** 2).mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    d1 = (n + 1) * B.F * Z.abs().amax(1, keepdim=True)
+    centre = (n + 2) * B.F * (var.sqrt() + d1) + 2 * B.F * ((Z - mean).abs() + d1) + (B.F * mean.abs() if stored_mean else 0)
+    xhat = (Z - mean) * rstd
+    relative = (n + 4) * B.F * (var + d1 ** 2) / (var + eps) + 4 * B.F
+    if stored_mean:
+        relative = relative + (B.F * mean.abs() * rstd) ** 2
+    return xhat, rstd, centre * rstd + relative * (xhat.abs() + centre * rstd)
+
+
+@pytest.mark.parametrize('dtype', list(B.TYPES))
+@pytest.mark.parametrize('D', [7, 24, 100, 777, 1000, 1111, 2500, 5000, 10000, 16000, 20000])
+def test_constant_rows_are_zero(D, dtype):
+    """The mean of D equal numbers is that number, whether or not 1 / D is one: y is the bias and the gradients of the scale are 0."""
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    t = B.TYPES[dtype]
+    ln = nn.LayerNorm(D, device=DEV)
+    with torch.no_grad():
+        ln.bias.fill_(0.5)
+    ln = ln.to(t)
+    # whole and dyadic numbers whose sums fp32 holds exactly; the others round on the way
+    x = torch.tensor([1000.0, 2.5, -3.0, 0.0, 0.1, 1234.567, -33333.0, 1e-3], device=DEV).to(t)[:, None].expand(8, D).contiguous()
+    if dtype != 'float32':
+        x[6] = -1000
+    xhat, _, bound = _norm_bound(x, 1e-5, None, None, False)
+    assert float(xhat.abs().max()) <= 1e-6
+    y = layer_norm(ln, x)
+    assert ((y.double() - 0.5).abs() <= bound + xhat.abs() + B.half_step(t) * 0.5).all() and (y[:4] == 0.5).all()
+    z, y = add_layer_norm(ln, (x, torch.zeros_like(x)))
+    assert torch.equal(z, x) and (y[:4] == 0.5).all()
+    X = x[:4].clone().requires_grad_()
+    dx, dg = torch.autograd.grad(layer_norm(ln, X), (X, ln.weight), torch.ones(4, D, device=DEV, dtype=t))
+    assert not dg.any() and not dx.any()                    # xhat is 0, and a constant gradient has no component that moves y
+
+
+@pytest.mark.parametrize('D', [7, 100, 1000, 1111, 5000, 10000, 20000])
+def test_fp32_rows_far_from_zero(D):
+    """Deviation 1e-5 of the mean, eps 1e-12 of its square and more."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    g = torch.Generator(device=DEV).manual_seed(D)
+    for mean, deviation in ((1000.0, 0.03), (-77.7, 1e-3), (1.0, 1e-4), (3e4, 3.0)):
+        x = mean + deviation * torch.randn(9, D, generator=g, device=DEV)
+        gamma, dy = 1 + 0.3 * torch.randn(D, generator=g, device=DEV), torch.randn(9, D, generator=g, device=DEV)
+        eps = 1e-5
+        xhat, rstd, bound = _norm_bound(x, eps, None, None, False)
+        _, y, stats, _, _ = k.layer_norm(x, eps=eps, stats=True)
+        assert ((y.double() - xhat).abs() <= bound + B.last_rounding(xhat, torch.float32)).all(), (mean, deviation)
+        true = x.double().mean(1)
+        n = 64 + 2 * D / 8192
+        off = (n + 3) * B.F * ((x.double() - true[:, None]).abs().mean(1) + (n + 1) * B.F * x.double().abs().amax(1))
+        assert ((stats[0].double() - true).abs() <= off + B.F * true.abs()).all()      # one rounding of the mean, and the correction's own
+        _, _, e = _norm_bound(x, eps, None, None, True)
+        dx, dg, db = k.layer_norm_backward(dy, stats, gamma, x=x, need_dgamma=True, need_dbeta=True)
+        DY = dy.double()
+        want = (DY * xhat).sum(0)
+        assert ((dg.double() - want).abs() <= (DY.abs() * e).sum(0) + 25 * B.F * (DY * xhat).abs().sum(0) + B.last_rounding(want, torch.float32)).all()
+
+
+@pytest.mark.parametrize('D', [7, 49, 1000, 1111, 4099, 10000, 20000])
+def test_a_constant_gradient_moves_nothing(D):
+    """t = dy gamma equal along a row that is constant itself: dx = rstd (t - mean t) = 0, the mean of D equal numbers being that number."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    x = torch.full((9, D), 2.5, device=DEV)
+    dy = torch.tensor([1.0, 3.0, 77.0, -1000.0, 801.0, 0.375, 1023.0, 5.0, 11.0], device=DEV)[:, None].expand(9, D).contiguous()   # sums are exact
+    _, _, stats, _, _ = k.layer_norm(x, eps=1e-5, stats=True)
+    assert torch.equal(stats[0], x[:, 0])
+    dx, dg, _ = k.layer_norm_backward(dy, stats, x=x, need_dgamma=True)
+    assert not dx.any() and not dg.any()

@@ -3,6 +3,9 @@
 //
 //   z = x (+ r, rounded to the tensors' type: what the caller keeps is what is normalised)
 //   mean = (sum_d z_d) / D ; var = (sum_d (z_d - mean)^2) / D ; rstd = 1 / sqrt(var + eps) ; xhat = (z - mean) rstd
+//   the mean's own rounding (its sum's, and the division's) would move every xhat of the row the same way, in rows far from zero by more
+//   than their deviation: with m the mean as it comes out, rest = (sum_d (z_d - m)) / D, mean = m + rest, xhat = ((z - m) - rest) rstd and
+//   var = (sum_d (z_d - m)^2) / D - rest^2. The backward pass has that mean rounded once, to fp32.
 //   y = xhat gamma + beta
 //   t = dy gamma ; dx = rstd (t - (sum_d t) / D - xhat (sum_d t xhat) / D) (+ dz) ; dgamma = sum_rows dy xhat ; dbeta = sum_rows dy
 //
@@ -33,6 +36,27 @@ __device__ __forceinline__ float row_sum(float v, float* red, int slot) {
         for (int w = 1; w < TPR / 64; ++w) v += r[w];
     }
     return v;
+}
+
+// two sums over a row at once, in the slots behind that of row_sum's slot 0: 3 x 16 floats of LDS
+template <int TPR>
+__device__ __forceinline__ float2 row_sums(float a, float b, float* red) {
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) a += __shfl_xor(a, o), b += __shfl_xor(b, o);
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) red[16 + (threadIdx.x >> 6)] = a, red[32 + (threadIdx.x >> 6)] = b;
+        __syncthreads();
+        a = red[16], b = red[32];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) a += red[16 + w], b += red[32 + w];
+    }
+    return make_float2(a, b);
+}
+
+// 1 / sqrt of the variance around m + rest; rounding may leave a constant row's below zero (a NaN stays one)
+__device__ __forceinline__ float inverse_deviation(float mean_square, float rest, float eps) {
+    const float var = mean_square - rest * rest;
+    return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);
 }
 
 // the exponent byte of this thread's block of 32 (V values here, the rest in the neighbouring 32 / V - 1 threads)
@@ -70,13 +94,13 @@ struct NormFwd {
     float *mean, *rstd;
     int8_t *q, *e;
     int64_t M, D;
-    float eps, inv_d;
+    float eps, d;                        // d: D, to divide by (1 / D is rounded for most widths)
 };
 
 template <typename T, typename P, int TPR, int CV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(NormFwd<T, P> a) {
     constexpr int V = Piece<T>::kN, C = CV / V, R = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float red[32];
+    __shared__ float red[48];
     const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * R + threadIdx.x / TPR;
     if (row >= a.M) return;                                  // TPR > 64: a workgroup is one row, so nobody waits for the leavers
     const int t = threadIdx.x % TPR;
@@ -98,8 +122,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(NormFwd<T, P
 #pragma unroll
         for (int i = 0; i < V; ++i) sum += v[c][i];
     }
-    const float mean = row_sum<TPR>(sum, red, 0) * a.inv_d;
-    float sq = 0.f;
+    const float mean = row_sum<TPR>(sum, red, 0) / a.d;
+    float off = 0.f, sq = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int64_t d = (int64_t)(c * TPR + t) * V;
@@ -111,11 +135,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(NormFwd<T, P
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             v[c][i] -= mean;
-            sq += d + i < a.D ? v[c][i] * v[c][i] : 0.f;
+            const float in = d + i < a.D ? v[c][i] : 0.f;
+            off += in, sq += in * in;
         }
     }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, red, 1) * a.inv_d + a.eps);
-    if (a.mean && t == 0) a.mean[row] = mean, a.rstd[row] = rstd;
+    const float2 sums = row_sums<TPR>(off, sq, red);
+    const float rest = sums.x / a.d, rstd = inverse_deviation(sums.y / a.d, rest, a.eps);
+    if (a.mean && t == 0) a.mean[row] = mean + rest, a.rstd[row] = rstd;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int64_t d = (int64_t)(c * TPR + t) * V, left = a.D - d;
@@ -124,7 +150,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(NormFwd<T, P
         if (a.beta) load_piece<P, V>(a.beta + d, left, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            float o = v[c][i] * rstd;
+            float o = (v[c][i] - rest) * rstd;
             if (a.gamma) o *= g[i];
             if (a.beta) o += b[i];
             v[c][i] = o;
@@ -143,7 +169,7 @@ struct NormBwd {
     T* dx;
     float* partial;                      // [gridDim.x][2][D], or NULL
     int64_t M, D;
-    float inv_d;
+    float d;
 };
 
 // a row's numbers of this thread as they are in memory
@@ -246,7 +272,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) 
             }
         }
         if constexpr (TPR > 64) __syncthreads();                 // the previous row's sums have been read
-        const float m1 = row_sum<TPR>(s1, red, 0) * a.inv_d, m2 = row_sum<TPR>(s2, red, 1) * a.inv_d;
+        const float m1 = row_sum<TPR>(s1, red, 0) / a.d, m2 = row_sum<TPR>(s2, red, 1) / a.d;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int64_t d = (int64_t)(c * TPR + t) * V, left = a.D - d;
@@ -292,7 +318,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void k_norm_bwd(NormBwd<T, P> a) 
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwd<T, P> a) {
     constexpr int V = Piece<T>::kN, TPR = 1024;
-    __shared__ float red[32];
+    __shared__ float red[48];
     const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, base = row * a.D, step = (int64_t)TPR * V;
     if (row >= a.M) return;                                  // the whole workgroup
     const int64_t qpitch = (a.D + kBlock8 - 1) / kBlock8 * kBlock8;
@@ -315,15 +341,19 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwd<T, P> a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) sum += v[i];
     }
-    const float mean = row_sum<TPR>(sum, red, 0) * a.inv_d;
-    float sq = 0.f;
+    const float mean = row_sum<TPR>(sum, red, 0) / a.d;
+    float off = 0.f, sq = 0.f;
     for (int64_t d = (int64_t)threadIdx.x * V; d < a.D; d += step) {
         load_piece<T, V>(src + base + d, a.D - d, v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) sq += d + i < a.D ? (v[i] - mean) * (v[i] - mean) : 0.f;
+        for (int i = 0; i < V; ++i) {
+            const float in = d + i < a.D ? v[i] - mean : 0.f;
+            off += in, sq += in * in;
+        }
     }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, red, 1) * a.inv_d + a.eps);
-    if (a.mean && threadIdx.x == 0) a.mean[row] = mean, a.rstd[row] = rstd;
+    const float2 sums = row_sums<TPR>(off, sq, red);
+    const float rest = sums.x / a.d, rstd = inverse_deviation(sums.y / a.d, rest, a.eps);
+    if (a.mean && threadIdx.x == 0) a.mean[row] = mean + rest, a.rstd[row] = rstd;
     for (int64_t d = (int64_t)threadIdx.x * V; d < a.D; d += step) {
         float g[V], b[V];
         load_piece<T, V>(src + base + d, a.D - d, v);
@@ -331,7 +361,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwd<T, P> a) {
         if (a.beta) load_piece<P, V>(a.beta + d, a.D - d, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            float o = (v[i] - mean) * rstd;
+            float o = (v[i] - mean - rest) * rstd;
             if (a.gamma) o *= g[i];
             if (a.beta) o += b[i];
             v[i] = o;
@@ -368,7 +398,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwd<T, P> a) {
             }
             if (walk && a.dx) store_piece<T, V>(a.dx + base + d, left, t);
         }
-        if (!walk) m1 = row_sum<TPR>(s1, red, 0) * a.inv_d, m2 = row_sum<TPR>(s2, red, 1) * a.inv_d;
+        if (!walk) m1 = row_sum<TPR>(s1, red, 0) / a.d, m2 = row_sum<TPR>(s2, red, 1) / a.d;
     }
 }
 
@@ -530,7 +560,7 @@ extern "C" int ursa_layer_norm_fwd(const void* x, const void* addend, void* z_ou
     const uintptr_t es = (uintptr_t)element_size(dtype) - 1, ps = (uintptr_t)element_size(pdtype) - 1;
     if (((uintptr_t)x | (uintptr_t)addend | (uintptr_t)z_out | (uintptr_t)y) & es || ((uintptr_t)gamma | (uintptr_t)beta) & ps ||
         ((uintptr_t)mean | (uintptr_t)rstd) & 3 || (uintptr_t)q & 15) return URSA_EALIGN;
-#define URSA_CALL(T, P) norm_fwd<T, P>({(const T*)x, (const T*)addend, (T*)z_out, (T*)y, (const P*)gamma, (const P*)beta, mean, rstd, q, e, M, D, eps, 1.f / (float)D}, (hipStream_t)stream)
+#define URSA_CALL(T, P) norm_fwd<T, P>({(const T*)x, (const T*)addend, (T*)z_out, (T*)y, (const P*)gamma, (const P*)beta, mean, rstd, q, e, M, D, eps, (float)D}, (hipStream_t)stream)
     return URSA_NORM_TYPES(dtype, pdtype, URSA_CALL);
 #undef URSA_CALL
 }
@@ -546,7 +576,7 @@ extern "C" int ursa_layer_norm_bwd(const void* x, const int8_t* q, const int8_t*
     if (((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dz | (uintptr_t)dx) & es || ((uintptr_t)gamma | (uintptr_t)dgamma | (uintptr_t)dbeta) & ps ||
         ((uintptr_t)mean | (uintptr_t)rstd | (uintptr_t)ws) & 3 || (uintptr_t)q & 15) return URSA_EALIGN;
     float* part = dgamma || dbeta ? ws : nullptr;
-#define URSA_CALL(T, P) norm_bwd<T, P>({(const T*)x, q, e, (const T*)dy, (const T*)dz, (const P*)gamma, mean, rstd, (T*)dx, part, M, D, 1.f / (float)D}, (P*)dgamma, (P*)dbeta, (hipStream_t)stream)
+#define URSA_CALL(T, P) norm_bwd<T, P>({(const T*)x, q, e, (const T*)dy, (const T*)dz, (const P*)gamma, mean, rstd, (T*)dx, part, M, D, (float)D}, (P*)dgamma, (P*)dbeta, (hipStream_t)stream)
     return URSA_NORM_TYPES(dtype, pdtype, URSA_CALL);
 #undef URSA_CALL
 }
