@@ -8,8 +8,8 @@ launches differ:
   backward          the activation's gradient and the bias gradient in one pass over dy, then dx and dW by the same product kernel
 
 float32, bfloat16 and float16, any sizes and leading dimensions, on a HIP device. Operands that are not contiguous are copied first.
-Anything else - host tensors, other or mixed types, autocast, a subclass with a forward of its own, hooks on `fc` - takes
-`fc(x)`, the activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises. On a HIP tensor
+Anything else - host tensors, other or mixed types, autocast, a class or an instance with a forward of its own, hooks on `fc` or on
+all modules - takes `fc(x)`, the activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises. On a HIP tensor
 the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the x that the weight gradient needs in 8 bits (K17, `act8`) instead of the tensor: a quarter / half of its
@@ -26,6 +26,7 @@ import os
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import _native
 
@@ -55,7 +56,7 @@ def in_models(flag=None):
 def _fusable(fc, w, b, x, residual):
     t, dev = x.dtype, x.get_device()
     return (_on and x.is_cuda and t in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
-            and type(fc).forward is nn.Linear.forward
+            and type(fc).forward is nn.Linear.forward and 'forward' not in fc.__dict__ and not _has_any_global_hook()
             and not (fc._forward_hooks or fc._forward_pre_hooks or fc._backward_hooks or fc._backward_pre_hooks)
             and w.dtype is t and w.get_device() == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
             and (b is None or (b.dtype is t and b.get_device() == dev))

@@ -9,8 +9,8 @@ convolutional blocks, for networks that normalise each row by itself.
                     small one that adds those in a fixed order
 
 float32, bfloat16 and float16 on a HIP device, parameters of the same type or float32, any width. Inputs that are not contiguous are
-copied first. Anything else - host tensors, other types, autocast, empty tensors, a subclass with a forward of its own, hooks on
-`ln` - takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward raises. On a HIP tensor
+copied first. Anything else - host tensors, other types, autocast, empty tensors, a class or an instance with a forward of its own, hooks on
+`ln` or on all modules - takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward raises. On a HIP tensor
 the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the normalised input in 8 bits for the backward pass (K17, `act8`): gradients are the formula's with xhat
@@ -22,6 +22,7 @@ import os
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import _native
 
@@ -40,7 +41,7 @@ def enabled(flag=None):
 def _fusable(ln, w, b, x):
     t, dev, shape = x.dtype, x.get_device(), ln.normalized_shape
     return (_on and x.is_cuda and t in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
-            and type(ln).forward is nn.LayerNorm.forward
+            and type(ln).forward is nn.LayerNorm.forward and 'forward' not in ln.__dict__ and not _has_any_global_hook()
             and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks or ln._backward_pre_hooks)
             and x.shape[-len(shape):] == shape and ln.eps >= 0
             and (w is None or (w.get_device() == dev and (w.dtype is t or w.dtype is torch.float32)))
