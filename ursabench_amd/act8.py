@@ -7,7 +7,7 @@ infinity or a NaN in it comes back as NaN. 1.03 bytes a value instead of 4 (fp32
 
 `fused_linear.linear_act(..., save8=True)` and `fused_norm.layer_norm(..., save8=True)` keep their inputs so and read them in this form
 in their backward launches; `pack` / `unpack` are for what else a program wants to keep. HIP tensors of float32, bfloat16 or float16
-(no CPU path: a host tensor raises); not differentiable.
+(no CPU path: a host tensor raises; so does a wrapped one, inside transforms, dispatch modes and tracing); not differentiable.
 """
 from typing import NamedTuple
 

@@ -5,9 +5,12 @@
 // backward pass needs.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/ursa_hip.h"
@@ -53,6 +56,28 @@ Tensor kept(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const T
 }
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// Whether a tensor is its memory and no more: not the wrapper of a function transform or of a dispatching subclass, nor a dual tensor,
+// whose tangent a launch would drop.
+bool memory(const Tensor& t) {
+    return !t.defined() || (t.has_storage() && !t.key_set().has(c10::DispatchKey::Python) && !t._fw_grad(0).defined());
+}
+
+// Whether a launch on the operands' memory is all that a call is to torch: not inside a function transform (vmap, grad, jvp), under a
+// dispatch mode (fake tensors, tracing to a graph, counters) or torch.jit.trace, all of which see operators only.
+bool plain(std::initializer_list<const Tensor*> operands) {
+    if (c10::impl::tls_local_dispatch_key_set().included_.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) ||
+        c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing()) return false;
+    for (const Tensor* t : operands)
+        if (!memory(*t)) return false;
+    return true;
+}
+
+void only_memory(const variable_list& grads) {
+    for (const auto& g : grads)
+        TORCH_CHECK(memory(g), "ursabench_amd: batched (is_grads_batched) and dual gradients are not offered in the backward pass; "
+                               "fused_linear.enabled(False) / fused_norm.enabled(False) before the forward pass select the stock ops");
+}
 
 // x as rows of `width`
 Tensor rows_of(const Tensor& x, int64_t width) { return (x.dim() == 2 && x.size(1) == width ? x : x.reshape({width ? x.numel() / width : 0, width})).contiguous(); }
@@ -130,6 +155,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        only_memory(grads);
         const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const int64_t needs = ctx->saved_data["needs"].toInt(), act = ctx->saved_data["act"].toInt();
@@ -160,8 +186,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     }
 };
 
-Tensor linear_act(const Tensor& x, const Tensor& w, const Maybe& b_, const Maybe& r_, int64_t act, bool save8) {
+// None where the call is the stock ops' (plain)
+Maybe linear_act(const Tensor& x, const Tensor& w, const Maybe& b_, const Maybe& r_, int64_t act, bool save8) {
     const Tensor b = given(b_), r = given(r_);
+    if (!plain({&x, &w, &b, &r})) return {};
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) return LinearAct::apply(x, w, b_, r_, act, save8);
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = w.size(0);
@@ -232,6 +260,7 @@ struct Norm : torch::autograd::Function<Norm> {
         return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        only_memory(grads);
         const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const int64_t needs = ctx->saved_data["needs"].toInt();
@@ -251,6 +280,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         return {o.z, o.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        only_memory(grads);
         const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const int64_t needs = ctx->saved_data["needs"].toInt();
@@ -274,21 +304,31 @@ bool recorded(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b
     return at::GradMode::is_enabled() && (wants(x) || wants(r) || wants(w) || wants(b));
 }
 
-Tensor layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, int64_t width, double eps, bool save8) {
-    if (recorded(x, Tensor(), given(w), given(b))) return Norm::apply(x, w, b, width, eps, save8);
-    return norm_forward(rows_of(x, width), Tensor(), given(w), given(b), eps, x.sizes(), false, false).y;
+// None where the call is the stock ops' (plain)
+Maybe layer_norm(const Tensor& x, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
+    const Tensor w = given(w_), b = given(b_);
+    if (!plain({&x, &w, &b})) return {};
+    if (recorded(x, Tensor(), w, b)) return Norm::apply(x, w_, b_, width, eps, save8);
+    return norm_forward(rows_of(x, width), Tensor(), w, b, eps, x.sizes(), false, false).y;
 }
 
-std::pair<Tensor, Tensor> add_layer_norm(const Tensor& a, const Tensor& r, const Maybe& w, const Maybe& b, int64_t width, double eps, bool save8) {
-    if (recorded(a, r, given(w), given(b))) {
-        auto out = AddNorm::apply(a, r, w, b, width, eps, save8);
-        return {out[0], out[1]};
+std::optional<std::pair<Tensor, Tensor>> add_layer_norm(const Tensor& a, const Tensor& r, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
+    const Tensor w = given(w_), b = given(b_);
+    if (!plain({&a, &r, &w, &b})) return {};
+    if (recorded(a, r, w, b)) {
+        auto out = AddNorm::apply(a, r, w_, b_, width, eps, save8);
+        return std::make_pair(out[0], out[1]);
     }
-    const NormOut o = norm_forward(rows_of(a, width), rows_of(r, width), given(w), given(b), eps, a.sizes(), false, false);
-    return {o.z, o.y};
+    const NormOut o = norm_forward(rows_of(a, width), rows_of(r, width), w, b, eps, a.sizes(), false, false);
+    return std::make_pair(o.z, o.y);
+}
+
+void only_plain(std::initializer_list<const Tensor*> operands, const char* what) {
+    TORCH_CHECK_VALUE(plain(operands), what, ": a plain tensor wanted, outside of function transforms, dispatch modes and tracing");
 }
 
 std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
+    only_plain({&x}, "act8.pack");
     at::NoGradGuard no_grad;
     const int64_t D = x.size(-1);
     const Tensor x2 = rows_of(x, D);
@@ -300,6 +340,7 @@ std::pair<Tensor, Tensor> act8_pack(const Tensor& x) {
 
 // q, e: contiguous, of `shape`'s rows and features
 Tensor act8_unpack(const Tensor& q, const Tensor& e, const std::vector<int64_t>& shape, const Tensor& like) {
+    only_plain({&q, &e}, "act8.unpack");
     const c10::DeviceGuard guard(q.device());
     Tensor x = at::empty(shape, like.options().device(q.device()));
     ok(ursa_act8_unpack((const int8_t*)at_(q), (const int8_t*)at_(e), at_(x), q.size(0), shape.back(), type_of(x), stream_of(q)), "ursa_act8_unpack");

@@ -9,8 +9,8 @@ launches differ:
 
 float32, bfloat16 and float16, any sizes and leading dimensions, on a HIP device. Operands that are not contiguous are copied first.
 Anything else - host tensors, other or mixed types, autocast, a class or an instance with a forward of its own, hooks on `fc` or on
-all modules - takes `fc(x)`, the activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises. On a HIP tensor
-the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
+all modules, tensor subclasses, `torch.func` transforms, forward-mode derivatives, dispatch modes and tracing - takes `fc(x)`, the
+activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises. On a HIP tensor the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the x that the weight gradient needs in 8 bits (K17, `act8`) instead of the tensor: a quarter / half of its
 memory, dW as if x had been rounded to 8 bits per block of 32 features; y, dx and db do not change.
@@ -32,6 +32,7 @@ from . import _native
 
 _on = os.environ.get('URSA_FUSED_LINEAR', '1') != '0'
 _models = os.environ.get('URSA_LINEAR_IN_MODELS', '0') == '1'
+_TENSORS = frozenset((torch.Tensor, nn.Parameter, type(None)))       # a subclass may have a meaning of its own for every operator
 _STOCK = {None: lambda z: z, 'relu': F.relu, 'gelu': F.gelu, 'silu': F.silu}
 
 
@@ -58,7 +59,7 @@ def _fusable(fc, w, b, x, residual):
     return (_on and x.is_cuda and t in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
             and type(fc).forward is nn.Linear.forward and 'forward' not in fc.__dict__ and not _has_any_global_hook()
             and not (fc._forward_hooks or fc._forward_pre_hooks or fc._backward_hooks or fc._backward_pre_hooks)
-            and w.dtype is t and w.get_device() == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
+            and type(x) in _TENSORS and type(w) in _TENSORS and type(residual) in _TENSORS and w.dtype is t and w.get_device() == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
             and (b is None or (b.dtype is t and b.get_device() == dev))
             and (residual is None or (residual.dtype is t and residual.get_device() == dev)))
 
@@ -76,7 +77,9 @@ def linear_act(fc, x, activation=None, residual=None, *, save8=False):
     shape = x.shape[:-1] + (w.shape[0],)
     if residual is not None and residual.shape != shape:
         raise ValueError(f'residual {tuple(residual.shape)} should have the result\'s shape {tuple(shape)}')
-    if not _fusable(fc, w, b, x, residual):
-        y = _STOCK[activation](fc(x))
-        return y if residual is None else y + residual
-    return _native.nodes().linear_act(x, w, b, residual, _native.ACTIVATIONS[activation], save8)
+    if _fusable(fc, w, b, x, residual):
+        y = _native.nodes().linear_act(x, w, b, residual, _native.ACTIVATIONS[activation], save8)
+        if y is not None:                                 # (None: the operands are more than memory to torch)
+            return y
+    y = _STOCK[activation](fc(x))
+    return y if residual is None else y + residual

@@ -10,7 +10,7 @@ convolutional blocks, for networks that normalise each row by itself.
 
 float32, bfloat16 and float16 on a HIP device, parameters of the same type or float32, any width. Inputs that are not contiguous are
 copied first. Anything else - host tensors, other types, autocast, empty tensors, a class or an instance with a forward of its own, hooks on
-`ln` or on all modules - takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward raises. On a HIP tensor
+`ln` or on all modules, tensor subclasses, `torch.func` transforms, forward-mode derivatives, dispatch modes and tracing - takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward raises. On a HIP tensor
 the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the normalised input in 8 bits for the backward pass (K17, `act8`): gradients are the formula's with xhat
@@ -26,6 +26,7 @@ from torch.nn.modules.module import _has_any_global_hook
 
 from . import _native
 
+_TENSORS = frozenset((torch.Tensor, nn.Parameter, type(None)))       # a subclass may have a meaning of its own for every operator
 _on = os.environ.get('URSA_FUSED_NORM', '1') != '0'
 
 
@@ -43,7 +44,7 @@ def _fusable(ln, w, b, x):
     return (_on and x.is_cuda and t in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
             and type(ln).forward is nn.LayerNorm.forward and 'forward' not in ln.__dict__ and not _has_any_global_hook()
             and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks or ln._backward_pre_hooks)
-            and x.shape[-len(shape):] == shape and ln.eps >= 0
+            and type(x) in _TENSORS and type(w) in _TENSORS and x.shape[-len(shape):] == shape and ln.eps >= 0
             and (w is None or (w.get_device() == dev and (w.dtype is t or w.dtype is torch.float32)))
             and (b is None or (b.get_device() == dev and (b.dtype is t or b.dtype is torch.float32) and (w is None or w.dtype is b.dtype))))
 
@@ -62,9 +63,10 @@ def layer_norm(ln, x, *, save8=False):
     if not isinstance(ln, nn.LayerNorm):
         raise TypeError(f'layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
     w, b = _params(ln)
-    if not _fusable(ln, w, b, x):
-        return ln(x)
-    return _native.nodes().layer_norm(x, _flat(w), _flat(b), math.prod(ln.normalized_shape), ln.eps, save8)
+    y = None
+    if _fusable(ln, w, b, x):
+        y = _native.nodes().layer_norm(x, _flat(w), _flat(b), math.prod(ln.normalized_shape), ln.eps, save8)
+    return ln(x) if y is None else y                      # (None from there: the operands are more than memory to torch)
 
 
 def add_layer_norm(ln, x, *, save8=False):
@@ -76,7 +78,9 @@ def add_layer_norm(ln, x, *, save8=False):
         raise TypeError(f'add_layer_norm wants an nn.LayerNorm, got {type(ln).__name__}')
     a, b = x
     w, bias = _params(ln)
-    if not (_fusable(ln, w, bias, a) and b.shape == a.shape and b.dtype is a.dtype and b.device == a.device):
-        z = a + b
-        return z, layer_norm(ln, z, save8=save8)
-    return _native.nodes().add_layer_norm(a, b, _flat(w), _flat(bias), math.prod(ln.normalized_shape), ln.eps, save8)
+    if _fusable(ln, w, bias, a) and b.shape == a.shape and b.dtype is a.dtype and b.device == a.device and type(b) in _TENSORS:
+        pair = _native.nodes().add_layer_norm(a, b, _flat(w), _flat(bias), math.prod(ln.normalized_shape), ln.eps, save8)
+        if pair is not None:
+            return pair
+    z = a + b
+    return z, layer_norm(ln, z, save8=save8)
