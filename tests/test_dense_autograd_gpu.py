@@ -106,3 +106,68 @@ def test_saved_tensors_that_are_not_what_was_saved_raise(unpack, op, save8):
         y = f(x, s=save8)
     with pytest.raises((RuntimeError, ValueError), match='saved'):
         torch.autograd.grad(y, [x, mod.weight, mod.bias], torch.randn(9, 40, device=DEV))
+
+
+# ---- one gradient of several: the others are neither computed nor allocated ---------------------
+@pytest.mark.parametrize('save8', [False, True])
+@pytest.mark.parametrize('bias,residual', list(itertools.product([False, True], repeat=2)))
+def test_every_choice_of_gradients_of_a_trainable_layer(bias, residual, save8):
+    from ursabench_amd.fused_linear import linear_act
+    torch.manual_seed(1)
+    fc = nn.Linear(48, 40, bias=bias, device=DEV)
+    x = torch.randn(33, 48, device=DEV, requires_grad=True)
+    r = torch.randn(33, 40, device=DEV, requires_grad=True) if residual else None
+    dy = torch.randn(33, 40, device=DEV)
+    leaves = [t for t in (x, fc.weight, fc.bias, r) if t is not None]
+    full = torch.autograd.grad(linear_act(fc, x, 'gelu', r, save8=save8), leaves, dy)
+    for n in range(1, len(leaves) + 1):
+        for some in itertools.combinations(range(len(leaves)), n):
+            got = torch.autograd.grad(linear_act(fc, x, 'gelu', r, save8=save8), [leaves[i] for i in some], dy)
+            assert all(torch.equal(a, full[i]) for a, i in zip(got, some)), some
+            linear_act(fc, x, 'gelu', r, save8=save8).backward(dy, inputs=[leaves[i] for i in some])
+            for i, t in enumerate(leaves):
+                assert (t.grad is not None) == (i in some) and (t.grad is None or torch.equal(t.grad, full[i])), (some, i)
+                t.grad = None
+
+
+@pytest.mark.parametrize('save8', [False, True])
+@pytest.mark.parametrize('add', [False, True])
+@pytest.mark.parametrize('affine', ['none', 'weight', 'both'])
+def test_every_choice_of_gradients_of_a_trainable_norm(affine, add, save8):
+    from ursabench_amd.fused_norm import add_layer_norm, layer_norm
+    torch.manual_seed(2)
+    ln = nn.LayerNorm(100, elementwise_affine=affine != 'none', bias=affine == 'both', device=DEV)
+    x, r, dy = (torch.randn(21, 100, device=DEV) for _ in range(3))
+    x.requires_grad_(), r.requires_grad_()
+    leaves = [t for t in (x, r if add else None, ln.weight, ln.bias) if t is not None]
+    f = lambda: add_layer_norm(ln, (x, r), save8=save8) if add else (layer_norm(ln, x, save8=save8),)      # noqa: E731
+    for outs, dys in (((0, 1), (dy, 2 * dy)), ((1,), (dy,))) if add else (((0,), (dy,)),):
+        y = lambda: [f()[o] for o in outs]                                                                # noqa: E731
+        full = torch.autograd.grad(y(), leaves, dys)
+        for n in range(1, len(leaves) + 1):
+            for some in itertools.combinations(range(len(leaves)), n):
+                got = torch.autograd.grad(y(), [leaves[i] for i in some], dys)
+                assert all(torch.equal(a, full[i]) for a, i in zip(got, some)), some
+
+
+def _peak(f):
+    f()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    f()
+    return torch.cuda.max_memory_allocated() - before
+
+
+def test_memory_of_one_gradient():
+    """dx of a trainable 4096 x 4096 layer: no room for its dW (64 MiB); dx of a trainable norm: no room for the partial sums."""
+    from ursabench_amd.fused_linear import linear_act
+    from ursabench_amd.fused_norm import layer_norm
+    fc, x = nn.Linear(4096, 4096, device=DEV), torch.randn(64, 4096, device=DEV, requires_grad=True)
+    y, dy = linear_act(fc, x), torch.ones(64, 4096, device=DEV)
+    assert _peak(lambda: torch.autograd.grad(y, x, dy, retain_graph=True)) < 4 * fc.weight.numel() <= _peak(
+        lambda: torch.autograd.grad(y, (x, fc.weight), dy, retain_graph=True))
+    ln = nn.LayerNorm(4096, device=DEV)
+    y = layer_norm(ln, x)
+    assert _peak(lambda: torch.autograd.grad(y, x, dy, retain_graph=True)) == 4 * x.numel()
+    assert _peak(lambda: torch.autograd.grad(y, ln.weight, dy, retain_graph=True)) < 4 * x.numel()         # no room for dx

@@ -130,6 +130,13 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
     return y;
 }
 
+// Which of a node's gradients this backward pass wants. `given`: bit i is set where operand i was a tensor; autograd numbers those.
+struct Wanted {
+    const AutogradContext* ctx;
+    int64_t given;
+    bool operator()(int i) const { return given >> i & 1 && ctx->needs_input_grad(__builtin_popcountll(given & ((1ll << i) - 1))); }
+};
+
 struct LinearAct : torch::autograd::Function<LinearAct> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b_, const Maybe& r_, int64_t act, bool save8) {
         const Tensor b = given(b_), r = given(r_);
@@ -149,7 +156,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         }
         ctx->save_for_backward({nw && !save8 ? x2 : Tensor(), nx ? wc : Tensor(), z, p.q, p.e});
         ctx->saved_data["act"] = act;
-        ctx->saved_data["needs"] = (int64_t)(nx + 2 * nw + 4 * nb + 8 * wants(r));
+        ctx->saved_data["given"] = (int64_t)(3 + 4 * b.defined() + 8 * r.defined());
         ctx->saved_data["x"] = x.sizes().vec();
         return y;
     }
@@ -158,8 +165,9 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         only_memory(grads);
         const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
-        const int64_t needs = ctx->saved_data["needs"].toInt(), act = ctx->saved_data["act"].toInt();
-        const bool nx = needs & 1, nw = needs & 2, nb = needs & 4;
+        const int64_t act = ctx->saved_data["act"].toInt();
+        const Wanted wanted{ctx, ctx->saved_data["given"].toInt()};
+        const bool nx = wanted(0), nw = wanted(1), nb = wanted(2);
         const auto saved = ctx->get_saved_variables();
         const Tensor& dy_ = grads[0];
         variable_list out(6);
@@ -172,8 +180,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             const int32_t dt = type_of(dy);
             const at::ScalarType t = dy.scalar_type();
             const int64_t blocks = (K + 31) / 32;
-            const Tensor x = kept(saved[0], {M, K}, t, dy), w = kept(saved[1], {N, K}, t, dy), z = kept(saved[2], {M, N}, t, dy),
-                         q = kept(saved[3], {M, 32 * blocks}, at::kChar, dy), e = kept(saved[4], {M, blocks}, at::kChar, dy);
+            Tensor x, w, q, e;
+            const Tensor z = kept(saved[2], {M, N}, t, dy);
+            if (nx) w = kept(saved[1], {N, K}, t, dy);
+            if (nw) x = kept(saved[0], {M, K}, t, dy), q = kept(saved[3], {M, 32 * blocks}, at::kChar, dy), e = kept(saved[4], {M, blocks}, at::kChar, dy);
             if (nx) out[0] = at::empty(shape, dy.options());
             if (nw) out[1] = at::empty({N, K}, dy.options());
             if (nb) out[2] = at::empty({N}, dy.options());
@@ -181,7 +191,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             ok(ursa_linear_bwd(at_(dy), at_(x), (const int8_t*)at_(q), (const int8_t*)at_(e), at_(w), at_(z), at_(out[0]), at_(out[1]), at_(out[2]), at_(ws), M,
                                N, K, dt, (int32_t)act, stream_of(dy)), "ursa_linear_bwd");
         }
-        if (needs & 8) out[3] = dy_;
+        if (wanted(3)) out[3] = dy_;
         return once(std::move(out), grads, create_graph);
     }
 };
@@ -216,9 +226,9 @@ NormOut norm_forward(const Tensor& x, const Tensor& r, const Tensor& w, const Te
 }
 
 // z: what was normalised, in any shape (of an output: that tensor itself, so that changes in place are noticed)
-void norm_keep(AutogradContext* ctx, const Tensor& z, const NormOut& o, const Tensor& w, const Tensor& b, const Tensor& x, int64_t width, int64_t needs, bool save8) {
+void norm_keep(AutogradContext* ctx, const Tensor& z, const NormOut& o, const Tensor& w, const Tensor& b, const Tensor& x, int64_t width, int64_t given, bool save8) {
     ctx->save_for_backward({save8 ? Tensor() : z, o.q, o.e, o.stats, w});
-    ctx->saved_data["needs"] = needs;
+    ctx->saved_data["given"] = given;
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->saved_data["kept"] = z.sizes().vec();
     ctx->saved_data["width"] = width;
@@ -252,19 +262,18 @@ std::array<Tensor, 3> norm_backward(AutogradContext* ctx, const Tensor& dy_, con
 struct Norm : torch::autograd::Function<Norm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
         const Tensor w = given(w_), b = given(b_);
-        const int64_t needs = wants(x) + 2 * wants(w) + 4 * wants(b);
         at::NoGradGuard no_grad;
         const Tensor x2 = rows_of(x, width);
         const NormOut o = norm_forward(x2, Tensor(), w, b, eps, x.sizes(), true, save8);
-        norm_keep(ctx, x2, o, w, b, x, width, needs, save8);
+        norm_keep(ctx, x2, o, w, b, x, width, 1 + 2 * w.defined() + 4 * b.defined(), save8);
         return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         only_memory(grads);
         const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
-        const int64_t needs = ctx->saved_data["needs"].toInt();
-        const auto g = norm_backward(ctx, grads[0], Tensor(), needs & 1, needs & 2, needs & 4);
+        const Wanted wanted{ctx, ctx->saved_data["given"].toInt()};
+        const auto g = norm_backward(ctx, grads[0], Tensor(), wanted(0), wanted(1), wanted(2));
         return once({g[0], g[1], g[2], Tensor(), Tensor(), Tensor()}, grads, create_graph);
     }
 };
@@ -272,19 +281,18 @@ struct Norm : torch::autograd::Function<Norm> {
 struct AddNorm : torch::autograd::Function<AddNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& a, const Tensor& r, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
         const Tensor w = given(w_), b = given(b_);
-        const int64_t needs = wants(a) + 2 * wants(w) + 4 * wants(b) + 8 * wants(r);
         at::NoGradGuard no_grad;
         ctx->set_materialize_grads(false);                     // an unused output's gradient arrives undefined, not as zeros
         const NormOut o = norm_forward(rows_of(a, width), rows_of(r, width), w, b, eps, a.sizes(), true, save8);
-        norm_keep(ctx, o.z, o, w, b, a, width, needs, save8);
+        norm_keep(ctx, o.z, o, w, b, a, width, 3 + 4 * w.defined() + 8 * b.defined(), save8);
         return {o.z, o.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         only_memory(grads);
         const bool create_graph = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
-        const int64_t needs = ctx->saved_data["needs"].toInt();
-        const bool na = needs & 1, nr = needs & 8;
+        const Wanted wanted{ctx, ctx->saved_data["given"].toInt()};
+        const bool na = wanted(0), nr = wanted(1);
         variable_list out(7);
         const Tensor &dz = grads[0], &dy = grads[1];
         if (!dy.defined()) {                                   // y unused: only the sum's own gradient flows
@@ -292,7 +300,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
             if (nr) out[1] = dz;
             return once(std::move(out), grads, create_graph);
         }
-        const auto g = norm_backward(ctx, dy, dz, na || nr, needs & 2, needs & 4);
+        const auto g = norm_backward(ctx, dy, dz, na || nr, wanted(2), wanted(3));
         if (na) out[0] = g[0];
         if (nr) out[1] = g[0];
         out[2] = g[1], out[3] = g[2];
