@@ -281,10 +281,12 @@ struct Norm : torch::autograd::Function<Norm> {
 struct AddNorm : torch::autograd::Function<AddNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& a, const Tensor& r, const Maybe& w_, const Maybe& b_, int64_t width, double eps, bool save8) {
         const Tensor w = given(w_), b = given(b_);
+        const bool constant = !wants(a) && !wants(r);
         at::NoGradGuard no_grad;
         ctx->set_materialize_grads(false);                     // an unused output's gradient arrives undefined, not as zeros
         const NormOut o = norm_forward(rows_of(a, width), rows_of(r, width), w, b, eps, a.sizes(), true, save8);
         norm_keep(ctx, o.z, o, w, b, a, width, 3 + 4 * w.defined() + 8 * b.defined(), save8);
+        if (constant) ctx->mark_non_differentiable({o.z});     // as the stock sum: only y depends on what needs a gradient
         return {o.z, o.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
