@@ -191,3 +191,28 @@ def test_the_sum_of_constants_stays_one():
     z.add_(1)                                            # what the backward pass needs has changed
     with pytest.raises(RuntimeError, match='modified by an inplace'):
         y.sum().backward()
+
+
+def test_relu_lets_a_gradient_pass_where_its_input_is_nan():
+    """As the stock op: the gate is shut where z <= 0, and a NaN is not. (A gradient that is NaN itself is not hidden behind a zero.)"""
+    from ursabench_amd.fused_linear import linear_act
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for M in (3, 100):
+            fc = nn.Linear(40, 24, device=DEV, dtype=dtype)
+            x = torch.randn(M, 40, device=DEV, dtype=dtype)
+            x[1, 5] = float('nan')
+            x.requires_grad_()
+            dy = torch.randn(M, 24, device=DEV, dtype=dtype)
+            y = linear_act(fc, x, 'relu')
+            assert y[1].isnan().all()
+            dx, db = torch.autograd.grad(y, (x, fc.bias), dy)
+            z = fc(x).detach()
+            want = torch.autograd.grad(torch.relu(z.requires_grad_()), z, dy)[0]
+            assert torch.equal(want[1], dy[1])
+            err = (24 + 2) * 2.0 ** -24 * (dy[1].double().abs() @ fc.weight.double().abs())
+            exact = dy[1].double() @ fc.weight.double()
+            # dz = dy exactly in that row; one rounding of the result
+            assert ((dx[1].double() - exact).abs() <= err + 2.0 ** -24 * 8 * exact.abs() + torch.finfo(dtype).eps / 2 * exact.abs()).all()
+            dy[1] = float('nan')
+            dx, db = torch.autograd.grad(linear_act(fc, x, 'relu'), (x, fc.bias), dy)
+            assert dx[1].isnan().all() and db.isnan().all() and dx[0].isfinite().all() and dx[2:].isfinite().all()

@@ -93,7 +93,7 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
         }
     } else if (act == URSA_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : 0.f;
+        for (int i = 0; i < N; ++i) g[i] = z[i] <= 0.f ? 0.f : g[i];             // shut where z <= 0: open for a NaN, as the stock op's
     }
 }
 
