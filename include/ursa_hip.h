@@ -662,7 +662,8 @@ int ursa_linear_bwd(const void* dy, const void* x /* or NULL */, const int8_t* q
  *   together: z_out is the sum rounded to the type, and what is normalised. mean, rstd [M] fp32 or both NULL. q, e (K17) or both
  *   NULL: the 8-bit form of z, written in the same pass, from which ursa_layer_norm_bwd can take xhat instead of x.
  *   backward: dx (or NULL) = d(loss)/dz + dz (dz: the gradient that reaches z by another way, or NULL); dgamma, dbeta [D] (or NULL).
- *   x: what was normalised (z_out if there was an addend). ws: ursa_layer_norm_ws_floats(M, D) floats when dgamma or dbeta is given.
+ *   x: what was normalised (z_out if there was an addend). ws: ursa_layer_norm_ws_floats(M, D) floats when dgamma or dbeta is given (0:
+ *   may be NULL); at most 32 MiB.
  *   M = 0 with dgamma or dbeta: URSA_EVALUE. Statistics and sums are fp32, summed in a fixed order. D at most 2^27.
  */
 int64_t ursa_layer_norm_ws_floats(int64_t M, int64_t D);

@@ -12,6 +12,12 @@ DEV = 'cuda'
 INF, NAN = math.inf, math.nan
 
 
+def _unpacked(x):
+    """The 8-bit form's values, by the host: its powers of two are exact (the device's fp64 pow is off by a rounding for some, which
+    breaks ties the other way)."""
+    return B.unpacked(x.cpu()).to(DEV)
+
+
 # ---- fp32 sums past the range -------------------------------------------------------------------
 # Every form of the fp32 product: (M, K, N) whose forward is 64 x 64 tiles, 64 x 64 with the contraction cut, 128 x 128 (rows that the
 # large form does not take), the large form, the large form with the contraction cut; and, for comparison, up to 64 rows.
@@ -65,7 +71,7 @@ def test_fp32_sums_past_the_range_with_the_input_in_8_bits(M, K, N):
     k = _native.default_kernels()
     x, w, _ = _signed(M, K, N)
     q, e = k.act8_pack(w.t().contiguous())                                  # dw [M, N] = x (as dy' [K, M]) times the kept [K, N]
-    kept = B.unpacked(w.t().contiguous())
+    kept = _unpacked(w.t())
     got = k.linear_backward(x.t().contiguous(), None, None, q=q, e=e, in_features=N, need_dx=False, need_db=False)[1]
     _agrees(got, x.double() @ kept, K)
 
@@ -201,3 +207,30 @@ def test_a_constant_gradient_moves_nothing(D):
     assert torch.equal(stats[0], x[:, 0])
     dx, dg, _ = k.layer_norm_backward(dy, stats, x=x, need_dgamma=True)
     assert not dx.any() and not dg.any()
+
+
+# ---- rows of a million features -----------------------------------------------------------------
+@pytest.mark.parametrize('dtype,M,D', [('float32', 3, 16385), ('bfloat16', 4, 20000), ('bfloat16', 40, 70001), ('float32', 9, 2 ** 20 + 5), ('float16', 40, 2 ** 20 + 5),
+                                       ('bfloat16', 6, 4500001), ('float32', 2, 4500000)])
+def test_column_sums_of_long_rows(dtype, M, D):
+    """One slice of the rows (no scratch), few and many: dgamma and dbeta, together and each alone, from x and from its 8-bit form."""
+    from ursabench_amd import _native
+    k, t = _native.default_kernels(), B.TYPES[dtype]
+    g = torch.Generator(device=DEV).manual_seed(D)
+    x, dy = (torch.randn(M, D, generator=g, device=DEV).to(t) for _ in range(2))
+    for pt in {t, torch.float32}:
+        gamma = torch.ones(D, device=DEV, dtype=pt)
+        _, _, stats, q, e = k.layer_norm(x, gamma, eps=1e-5, stats=True, save8=True)
+        for kept, source in ((None, dict(x=x)), (_unpacked(x), dict(q=q, e=e))):
+            Z, DY = x.double(), dy.double()
+            mean, var = Z.mean(1, keepdim=True), Z.var(1, unbiased=False, keepdim=True)
+            xhat = ((Z if kept is None else kept) - mean) / torch.sqrt(var + 1e-5)
+            n = 64 + 2 * D / 8192
+            exh = n * B.F * (xhat.abs() * 2 + 2)                                 # |mean| and the deviation's roundings are below one each
+            want = dict(dg=(DY * xhat).sum(0), db=DY.sum(0))
+            bound = dict(dg=(DY.abs() * exh).sum(0) + (M + 16) * B.F * (DY * xhat).abs().sum(0) + B.last_rounding(want['dg'], pt),
+                         db=(M + 16) * B.F * DY.abs().sum(0) + B.last_rounding(want['db'], pt))
+            _, dg, db = k.layer_norm_backward(dy, stats, gamma, need_dx=False, need_dgamma=True, need_dbeta=True, **source)
+            B.check(dict(dg=dg, db=db), want, bound, where=(dtype, M, D, pt))
+            assert torch.equal(k.layer_norm_backward(dy, stats, gamma, need_dx=False, need_dgamma=True, **source)[1], dg)
+            assert torch.equal(k.layer_norm_backward(dy, stats, gamma, need_dx=False, need_dbeta=True, **source)[2], db)

@@ -15,7 +15,9 @@
 // per thread. dgamma / dbeta: a workgroup walks rows with a fixed stride and keeps its columns' sums in registers, stores them
 // once, and a second launch adds the workgroups' sums in a fixed order - no atomics, the same bits every time.
 // 16,384 x 4,096 bf16: the sum and its norm 107 us (537 MB, 5.0 TB/s), backward with a gradient past the norm 125 us (4.3 TB/s; a
-// large copy moves 4.8). One row of any width: the launch, 5 us.
+// large copy moves 4.8). One row: the launch, 5 us up to 16,384 features. A longer one does not fit a workgroup's registers and is
+// walked three times (twice) by one workgroup: 20,000 features 12 us forward and 21 backward, 2^20 417 and 707; 512 rows of 2^17
+// bf16 121 and 290 us (dgamma / dbeta 82 of them).
 #include "ursa_ops.h"
 
 namespace {
@@ -402,9 +404,9 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwd<T, P> a) {
     }
 }
 
-// dgamma / dbeta of long rows: a thread owns V columns and walks the rows of its slice (gridDim.y of them)
+// dgamma / dbeta of long rows: a thread owns V columns and walks the rows of its slice (gridDim.y of them; one: nothing to add up)
 template <typename T, typename P>
-__global__ __launch_bounds__(256) void k_norm_columns_long(NormBwd<T, P> a) {
+__global__ __launch_bounds__(256) void k_norm_columns_long(NormBwd<T, P> a, P* __restrict__ dgamma, P* __restrict__ dbeta) {
     constexpr int V = Piece<T>::kN;
     const int64_t d = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (d >= a.D) return;
@@ -418,6 +420,11 @@ __global__ __launch_bounds__(256) void k_norm_columns_long(NormBwd<T, P> a) {
         const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
         for (int i = 0; i < V; ++i) dg[i] += t[i] * ((xh[i] - mean) * rstd), db[i] += t[i];
+    }
+    if (gridDim.y == 1) {
+        if (dgamma) store_piece<P, V>(dgamma + d, left, dg);
+        if (dbeta) store_piece<P, V>(dbeta + d, left, db);
+        return;
     }
     float* out = a.partial + (int64_t)blockIdx.y * 2 * a.D;
     store_piece<float, V>(out + d, left, dg);
@@ -486,9 +493,13 @@ dim3 grid_of(int64_t blocks) {
 int bwd_row_threads(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 
 // Workgroups of the walk: 1,024 threads a CU, and no more than leave each row slot four rows, so that the partial sums (2 D floats
-// a workgroup: 16 MiB at most) stay small beside the rows
+// a workgroup: 16 MiB at most up to 8,192 features, 32 MiB above) stay small beside the rows. Long rows: slices of the columns' walk,
+// which has a workgroup for every 4 KiB of a row already: 64 at most, four rows each, and within the same 32 MiB - one above 2^21 features.
 int64_t bwd_groups(int64_t M, int64_t D) {
-    if (D > kLong) return M < 64 ? M : 64;
+    if (D > kLong) {
+        const int64_t rows = (M + 3) / 4, room = (32 << 20) / (8 * D), n = rows < room ? rows : room;
+        return n < 1 ? 1 : n < 64 ? n : 64;
+    }
     const int64_t tpr = bwd_row_threads(D), threads = bwd_threads((int)tpr), R = threads / tpr, most = 256 * 1024 / threads, need = (M + 4 * R - 1) / (4 * R);
     return need < most ? need : most;
 }
@@ -518,7 +529,9 @@ int norm_bwd(const NormBwd<T, P>& a, P* dgamma, P* dbeta, hipStream_t s) {
     if (D > kLong) {
         if (a.dx) hipLaunchKernelGGL((k_norm_bwd_long<T, P>), grid_of(a.M), dim3(1024), 0, s, a);
         if ((rc = launch_status())) return rc;
-        if (a.partial) hipLaunchKernelGGL((k_norm_columns_long<T, P>), dim3((unsigned)((D + 256 * Piece<T>::kN - 1) / (256 * Piece<T>::kN)), groups), dim3(256), 0, s, a);
+        if (!dgamma && !dbeta) return rc;
+        hipLaunchKernelGGL((k_norm_columns_long<T, P>), dim3((unsigned)((D + 256 * Piece<T>::kN - 1) / (256 * Piece<T>::kN)), groups), dim3(256), 0, s, a, dgamma, dbeta);
+        if (groups == 1) return launch_status();
     } else {
         void (*fn)(NormBwd<T, P>) = a.q ? (a.dz ? norm_bwd_for<T, P, true, true>(D) : norm_bwd_for<T, P, true, false>(D))
                                         : (a.dz ? norm_bwd_for<T, P, false, true>(D) : norm_bwd_for<T, P, false, false>(D));
@@ -546,7 +559,8 @@ int sizes_ok(int64_t M, int64_t D) {
 
 extern "C" int64_t ursa_layer_norm_ws_floats(int64_t M, int64_t D) {
     if (sizes_ok(M, D) || M == 0) return 0;
-    return bwd_groups(M, D) * 2 * D;
+    const int64_t n = bwd_groups(M, D);
+    return D > kLong && n == 1 ? 0 : n * 2 * D;
 }
 
 extern "C" int ursa_layer_norm_fwd(const void* x, const void* addend, void* z_out, void* y, const void* gamma, const void* beta, float* mean,
@@ -571,7 +585,7 @@ extern "C" int ursa_layer_norm_bwd(const void* x, const int8_t* q, const int8_t*
     if (bad_dtype(dtype) || (pdtype != dtype && pdtype != URSA_F32)) return URSA_EFLAGS;
     if (int rc = sizes_ok(M, D)) return rc;
     if (M == 0 || D == 0) return M == 0 && D && (dgamma || dbeta) ? URSA_EVALUE : URSA_OK;     // no rows: the caller's zeros
-    if ((x != nullptr) == (q != nullptr) || (q != nullptr) != (e != nullptr) || !dy || !mean || !rstd || ((dgamma || dbeta) && !ws)) return URSA_ENULL;
+    if ((x != nullptr) == (q != nullptr) || (q != nullptr) != (e != nullptr) || !dy || !mean || !rstd || ((dgamma || dbeta) && ursa_layer_norm_ws_floats(M, D) && !ws)) return URSA_ENULL;
     const uintptr_t es = (uintptr_t)element_size(dtype) - 1, ps = (uintptr_t)element_size(pdtype) - 1;
     if (((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dz | (uintptr_t)dx) & es || ((uintptr_t)gamma | (uintptr_t)dgamma | (uintptr_t)dbeta) & ps ||
         ((uintptr_t)mean | (uintptr_t)rstd | (uintptr_t)ws) & 3 || (uintptr_t)q & 15) return URSA_EALIGN;
