@@ -234,3 +234,27 @@ def test_column_sums_of_long_rows(dtype, M, D):
             B.check(dict(dg=dg, db=db), want, bound, where=(dtype, M, D, pt))
             assert torch.equal(k.layer_norm_backward(dy, stats, gamma, need_dx=False, need_dgamma=True, **source)[1], dg)
             assert torch.equal(k.layer_norm_backward(dy, stats, gamma, need_dx=False, need_dbeta=True, **source)[2], db)
+
+
+# ---- the roundings of a 16-bit layer's gradients ------------------------------------------------
+@pytest.mark.parametrize('dtype,act', [('bfloat16', 'gelu'), ('bfloat16', 'silu'), ('float16', 'gelu'), ('float16', 'silu')])
+@pytest.mark.parametrize('M,K,N', [(300, 200, 333), (2048, 1024, 2048)])
+def test_gradients_carry_the_rounding_of_z_of_dz_and_their_own(M, K, N, dtype, act):
+    """Against the formula with z and dz rounded to the type, dx and dW are off by one rounding - the root of the mean square of the
+    result's own, and no third one. An fp32 sum that ends beside a tie of z or dz may round to the other side: a sum's error is 2^-20 of
+    its scale at most, which moves 2^-12 of the elements (bf16; fp16: 2^-9) by a step, 1 / sqrt(12) of which is a rounding's root mean
+    square: sqrt(1 + 12 x 2^-9) of it together, and two operands so: 5 % in all."""
+    from ursabench_amd import _native
+    k, t = _native.default_kernels(), B.TYPES[dtype]
+    g = torch.Generator(device=DEV).manual_seed(M)
+    x, dy = torch.randn(M, K, generator=g, device=DEV).to(t), (torch.randn(M, N, generator=g, device=DEV) / M ** 0.5).to(t)
+    w, b = ((2 * torch.rand(*s, generator=g, device=DEV) - 1) / K ** 0.5 for s in ((N, K), (N,)))
+    w, b = w.to(t), b.to(t)
+    once = lambda v: v.to(t).double()                                            # noqa: E731
+    z = once(x.double() @ w.double().t() + b.double())
+    _, kept = k.linear_act(x, w, b, activation=act, save_z=True)
+    exact = dy.double() * B.act(z, act)[1]
+    dz = once(exact)
+    got = k.linear_backward(dy, x, w, kept, activation=act)
+    for v, want in zip(got, (dz @ w.double(), dz.t() @ x.double(), exact.sum(0))):
+        assert float((v.double() - want).norm()) <= 1.05 * float((once(want) - want).norm())

@@ -257,7 +257,8 @@ __device__ __forceinline__ void sums_again(f32x4 (&acc)[FY][FX], const Operand& 
     }
 }
 
-// C consecutive n of one m through the epilogue; `bias`: those of the bias, or zeros
+// C consecutive n of one m through the epilogue; `bias`: those of the bias, or zeros. z is kept in the tensors' type: half the bytes of
+// fp32 to write, hold and read again, for a slope that is off by that rounding of z (gradients 1.66e-3 -> 1.77e-3, bf16 gelu).
 template <typename T, int C>
 __device__ __forceinline__ void finish(const Epilogue& ep, int64_t m, int n, int N, float (&v)[C], const float (&bias)[C]) {
     const int valid = N - n;
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(256) void k_product(Operand X, Operand Y, Shape s, 
 
 // ---- 256 x 256 outputs by eight waves, 16-bit operands straight from memory to LDS ------------------------------------------
 // A wave owns 128 x 64 outputs (32 accumulators of 16 x 16, two waves on each SIMD): 12 fragment reads feed 32 matrix instructions
-// (bf16 8192^3: 1380 TFLOP/s forward, matrix pipe busy 0.69 of the cycles at the 1.77 GHz that the power allows, LDS 0.26). The
+// (bf16 8192^3: 1330 TFLOP/s each way, matrix pipe busy 0.69 of the cycles at the 1.77 GHz that the power allows, LDS 0.27). The
 // fragments of the next 32 k are read while the present ones are multiplied. Two stages of 64 k in LDS: as soon as every wave has its
 // last fragments of a stage, the pieces of the stage after the next start from memory to LDS, past the registers, and have a whole
 // stage's time to arrive. A wave's 64 pieces land side by side, so what spreads the banks is a permutation of the addresses that they
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(R == 256 ? 512 : 256, 2) void k_product_wide(Operan
 // A wave owns 64 x 64 outputs; 24 fragment reads (three planes of each operand) feed 96 matrix instructions. Two stages of 32 k: while
 // one is multiplied, the numbers of the next, which are in registers already, are split and stored to the other, and those of the
 // one after it are fetched; one barrier a stage. 24 numbers a thread and stage take about 220 vector instructions, beside the matrix
-// instructions of both waves of the SIMD (4096^3: 222 TFLOP/s, matrix pipe busy 0.59 of the cycles at 1.95 GHz; the two waves in
+// instructions of both waves of the SIMD (4096^3: 217 TFLOP/s, matrix pipe busy 0.59 of the cycles at 1.9 GHz; the two waves in
 // opposite phases, one staging while the other multiplies, measured the same). Buffer loads, as above; rows of at most 2^21 numbers,
 // kFlat ones a multiple of 8.
 constexpr int kSplitM = 256, kSplitN = 128, kSplitK = 32, kSplitThreads = 512;
@@ -772,7 +773,7 @@ __global__ __launch_bounds__(kSplitThreads, 2) void k_product_split(Operand X, O
 // ---- few rows: y for M <= 16 MT, the weights read once ----------------------------------------------------------------------
 // Bound by the weights' bytes. A workgroup owns 16 features; its waves take turns at 32 kAhead k, whose pieces of 16 rows of W it
 // fetches together, straight into the registers of the matrix instruction - no LDS on the way, no barrier until the waves' sums
-// are added up, in their order, by LDS (one row, 4096 x 4096 bf16: 8.2 us, 4.1 TB/s). fp32: the fp32 instruction, eight times for
+// are added up, in their order, by LDS (one row, 4096 x 4096 bf16: 8.5 us, 3.9 TB/s). fp32: the fp32 instruction, eight times for
 // 32 k (lane l has k = 8 (l / 16) + i for the i-th, in both operands); there is time for it beside the loads, and the split would cost
 // more vector work than that.
 template <typename T, int MT, int WAVES>
@@ -872,7 +873,10 @@ __global__ __launch_bounds__(256) void k_join(Shape s, Epilogue ep) {
 // dz = dy act'(z) and the slices' sums of its columns: one pass, bound by its bytes. A workgroup: PIECES column pieces x 256 / PIECES
 // rows at a time, the loads of kRows of those together. 32 pieces; 8 where one slice has all rows, so that the activation's
 // arithmetic is spread over more workgroups (gelu, 128 x 200 fp16: 14.9 -> 7.8 us, 256 x 4096 bf16: 28.7 -> 9.0). 8192 x 8192 bf16,
-// gelu, from memory: 100 us for 402 MB, 4 TB/s.
+// gelu, from memory: 102 us for 402 MB, 3.9 TB/s.
+// dz is rounded to the tensors' type: it is the matrix instruction's operand, and a second part of it would double both products (8192 x
+// 2048 -> 8192 bf16: 470 us more of 795). dx and dW are then off by two roundings, dz's and their own, where the sums alone would leave
+// one: relative L2 2.42e-3 against 1.66e-3 in bf16, 3.0e-4 against 2.1e-4 in fp16 - as the stock ops of the type are. db has dz in fp32.
 constexpr int kRows = 4;
 
 // V elements from p as they are in memory, of which `room` are the tensor's: past a row's end those of the next one, whose sums are
@@ -959,14 +963,18 @@ struct Plan {
 
 // The form, by the number of workgroups that it gives the 256 CUs, and the cut of the contraction where there are fewer than one
 // (two of the smaller forms) for each: at most 16 slices of at least eight k steps. `wide`: the operands suit the large forms (see
-// there); `packed`: one of them comes in 8 bits. Measured, both sides of each border:
-//   16 bits, 256 x 256 from 192 tiles on: 8192 x 1024 outputs, K 4096 (128 tiles): 64 us in 128 x 128, 79 cut in two;
-//            8192 x 8192, K 2048: 219 against 267. With an operand in 8 bits, whose conversion the larger tile halves, also cut:
-//            1024 x 4096, K 8192: 97 against 118
-//   16 bits, 128 x 128 where they reach 256 workgroups, cut in four at most: 2048^3: 28 us against 37 in 64 x 64; 1024^3 (too few):
-//            16.8 against 14.6. Two workgroups a CU where each has 48 steps left: 1024 x 4096, K 8192: 79 us against 92
-//   fp32, 256 x 128 where they reach 192 workgroups, cut from 96 tiles or K 2048 on: 1024 x 1024 outputs, K 4096: 64 us against 93;
-//            4096 x 1024, K 1024: 62 against 66; 2048 x 1024, K 1024 (64 tiles): 44 against 40 in 64 x 64; 1024^3: 34 against 29
+// there); `packed`: one of them comes in 8 bits. Measured, both sides of each border (us; more points in profiles/dense_borders.txt):
+//   16 bits, 256 x 256 from 192 tiles on: 8192 x 1024 outputs, K 4096 (128 tiles): 92, cut in two 82, in 128 x 128 67; x 1280 (160
+//            tiles, the one point where the other form is ahead): 89 against 104; x 1536 (192): 93 against 107; 8192 x 8192, K 2048:
+//            224 against 277. With an operand in 8 bits, whose conversion the larger tile halves, also cut: 1024 x 4096, K 8192: 93
+//            against 104; 2048 x 2048, K 4096: 63 against 64
+//   16 bits, 128 x 128 where they reach 256 workgroups, cut in four at most: 2048^3: 28 against 34 in 64 x 64; 2048 x 1536, K 1024
+//            (192, too few): 14.9 against 16.7; 1024^3 (64): 13.5 against 10.3. A cut form costs its join: 2048 x 1024, K 2048 in two 25
+//            against 21 in 64 x 64. Two workgroups a CU where each has 48 steps left: 1024 x 4096, K 8192: 79 against 90, K 6144: 64
+//            against 68; K 4096 (32 steps): 50 against 47
+//   fp32, 256 x 128 where they reach 192 workgroups, cut from 96 tiles or K 2048 on: 1024 x 1024 outputs, K 4096: 65 against 75 in
+//            64 x 64; 4096 x 1024, K 1024 (128 tiles): 63 - 66 against 63; 2048 x 1536 (96): 55 against 49; 2048 x 1024 (64): 42 against
+//            37; 1024^3: 34 against 28; uncut 4096 x 2048, K 512 (256): 53 against 62, x 1536 (192): 46 against 49
 Plan plan_of(int64_t M, int64_t N, int64_t K, int32_t dtype, bool wide, bool packed) {
     Plan p;
     const int bk = dtype == URSA_F32 ? 32 : 64;

@@ -14,7 +14,7 @@
 // fp32. A row belongs to TPR threads (16 for the narrowest, so that a wave holds four rows; one wave; one workgroup), CV values
 // per thread. dgamma / dbeta: a workgroup walks rows with a fixed stride and keeps its columns' sums in registers, stores them
 // once, and a second launch adds the workgroups' sums in a fixed order - no atomics, the same bits every time.
-// 16,384 x 4,096 bf16: the sum and its norm 107 us (537 MB, 5.0 TB/s), backward with a gradient past the norm 125 us (4.3 TB/s; a
+// 16,384 x 4,096 bf16: the sum and its norm 108 us (537 MB, 5.0 TB/s), backward with a gradient past the norm 135 us (4.0 TB/s; a
 // large copy moves 4.8). One row: the launch, 5 us up to 16,384 features. A longer one does not fit a workgroup's registers and is
 // walked three times (twice) by one workgroup: 20,000 features 12 us forward and 21 backward, 2^20 417 and 707; 512 rows of 2^17
 // bf16 121 and 290 us (dgamma / dbeta 82 of them).
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256) void k_norm_join(const float* __restrict__ par
     if (out) out[j < D ? j : j - D] = (P)acc;
 }
 
-// one pass each way, 16 bytes of x a thread and turn: 8192 x 4096 bf16 (102 MB) 20 us to pack, 21 to unpack
+// one pass each way, 16 bytes of x a thread and turn: 8192 x 4096 bf16 (102 MB) 20 us to pack, 22 to unpack
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, int8_t* __restrict__ q, int8_t* __restrict__ e, int64_t M, int64_t D, int64_t qpitch) {
     constexpr int V = Piece<T>::kN;
@@ -489,7 +489,7 @@ dim3 grid_of(int64_t blocks) {
 }
 
 // Threads of a row in the backward's walk: 8 columns each, so that their sums leave registers for many waves (with 16 or 32 a CU holds
-// few, and 16,384 x 4,096 bf16 with a gradient past the norm took 197 us instead of 125). Above 8,192: 16 columns.
+// few, and 16,384 x 4,096 bf16 with a gradient past the norm took 1.6 times as long). Above 8,192: 16 columns.
 int bwd_row_threads(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 
 // Workgroups of the walk: 1,024 threads a CU, and no more than leave each row slot four rows, so that the partial sums (2 D floats
