@@ -59,7 +59,8 @@ def _fusable(fc, w, b, x, residual):
     return (_on and x.is_cuda and t in _native.DTYPES and x.dim() >= 1 and not torch.is_autocast_enabled()
             and type(fc).forward is nn.Linear.forward and 'forward' not in fc.__dict__ and not _has_any_global_hook()
             and not (fc._forward_hooks or fc._forward_pre_hooks or fc._backward_hooks or fc._backward_pre_hooks)
-            and type(x) in _TENSORS and type(w) in _TENSORS and type(residual) in _TENSORS and w.dtype is t and w.get_device() == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
+            and type(x) in _TENSORS and type(w) in _TENSORS and type(b) in _TENSORS and type(residual) in _TENSORS
+            and w.dtype is t and w.get_device() == dev and x.shape[-1] == w.shape[1] and w.numel() > 0
             and (b is None or (b.dtype is t and b.get_device() == dev))
             and (residual is None or (residual.dtype is t and residual.get_device() == dev)))
 

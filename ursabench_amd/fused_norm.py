@@ -44,7 +44,7 @@ def _fusable(ln, w, b, x):
     return (_on and x.is_cuda and t in _native.DTYPES and x.numel() > 0 and not torch.is_autocast_enabled()
             and type(ln).forward is nn.LayerNorm.forward and 'forward' not in ln.__dict__ and not _has_any_global_hook()
             and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks or ln._backward_pre_hooks)
-            and type(x) in _TENSORS and type(w) in _TENSORS and x.shape[-len(shape):] == shape and ln.eps >= 0
+            and type(x) in _TENSORS and type(w) in _TENSORS and type(b) in _TENSORS and x.shape[-len(shape):] == shape and ln.eps >= 0
             and (w is None or (w.get_device() == dev and (w.dtype is t or w.dtype is torch.float32)))
             and (b is None or (b.get_device() == dev and (b.dtype is t or b.dtype is torch.float32) and (w is None or w.dtype is b.dtype))))
 
