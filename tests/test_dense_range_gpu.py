@@ -209,6 +209,18 @@ def test_a_constant_gradient_moves_nothing(D):
     assert not dx.any() and not dg.any()
 
 
+@pytest.mark.parametrize('D', [64, 777, 5000, 20000])
+def test_fp32_rows_whose_variance_is_past_the_range(D):
+    """Squares above 2^128: the variance is infinite and 1 / sqrt of it 0, so y is the bias - not a NaN of two infinities."""
+    from ursabench_amd import _native
+    k = _native.default_kernels()
+    g = torch.Generator(device=DEV).manual_seed(D)
+    x = torch.randn(4, D, generator=g, device=DEV) * torch.tensor([1e20, 1e28, 1e33, 1.0], device=DEV)[:, None]
+    beta = torch.full((D,), 0.5, device=DEV)
+    _, y, stats, _, _ = k.layer_norm(x, torch.ones(D, device=DEV), beta, eps=1e-5, stats=True)
+    assert (y[:3] == 0.5).all() and not stats[1, :3].any() and y[3].isfinite().all() and stats[1, 3] > 0.5
+
+
 # ---- rows of a million features -----------------------------------------------------------------
 @pytest.mark.parametrize('dtype,M,D', [('float32', 3, 16385), ('bfloat16', 4, 20000), ('bfloat16', 40, 70001), ('float32', 9, 2 ** 20 + 5), ('float16', 40, 2 ** 20 + 5),
                                        ('bfloat16', 6, 4500001), ('float32', 2, 4500000)])

@@ -55,9 +55,10 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float* red) {
     return make_float2(a, b);
 }
 
-// 1 / sqrt of the variance around m + rest; rounding may leave a constant row's below zero (a NaN stays one)
+// 1 / sqrt of the variance around m + rest; rounding may leave a constant row's below zero. Past the range it is infinite (rest^2 may
+// be, too), and a NaN stays one.
 __device__ __forceinline__ float inverse_deviation(float mean_square, float rest, float eps) {
-    const float var = mean_square - rest * rest;
+    const float var = mean_square < INFINITY ? mean_square - rest * rest : mean_square;
     return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);
 }
 
