@@ -10,7 +10,9 @@ launches differ:
 float32, bfloat16 and float16, any sizes and leading dimensions, on a HIP device. Operands that are not contiguous are copied first.
 Anything else - host tensors, other or mixed types, autocast, a class or an instance with a forward of its own, hooks on `fc` or on
 all modules, tensor subclasses, `torch.func` transforms, forward-mode derivatives, dispatch modes and tracing - takes `fc(x)`, the
-activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises. On a HIP tensor the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
+activation and the sum as stock ops, where `save8` keeps x itself. Double backward raises, and so do batched (`is_grads_batched`) and
+dual gradients in the backward pass. On a HIP tensor the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd
+nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the x that the weight gradient needs in 8 bits (K17, `act8`) instead of the tensor: a quarter / half of its
 memory, dW as if x had been rounded to 8 bits per block of 32 features; y, dx and db do not change.

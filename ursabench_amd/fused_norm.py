@@ -9,9 +9,11 @@ convolutional blocks, for networks that normalise each row by itself.
                     small one that adds those in a fixed order
 
 float32, bfloat16 and float16 on a HIP device, parameters of the same type or float32, any width. Inputs that are not contiguous are
-copied first. Anything else - host tensors, other types, autocast, empty tensors, a class or an instance with a forward of its own, hooks on
-`ln` or on all modules, tensor subclasses, `torch.func` transforms, forward-mode derivatives, dispatch modes and tracing - takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward raises. On a HIP tensor
-the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd nodes (no silent fallback: a missing library raises).
+copied first. Anything else - host tensors, other types, autocast, empty tensors, a class or an instance with a forward of its own,
+hooks on `ln` or on all modules, tensor subclasses, `torch.func` transforms, forward-mode derivatives, dispatch modes and tracing -
+takes `ln(x)`, the stock path, where `save8` keeps the input itself. Double backward raises, and so do batched (`is_grads_batched`) and
+dual gradients in the backward pass. On a HIP tensor the fused path needs csrc/libursa_hip.so and csrc/_ursa_torch.so, its autograd
+nodes (no silent fallback: a missing library raises).
 
 `save8=True` keeps the normalised input in 8 bits for the backward pass (K17, `act8`): gradients are the formula's with xhat
 taken from those values; mean and 1 / std are the exact input's. `URSA_FUSED_NORM=0` / `enabled(False)` selects the stock path
